@@ -757,6 +757,93 @@ int nsp_lstm_cell_fwd(const float* gates, const float* c_prev, float* h, float* 
 int nsp_lstm_cell_bwd(const float* dh, const float* dc_next, const float* gates, const float* c_prev, const float* c,
                       float* dgates, float* dc_prev, int B, int H, void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * Decoder operators: attention of new tokens over a cache or over encoder     *
+ * states, the append to a paged cache, sampling.  The parameter structs hold   *
+ * 8-byte fields only (one struct.pack on the Python side); strides count       *
+ * elements, the last dimension of every tensor is contiguous, rows are 16-byte *
+ * aligned and all strides multiples of 8 elements.  D % 8 == 0, D <= 128.      *
+ *                                                                              *
+ * nsp_decode_attn: out[b,t,h,:] = sum_j p_j v_j, p = softmax_j(scale q[b,t,h] . *
+ *   k_j), j < lens[b]; query head h reads key head h / (H / Hkv).              *
+ *   table != NULL: keys are slots j % page of page table[b][j / page] of        *
+ *     k / v = [n_pages, Hkv, page, D] (strides *_sp, *_sh, *_ss); width =       *
+ *     entries of a table row.  k_new / v_new [B,Hkv,D] (or both NULL): stored    *
+ *     at position lens[b] and attended to as well.  A sequence without a key     *
+ *     gets zeros; lens[b] < 0 marks an unused row (zeros, nothing stored);       *
+ *     lens[b] > width * page counts as that; keys of a page outside [0, n_pages) *
+ *     count as absent, and a new token whose page is outside, or whose position  *
+ *     is behind the table, is neither stored nor attended to.                    *
+ *   table == NULL: k / v = [B, width, Hkv, D] (strides *_sp per sequence, *_ss    *
+ *     per key, *_sh per head), lens may be NULL (= width).  lens[b] <= 0: all      *
+ *     `width` keys alike, as the training softmax has it with its finite mask.     *
+ *   out [B,Tq,H,D] contiguous.  dtype (NSP_DT_*) is that of every tensor.          *
+ *   ws: nsp_decode_attn_workspace_bytes(..., cap = width * page resp. width) bytes, *
+ *     may be NULL if that is 0; contents need not survive the call.                 *
+ * nsp_paged_append: k / v [B,n,Hkv,D]; token t < min(n, counts[b]) of row b goes to  *
+ *   position starts[b] + t (counts may be NULL: all n; starts[b] < 0: none); fp32     *
+ *   rounds to the cache's bf16 (nearest even).  What has no valid page or lies behind  *
+ *   the table is dropped.                                                              *
+ * nsp_sample_rows: see sample.hip for the definition.  x [rows, V] with row pitch ld,   *
+ *   u [rows] in [0,1); temperature / top_k / top_p / min_p are per row if their pointer  *
+ *   is set, else the *_all value; out int32 [rows].  V <= 2^18.                           *
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  const void* q; void* out;
+  const void* k; const void* v;
+  const int* table; const int* lens;
+  const void* k_new; const void* v_new;
+  float* ws;
+  long long B, H, Hkv, D, Tq, page, n_pages, width, dtype;
+  long long q_sb, q_st, q_sh;
+  long long k_sp, k_ss, k_sh;
+  long long v_sp, v_ss, v_sh;
+  long long kn_sb, kn_sh, vn_sb, vn_sh;
+  double scale;
+} nsp_decode_attn_params;
+long long nsp_decode_attn_workspace_bytes(int B, int H, int Hkv, int Tq, int D, int cap);
+int nsp_decode_attn(const nsp_decode_attn_params* p, void* stream);
+
+typedef struct {
+  const void* k; const void* v; void* k_pages; void* v_pages;
+  const int* table; const int* starts; const int* counts;
+  long long B, n, Hkv, D, page, n_pages, width, src_dtype, dtype;
+  long long k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  long long kp_sp, kp_ss, kp_sh, vp_sp, vp_ss, vp_sh;
+} nsp_paged_append_params;
+int nsp_paged_append(const nsp_paged_append_params* p, void* stream);
+
+typedef struct {
+  const void* x; const float* u;
+  const float* temperature; const int* top_k; const float* top_p; const float* min_p;
+  int* out;
+  long long rows, V, ld, dtype, k_all;
+  double t_all, tp_all, mp_all;
+} nsp_sample_params;
+int nsp_sample_rows(const nsp_sample_params* p, void* stream);
+
+/* nsp_cross_attn_fwd / _bwd: out[b,i,h,:] = sum_j dropout(p_ij) v_j, p = softmax_j(scale q[b,i,h] . k[b,j,h / (H / Hkv)]) over
+ *   j < klens[b] (klens NULL: all Tk; klens[b] <= 0: all Tk keys alike and no gradient through the scores).  q [B,Tq,H,D],
+ *   k / v [B,Tk,Hkv,D] and dout (strides g_*) as above; out, o_lo, dq [B,Tq,H,D] and dk, dv [B,Tk,Hkv,D] contiguous, all of type
+ *   dtype.  Training: fwd also fills stats [2][B,H,Tq] fp32 and, for bf16, o_lo (what the rounding of out left; both NULL for
+ *   inference); bwd reads out, o_lo, stats, uses dsum [B,H,Tq] fp32 as scratch and writes dq, dk, dv completely.
+ *   dropout: element (b,h,i,j) is kept as nsp_attn_softmax_fwd keeps it: counter offset + ((b H + h) Tq + i) Tk + j.
+ *   scale > 0.  Tq == 0 or Tk == 0: nothing is written. */
+typedef struct {
+  const void* q; const void* k; const void* v; const void* dout;
+  void* out; void* o_lo; void* dq; void* dk; void* dv;
+  float* stats; float* dsum; const int* klens;
+  long long B, H, Hkv, D, Tq, Tk, dtype;
+  long long q_sb, q_st, q_sh;
+  long long k_sb, k_st, k_sh;
+  long long v_sb, v_st, v_sh;
+  long long g_sb, g_st, g_sh;
+  unsigned long long seed, offset;
+  double scale, dropout_p;
+} nsp_cross_attn_params;
+int nsp_cross_attn_fwd(const nsp_cross_attn_params* p, void* stream);
+int nsp_cross_attn_bwd(const nsp_cross_attn_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,608 @@
+// cross_attn.hip -- attention of target tokens over encoder states of another length, forward and backward.
+//
+//   S = scale Q K^T,  P = softmax over the keys j < klens[b],  O = dropout(P) V
+//   dV = dropout(P)^T dO,  dP = dropout'(dO V^T),  D_i = sum_d dO_id O_id,  dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q
+//
+// No score leaves the compute unit.  All three kernels are one loop: a wave owns 16 (NQ x 16) rows whose operands stay in
+// registers, a workgroup of four waves streams tiles of the other side's rows through LDS (LDS-DMA, double buffered, one
+// barrier per tile), and the score tile is computed with the OWNED row on the lane's column: row statistics are per lane, and
+// the probabilities already are the operand of the second product -- their contraction runs over the streamed rows, four of
+// which a lane holds per 16.
+//   forward   owns queries, streams K and V;   O^T += V^T P^T
+//   dQ        owns queries, streams K and V;   dQ^T += K^T dS^T; also D, which it leaves for
+//   dK / dV   owns keys, streams Q and dO (of every query head of the key head: shared heads are summed in registers, in a
+//             fixed order);                    dV^T += dO^T P, dK^T += Q^T dS
+// The second operand of those products has the STREAMED row as contraction, i.e. wants a tile read across its rows: bf16 takes
+// it with the transposing LDS read (ds_read_b64_tr_b16), fp32 holds one contraction element per lane and instruction and
+// just picks the row.
+// The softmax is kept as its maximum (log2 domain) and the reciprocal of its sum, both fp32; backward recomputes P from them.
+// bf16 roundings inside: P resp. dS, once each, as operands of the second products (their error, 2^-9 rms 2^-10, is that of the
+// output's own rounding); O is kept for D as two bf16 parts (16 bits) because D is subtracted from dP.
+// A row without a visible key is uniform over all Tk keys, as with the finite mask value of attn_softmax_fwd, and passes no
+// gradient through its scores.  Keys behind klens are never read.
+#include "attn_frag.h"
+
+namespace {
+
+struct XArgs {
+  const void *q, *k, *v, *dout;
+  void *out, *o_lo, *dq, *dk, *dv;
+  float* stats;        // [2][B,H,Tq]: maximum, 1 / sum
+  float* dsum;         // [B,H,Tq]
+  const int* klens;
+  int B, H, Hkv, D, Tq, Tk;
+  long long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
+  unsigned long long seed, offset;
+  float scale, sl2, drop;
+};
+
+typedef __attribute__((address_space(3))) bf16x4 x_lds_bf16x4;
+typedef __attribute__((address_space(3))) void x_lds_void;
+typedef const __attribute__((address_space(1))) void x_glb_void;
+
+// ---- a tile: KT rows of DP elements, 16-byte chunks XOR-swizzled by the row (unpadded: the DMA writes lane-linear)
+template <typename T, int DP>
+struct XTile {
+  typedef AttnElem<T> E;
+  static constexpr int KT = sizeof(T) == 2 ? 64 : 32;
+  static constexpr int RB = DP * (int)sizeof(T);     // bytes of a row
+  static constexpr int CPR = RB / 16;                // chunks of a row
+  static constexpr int NS = CPR / 4;                 // steps of a product over the head size
+  static constexpr int NB = DP / 16;                 // 16-row blocks of a transposed accumulator
+  static constexpr int BYTES = KT * RB;
+  __device__ static __forceinline__ int swz(int row) { return RB >= 128 ? (row & 7) : ((row >> 1) & 3); }
+  // rows row0 .. row0 + KT - 1 of src (limit > 0 rows; later ones re-read the last) into LDS
+  __device__ static __forceinline__ void dma(unsigned char* tile, const T* src, long long ld, int row0, int limit, int chunks,
+                                             int wave, int lane) {
+    constexpr int PIECES = BYTES / 1024;             // 1 KB = one instruction of a wave
+#pragma unroll
+    for (int i = 0; i < PIECES / 4; ++i) {
+      const int piece = wave * (PIECES / 4) + i;
+      const int row = piece * (64 / CPR) + lane / CPR, c = lane % CPR;
+      int sc = c ^ swz(row);
+      sc = min(sc, chunks - 1);                      // (head sizes below DP: the owned operand is zero there)
+      const T* p = src + (long long)min(row0 + row, limit - 1) * ld + sc * E::CE;
+      __builtin_amdgcn_global_load_lds((x_glb_void*)p, (x_lds_void*)(tile + piece * 1024), 16, 0, 0);
+    }
+  }
+  // operand of a product over the head size: chunk 4 s + g of row rbase + r
+  __device__ static __forceinline__ typename E::chunk rows(const unsigned char* tile, int rbase, int s, int r, int g) {
+    const int row = rbase + r;
+    return *reinterpret_cast<const typename E::chunk*>(tile + row * RB + (((4 * s + g) ^ swz(row)) << 4));
+  }
+};
+
+// acc[blk] (rows: dimension x_dim(blk, g, e), column: owned row) += tile^T w for all KT rows of the tile; w[kf][e] = weight of
+// row 16 kf + 4 g + e
+template <int DP, int N>
+__device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], const unsigned char* tile, const f32x4 (&w)[N][2],
+                                             float, int r, int g) {
+  typedef XTile<float, DP> X;
+  constexpr int VW = DP / 16;
+#pragma unroll
+  for (int kf = 0; kf < X::KT / 16; ++kf)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = 16 * kf + 4 * g + e;
+      const float* base = reinterpret_cast<const float*>(tile + row * X::RB);
+      float x[VW];
+#pragma unroll
+      for (int i = 0; i < VW; i += (VW < 4 ? VW : 4)) {
+        const int el = r * VW + i, c = el >> 2;
+        const float* p = base + ((c ^ X::swz(row)) << 2) + (el & 3);
+        if constexpr (VW == 2) {
+          const float2 a = *reinterpret_cast<const float2*>(p);
+          x[0] = a.x; x[1] = a.y;
+        } else {
+          const f32x4 a = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i + j] = a[j];
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < N; ++f)
+#pragma unroll
+        for (int j = 0; j < VW; ++j) acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], w[f][kf][e], acc[f][j], 0, 0, 0);
+    }
+}
+
+// four transposed fragments (16 dimensions each, 32 rows): eight reads and their wait in ONE statement, so that no other
+// instruction can touch a destination in between.  (The builtin is modelled as reading memory that an LDS-DMA in flight
+// may write: hipcc would wait for the next tile's DMA in front of it.)
+template <int DP>
+__device__ __forceinline__ const unsigned char* x_tr_addr(const unsigned char* tile, int row, int cbase, int r) {
+  typedef XTile<__bf16, DP> X;
+  const int b = r & 3, c = (cbase >> 3) + (b >> 1);
+  return tile + row * X::RB + ((c ^ X::swz(row)) << 4) + (b & 1) * 8;
+}
+template <int DP, int NF>
+__device__ __forceinline__ void x_tr_read(bf16x8 (&out)[NF], const unsigned char* tile, int d0, int k0, int r, int g) {
+  const int ra = k0 + 4 * g + (r >> 2), rb = ra + 16;
+  bf16x4 lo[NF], hi[NF];
+#ifdef NSP_HOST_EMULATION
+  for (int i = 0; i < NF; ++i) {
+    lo[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)x_tr_addr<DP>(tile, ra, d0 + 16 * i, r));
+    hi[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)x_tr_addr<DP>(tile, rb, d0 + 16 * i, r));
+  }
+#else
+  typedef __attribute__((address_space(3))) unsigned char lds_uchar;
+  unsigned a[2 * NF];
+#pragma unroll
+  for (int i = 0; i < NF; ++i) {
+    a[2 * i] = (unsigned)(uintptr_t)((lds_uchar*)const_cast<unsigned char*>(x_tr_addr<DP>(tile, ra, d0 + 16 * i, r)));
+    a[2 * i + 1] = (unsigned)(uintptr_t)((lds_uchar*)const_cast<unsigned char*>(x_tr_addr<DP>(tile, rb, d0 + 16 * i, r)));
+  }
+  if constexpr (NF == 2)
+    asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %6\n\t"
+                 "ds_read_b64_tr_b16 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3])
+                 : "memory");
+  else
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %10\n\t"
+                 "ds_read_b64_tr_b16 %3, %11\n\tds_read_b64_tr_b16 %4, %12\n\tds_read_b64_tr_b16 %5, %13\n\t"
+                 "ds_read_b64_tr_b16 %6, %14\n\tds_read_b64_tr_b16 %7, %15\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7])
+                 : "memory");
+#endif
+#pragma unroll
+  for (int i = 0; i < NF; ++i) out[i] = __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int DP, int N>
+__device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], const unsigned char* tile, const f32x4 (&w)[N][4],
+                                             __bf16, int r, int g) {
+  constexpr int NF = DP == 32 ? 2 : 4;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    bf16x8 p[N];
+#pragma unroll
+    for (int f = 0; f < N; ++f)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[f][i] = (__bf16)w[f][2 * u + (i >> 2)][i & 3];
+#pragma unroll
+    for (int d0 = 0; d0 < DP; d0 += 16 * NF) {
+      bf16x8 t[NF];
+      x_tr_read<DP, NF>(t, tile, d0, 32 * u, r, g);
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int f = 0; f < N; ++f)
+          acc[f][d0 / 16 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t[i], p[f], acc[f][d0 / 16 + i], 0, 0, 0);
+    }
+  }
+}
+
+// row `dst` (D elements) <- a transposed accumulator's column, times f; LO: what the rounding to T left, as T
+template <int DP, bool LO>
+__device__ __forceinline__ void x_store(float* dst, const f32x4 (&acc)[DP / 16], float f, int D, int g) {
+  constexpr int VW = DP / 16;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int d = (4 * g + e) * VW;
+    if (d >= D) continue;
+    if constexpr (VW == 2) {
+      *reinterpret_cast<float2*>(dst + d) = make_float2(acc[0][e] * f, acc[1][e] * f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VW; i += 4)
+        *reinterpret_cast<f32x4*>(dst + d + i) = f32x4{acc[i][e] * f, acc[i + 1][e] * f, acc[i + 2][e] * f, acc[i + 3][e] * f};
+    }
+  }
+}
+template <int DP, bool LO>
+__device__ __forceinline__ void x_store(__bf16* dst, const f32x4 (&acc)[DP / 16], float f, int D, int g) {
+#pragma unroll
+  for (int blk = 0; blk < DP / 16; ++blk) {
+    const int d = 16 * blk + 4 * g;
+    if (d >= D) continue;
+    bf16x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = acc[blk][e] * f;
+      x[e] = (__bf16)v;
+      if (LO) x[e] = (__bf16)(v - (float)x[e]);
+    }
+    *reinterpret_cast<bf16x4*>(dst + d) = x;
+  }
+}
+
+// which (sequence, key head, query head of the group, row tile) a workgroup takes: workgroups go round the eight XCDs in
+// turn, and all the ones that stream the same rows are put on one of them, one after the other
+__device__ __forceinline__ bool x_place(int groups, int per, int& grp, int& item) {
+  const int id = (int)blockIdx.x, i = id >> 3;
+  grp = (i / per) * 8 + (id & 7);
+  item = i % per;
+  return grp < groups;
+}
+
+template <typename T, int N, int NS>
+__device__ __forceinline__ void x_load_rows(typename AttnElem<T>::chunk (&f)[N][NS], const T* base, long long ld, int row0,
+                                            int limit, int D, int r, int g) {
+  typedef AttnElem<T> E;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const T* p = base + (long long)min(row0 + 16 * i + r, limit - 1) * ld;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int c = (4 * s + g) * E::CE;
+      f[i][s] = c < D ? *reinterpret_cast<const typename E::chunk*>(p + c) : E::zero();
+    }
+  }
+}
+
+// score tile: s[f][kf] rows = streamed rows 16 kf + 4 g + e, column = owned row
+template <typename T, int DP, int N, int KF, int NS>
+__device__ __forceinline__ void x_product(f32x4 (&s)[N][KF], const unsigned char* tile,
+                                          const typename AttnElem<T>::chunk (&own)[N][NS], int r, int g) {
+  typedef XTile<T, DP> X;
+#pragma unroll
+  for (int kf = 0; kf < KF; ++kf) {
+#pragma unroll
+    for (int f = 0; f < N; ++f) s[f][kf] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const auto a = X::rows(tile, 16 * kf, i, r, g);
+#pragma unroll
+      for (int f = 0; f < N; ++f) s[f][kf] = AttnElem<T>::mma(a, own[f][i], s[f][kf]);
+    }
+  }
+}
+
+template <typename T, int DP, int NQ, bool DROP>
+__global__ __launch_bounds__(256) void cross_fwd_kernel(const XArgs p) {
+  typedef XTile<T, DP> X;
+  constexpr int KF = X::KT / 16;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int G = p.H / p.Hkv, nqt = (p.Tq + 64 * NQ - 1) / (64 * NQ);
+  int grp, item;
+  if (!x_place(p.B * p.Hkv, G * nqt, grp, item)) return;
+  const int b = grp / p.Hkv, hkv = grp % p.Hkv, h = hkv * G + item / nqt;
+  const int q0 = (item % nqt) * (64 * NQ) + wave * (16 * NQ);
+  int klen = p.klens ? min(p.klens[b], p.Tk) : p.Tk;
+  const bool uniform = klen <= 0;
+  if (uniform) klen = p.Tk;
+  const T* kb = reinterpret_cast<const T*>(p.k) + (long long)b * p.k_sb + (long long)hkv * p.k_sh;
+  const T* vb = reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh;
+  const int chunks = p.D / X::E::CE;
+  typename X::E::chunk Q[NQ][X::NS];
+  x_load_rows<T, NQ>(Q, reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)h * p.q_sh, p.q_st, q0, p.Tq,
+                         p.D, r, g);
+  f32x4 o[NQ][X::NB];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int f = 0; f < NQ; ++f) {
+#pragma unroll
+    for (int i = 0; i < X::NB; ++i) o[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[f] = -INFINITY;
+    l[f] = 0.f;
+  }
+  const int nkt = (klen + X::KT - 1) / X::KT;
+  X::dma(lds, kb, p.k_st, 0, klen, chunks, wave, lane);
+  X::dma(lds + X::BYTES, vb, p.v_st, 0, klen, chunks, wave, lane);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int kt = 0; kt < nkt; ++kt) {
+    const unsigned char* Kc = lds + (kt & 1) * (2 * X::BYTES);
+    if (kt + 1 < nkt) {     // the other buffers were last read in iteration kt - 1, behind that iteration's barrier
+      unsigned char* Kn = lds + ((kt + 1) & 1) * (2 * X::BYTES);
+      X::dma(Kn, kb, p.k_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
+      X::dma(Kn + X::BYTES, vb, p.v_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
+    }
+    f32x4 s[NQ][KF];
+    x_product<T, DP, NQ>(s, Kc, Q, r, g);
+    const bool whole = (kt + 1) * X::KT <= klen;
+#pragma unroll
+    for (int f = 0; f < NQ; ++f) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kf = 0; kf < KF; ++kf)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (uniform) s[f][kf][e] = 0.f;
+          if (!whole && kt * X::KT + 16 * kf + 4 * g + e >= klen) s[f][kf][e] = -INFINITY;
+          mx = fmaxf(mx, s[f][kf][e]);
+        }
+      // (scale > 0: the maximum commutes with it; a tile always has a visible key, so it is finite)
+      const float mn = fmaxf(m[f], attn_max4(mx) * p.sl2);
+      const float alpha = __builtin_amdgcn_exp2f(m[f] - mn);
+      m[f] = mn;
+      l[f] *= alpha;
+#pragma unroll
+      for (int i = 0; i < X::NB; ++i) o[f][i] *= alpha;
+      const int qi = min(q0 + 16 * f + r, p.Tq - 1);
+      const unsigned long long row =
+          DROP ? p.offset + (unsigned long long)((((long long)b * p.H + h) * p.Tq + qi) * p.Tk) : 0ull;
+#pragma unroll
+      for (int kf = 0; kf < KF; ++kf) {
+        float keep[4];
+        if constexpr (DROP) nsp_keep_scale4(p.seed, row + (unsigned long long)(kt * X::KT + 16 * kf + 4 * g), p.drop, keep);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -mn));
+          l[f] += x;
+          s[f][kf][e] = DROP ? x * keep[e] : x;
+        }
+      }
+    }
+    x_accumulate<DP, NQ>(o, Kc + X::BYTES, s, T(0), r, g);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+#pragma unroll
+  for (int f = 0; f < NQ; ++f) {
+    const float inv = 1.f / attn_sum4(l[f]);
+    const int qi = q0 + 16 * f + r;
+    if (qi >= p.Tq) continue;
+    const long long at = (((long long)b * p.Tq + qi) * p.H + h) * p.D;
+    x_store<DP, false>(reinterpret_cast<T*>(p.out) + at, o[f], inv, p.D, g);
+    if (p.o_lo) x_store<DP, true>(reinterpret_cast<T*>(p.o_lo) + at, o[f], inv, p.D, g);
+    if (p.stats && g == 0) {
+      const long long sr = ((long long)b * p.H + h) * p.Tq + qi;
+      p.stats[sr] = m[f];
+      p.stats[(long long)p.B * p.H * p.Tq + sr] = inv;
+    }
+  }
+}
+
+template <typename T, int DP, int NQ, bool DROP>
+__global__ __launch_bounds__(256) void cross_dq_kernel(const XArgs p) {
+  typedef XTile<T, DP> X;
+  constexpr int KF = X::KT / 16;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int G = p.H / p.Hkv, nqt = (p.Tq + 64 * NQ - 1) / (64 * NQ);
+  int grp, item;
+  if (!x_place(p.B * p.Hkv, G * nqt, grp, item)) return;
+  const int b = grp / p.Hkv, hkv = grp % p.Hkv, h = hkv * G + item / nqt;
+  const int q0 = (item % nqt) * (64 * NQ) + wave * (16 * NQ);
+  const int klen = p.klens ? min(p.klens[b], p.Tk) : p.Tk;
+  const T* kb = reinterpret_cast<const T*>(p.k) + (long long)b * p.k_sb + (long long)hkv * p.k_sh;
+  const T* vb = reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh;
+  const int chunks = p.D / X::E::CE;
+  const long long srow = ((long long)b * p.H + h) * p.Tq;
+  typename X::E::chunk Q[NQ][X::NS], dO[NQ][X::NS];
+  x_load_rows<T, NQ>(Q, reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)h * p.q_sh, p.q_st, q0, p.Tq,
+                         p.D, r, g);
+  x_load_rows<T, NQ>(dO, reinterpret_cast<const T*>(p.dout) + (long long)b * p.g_sb + (long long)h * p.g_sh, p.g_st, q0,
+                         p.Tq, p.D, r, g);
+  float m[NQ], inv[NQ], ds[NQ];
+  f32x4 acc[NQ][X::NB];
+  {
+    const long long orow = (long long)b * p.Tq * p.H * p.D + (long long)h * p.D;
+#pragma unroll
+    for (int f = 0; f < NQ; ++f) {
+      typename X::E::chunk O[1][X::NS];
+      float d = 0.f;
+      x_load_rows<T, 1>(O, reinterpret_cast<const T*>(p.out) + orow, (long long)p.H * p.D, q0 + 16 * f, p.Tq, p.D, r, g);
+#pragma unroll
+      for (int s = 0; s < X::NS; ++s)
+#pragma unroll
+        for (int e = 0; e < X::E::CE; ++e) d = fmaf((float)dO[f][s][e], (float)O[0][s][e], d);
+      if (p.o_lo) {
+        x_load_rows<T, 1>(O, reinterpret_cast<const T*>(p.o_lo) + orow, (long long)p.H * p.D, q0 + 16 * f, p.Tq, p.D, r, g);
+#pragma unroll
+        for (int s = 0; s < X::NS; ++s)
+#pragma unroll
+          for (int e = 0; e < X::E::CE; ++e) d = fmaf((float)dO[f][s][e], (float)O[0][s][e], d);
+      }
+      ds[f] = attn_sum4(d);
+      const int qi = min(q0 + 16 * f + r, p.Tq - 1);
+      m[f] = p.stats[srow + qi];
+      inv[f] = p.stats[(long long)p.B * p.H * p.Tq + srow + qi];
+      if (g == 0 && q0 + 16 * f + r < p.Tq) p.dsum[srow + qi] = ds[f];
+#pragma unroll
+      for (int i = 0; i < X::NB; ++i) acc[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  const int nkt = klen <= 0 ? 0 : (klen + X::KT - 1) / X::KT;     // no visible key: no gradient
+  if (nkt > 0) {
+    X::dma(lds, kb, p.k_st, 0, klen, chunks, wave, lane);
+    X::dma(lds + X::BYTES, vb, p.v_st, 0, klen, chunks, wave, lane);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int kt = 0; kt < nkt; ++kt) {
+    const unsigned char* Kc = lds + (kt & 1) * (2 * X::BYTES);
+    if (kt + 1 < nkt) {
+      unsigned char* Kn = lds + ((kt + 1) & 1) * (2 * X::BYTES);
+      X::dma(Kn, kb, p.k_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
+      X::dma(Kn + X::BYTES, vb, p.v_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
+    }
+    f32x4 s[NQ][KF], dp[NQ][KF];
+    x_product<T, DP, NQ>(s, Kc, Q, r, g);
+    x_product<T, DP, NQ>(dp, Kc + X::BYTES, dO, r, g);
+    const bool whole = (kt + 1) * X::KT <= klen;
+#pragma unroll
+    for (int f = 0; f < NQ; ++f) {
+      const int qi = min(q0 + 16 * f + r, p.Tq - 1);
+      const unsigned long long row = DROP ? p.offset + (unsigned long long)((srow + qi) * p.Tk) : 0ull;
+#pragma unroll
+      for (int kf = 0; kf < KF; ++kf) {
+        float keep[4];
+        if constexpr (DROP) nsp_keep_scale4(p.seed, row + (unsigned long long)(kt * X::KT + 16 * kf + 4 * g), p.drop, keep);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -m[f])) * inv[f];
+          const float dpe = DROP ? dp[f][kf][e] * keep[e] : dp[f][kf][e];
+          x *= dpe - ds[f];
+          if (!whole && kt * X::KT + 16 * kf + 4 * g + e >= klen) x = 0.f;
+          s[f][kf][e] = x;
+        }
+      }
+    }
+    x_accumulate<DP, NQ>(acc, Kc, s, T(0), r, g);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+#pragma unroll
+  for (int f = 0; f < NQ; ++f) {
+    const int qi = q0 + 16 * f + r;
+    if (qi < p.Tq)
+      x_store<DP, false>(reinterpret_cast<T*>(p.dq) + (((long long)b * p.Tq + qi) * p.H + h) * p.D, acc[f], p.scale, p.D, g);
+  }
+}
+
+template <typename T, int DP, bool DROP>
+__global__ __launch_bounds__(256) void cross_dkv_kernel(const XArgs p) {
+  typedef XTile<T, DP> X;
+  constexpr int QF = X::KT / 16;
+  // tiles, then per buffer KT maxima, KT reciprocal sums, KT values of D
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES + 2 * 3 * X::KT * 4];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int G = p.H / p.Hkv, nkt = (p.Tk + 63) / 64;
+  int grp, item;
+  if (!x_place(p.B * p.Hkv, nkt, grp, item)) return;
+  const int b = grp / p.Hkv, hkv = grp % p.Hkv;
+  int klen = p.klens ? min(p.klens[b], p.Tk) : p.Tk;
+  const bool uniform = klen <= 0;
+  if (uniform) klen = p.Tk;
+  const int k0 = item * 64 + wave * 16, key = k0 + r;
+  T* dkr = reinterpret_cast<T*>(p.dk) + (((long long)b * p.Tk + key) * p.Hkv + hkv) * p.D;
+  T* dvr = reinterpret_cast<T*>(p.dv) + (((long long)b * p.Tk + key) * p.Hkv + hkv) * p.D;
+  f32x4 dk[1][X::NB], dv[1][X::NB];
+#pragma unroll
+  for (int i = 0; i < X::NB; ++i) dk[0][i] = dv[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (item * 64 < klen && p.Tq > 0) {      // (uniform over the workgroup; keys behind klen get zeros)
+    const int chunks = p.D / X::E::CE, nqt = (p.Tq + X::KT - 1) / X::KT, n = G * nqt;
+    typename X::E::chunk K[1][X::NS], V[1][X::NS];
+    x_load_rows<T, 1>(K, reinterpret_cast<const T*>(p.k) + (long long)b * p.k_sb + (long long)hkv * p.k_sh, p.k_st, k0, klen,
+                          p.D, r, g);
+    x_load_rows<T, 1>(V, reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh, p.v_st, k0, klen,
+                          p.D, r, g);
+    const T* qb = reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)hkv * G * p.q_sh;
+    const T* gb = reinterpret_cast<const T*>(p.dout) + (long long)b * p.g_sb + (long long)hkv * G * p.g_sh;
+    const long long srow = ((long long)b * p.H + (long long)hkv * G) * p.Tq, nst = (long long)p.B * p.H * p.Tq;
+    float* st = reinterpret_cast<float*>(lds + 4 * X::BYTES);
+    auto stat = [&](int it) -> float {     // this thread's statistic of tile it
+      const int which = (int)threadIdx.x / X::KT, q = (it % nqt) * X::KT + (int)threadIdx.x % X::KT;
+      if (which >= 3) return 0.f;
+      if (which == 1 && q >= p.Tq) return 0.f;      // rows behind the last query: probability 0
+      const long long at = srow + (long long)(it / nqt) * p.Tq + min(q, p.Tq - 1);
+      return which == 0 ? p.stats[at] : which == 1 ? p.stats[nst + at] : p.dsum[at];
+    };
+    auto fetch = [&](unsigned char* to, int it) {
+      const int hq = it / nqt, row0 = (it % nqt) * X::KT;
+      X::dma(to, qb + (long long)hq * p.q_sh, p.q_st, row0, p.Tq, chunks, wave, lane);
+      X::dma(to + X::BYTES, gb + (long long)hq * p.g_sh, p.g_st, row0, p.Tq, chunks, wave, lane);
+    };
+    const float first = stat(0);
+    if ((int)threadIdx.x < 3 * X::KT) st[threadIdx.x] = first;
+    fetch(lds, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int it = 0; it < n; ++it) {
+      const unsigned char* Qc = lds + (it & 1) * (2 * X::BYTES);
+      const float* sc = st + (it & 1) * (3 * X::KT);
+      float next = 0.f;
+      if (it + 1 < n) {
+        next = stat(it + 1);
+        fetch(lds + ((it + 1) & 1) * (2 * X::BYTES), it + 1);
+      }
+      f32x4 s[1][QF], dp[1][QF];
+      x_product<T, DP, 1>(s, Qc, K, r, g);
+      x_product<T, DP, 1>(dp, Qc + X::BYTES, V, r, g);
+#pragma unroll
+      for (int qf = 0; qf < QF; ++qf) {
+        const f32x4 m4 = *reinterpret_cast<const f32x4*>(sc + 16 * qf + 4 * g);
+        const f32x4 i4 = *reinterpret_cast<const f32x4*>(sc + X::KT + 16 * qf + 4 * g);
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(sc + 2 * X::KT + 16 * qf + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(uniform ? 0.f : fmaf(s[0][qf][e], p.sl2, -m4[e])) * i4[e];
+          float keep = 1.f;
+          if constexpr (DROP) {
+            const int qi = min((it % nqt) * X::KT + 16 * qf + 4 * g + e, p.Tq - 1);
+            keep = nsp_keep_scale(p.seed, p.offset + (unsigned long long)((srow + (long long)(it / nqt) * p.Tq + qi) * p.Tk + key), p.drop);
+          }
+          const float dpe = DROP ? dp[0][qf][e] * keep : dp[0][qf][e];
+          dp[0][qf][e] = uniform ? 0.f : x * (dpe - d4[e]);
+          s[0][qf][e] = DROP ? x * keep : x;
+        }
+      }
+      x_accumulate<DP, 1>(dv, Qc + X::BYTES, s, T(0), r, g);
+      x_accumulate<DP, 1>(dk, Qc, dp, T(0), r, g);
+      if (it + 1 < n && (int)threadIdx.x < 3 * X::KT) st[((it + 1) & 1) * (3 * X::KT) + threadIdx.x] = next;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    }
+  }
+  if (key < p.Tk) {
+    const bool in = key < klen;
+    if (!in) {
+#pragma unroll
+      for (int i = 0; i < X::NB; ++i) dk[0][i] = dv[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    x_store<DP, false>(dkr, dk[0], p.scale, p.D, g);
+    x_store<DP, false>(dvr, dv[0], 1.f, p.D, g);
+  }
+}
+
+template <typename T, int DP, int NQ, bool DROP>
+int launch_fwd(const XArgs& p, hipStream_t st) {
+  const long long per = (long long)(p.H / p.Hkv) * ((p.Tq + 64 * NQ - 1) / (64 * NQ));
+  const long long wgs = ((long long)p.B * p.Hkv + 7) / 8 * 8 * per;
+  if (wgs > 0x7fffffffLL) return NSP_EUNSUPPORTED;
+  hipLaunchKernelGGL((cross_fwd_kernel<T, DP, NQ, DROP>), dim3((unsigned)wgs), dim3(256), 0, st, p);
+  NSP_LAUNCH_CHECK();
+  return NSP_OK;
+}
+template <typename T, int DP, int NQ, bool DROP>
+int launch_bwd(const XArgs& p, hipStream_t st) {
+  const long long groups = ((long long)p.B * p.Hkv + 7) / 8 * 8;
+  const long long wq = groups * (p.H / p.Hkv) * ((p.Tq + 64 * NQ - 1) / (64 * NQ)), wk = groups * ((p.Tk + 63) / 64);
+  if (wq > 0x7fffffffLL || wk > 0x7fffffffLL) return NSP_EUNSUPPORTED;
+  hipLaunchKernelGGL((cross_dq_kernel<T, DP, NQ, DROP>), dim3((unsigned)wq), dim3(256), 0, st, p);
+  NSP_LAUNCH_CHECK();
+  hipLaunchKernelGGL((cross_dkv_kernel<T, DP, DROP>), dim3((unsigned)wk), dim3(256), 0, st, p);
+  NSP_LAUNCH_CHECK();
+  return NSP_OK;
+}
+
+template <typename T, int DP, bool DROP>
+int launch(const XArgs& p, bool bwd, hipStream_t st) {
+  return bwd ? launch_bwd<T, DP, 1, DROP>(p, st) : launch_fwd<T, DP, 1, DROP>(p, st);
+}
+template <typename T, bool DROP>
+int launch_d(const XArgs& p, bool bwd, hipStream_t st) {
+  if (p.D <= 32) return launch<T, 32, DROP>(p, bwd, st);
+  if (p.D <= 64) return launch<T, 64, DROP>(p, bwd, st);
+  return launch<T, 128, DROP>(p, bwd, st);
+}
+
+int cross_attn(const nsp_cross_attn_params* a, bool bwd, void* stream) {
+  if (!a || a->B < 0 || a->Tq < 0 || a->Tk < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->D <= 0) return NSP_EINVAL;
+  if (a->D % 8 || a->D > 128 || (a->dtype != NSP_DT_F32 && a->dtype != NSP_DT_BF16)) return NSP_EUNSUPPORTED;
+  if (a->B * a->H > 0x7ffffff0LL || a->Tq > 0x7fffff00LL || a->Tk > 0x7fffff00LL || !(a->scale > 0.)) return NSP_EUNSUPPORTED;
+  if (!(a->dropout_p >= 0. && a->dropout_p < 1.)) return NSP_EINVAL;
+  if (a->B == 0 || a->Tk == 0 || (a->Tq == 0 && !bwd)) return NSP_OK;     // (nothing to read, or nothing to write but empty rows: the caller's)
+  if (!a->k || !a->v || (a->Tq > 0 && (!a->q || !a->out))) return NSP_EINVAL;
+  if (bwd && (a->Tq == 0 || !a->dout || !a->dq || !a->dk || !a->dv || !a->stats || !a->dsum)) return NSP_EINVAL;
+  if (bwd && a->dtype == NSP_DT_BF16 && !a->o_lo) return NSP_EINVAL;
+  XArgs p;
+  p.q = a->q; p.k = a->k; p.v = a->v; p.dout = a->dout; p.out = a->out;
+  p.o_lo = a->dtype == NSP_DT_BF16 ? a->o_lo : nullptr;
+  p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.stats = a->stats; p.dsum = a->dsum; p.klens = a->klens;
+  p.B = (int)a->B; p.H = (int)a->H; p.Hkv = (int)a->Hkv; p.D = (int)a->D; p.Tq = (int)a->Tq; p.Tk = (int)a->Tk;
+  p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
+  p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;
+  p.v_sb = a->v_sb; p.v_st = a->v_st; p.v_sh = a->v_sh;
+  p.g_sb = a->g_sb; p.g_st = a->g_st; p.g_sh = a->g_sh;
+  p.seed = a->seed; p.offset = a->offset;
+  p.scale = (float)a->scale;
+  p.sl2 = (float)(a->scale * 1.4426950408889634);
+  p.drop = (float)a->dropout_p;
+  const hipStream_t st = (hipStream_t)stream;
+  if (p.drop > 0.f)
+    return a->dtype == NSP_DT_BF16 ? launch_d<__bf16, true>(p, bwd, st) : launch_d<float, true>(p, bwd, st);
+  return a->dtype == NSP_DT_BF16 ? launch_d<__bf16, false>(p, bwd, st) : launch_d<float, false>(p, bwd, st);
+}
+
+}  // namespace
+
+extern "C" int nsp_cross_attn_fwd(const nsp_cross_attn_params* a, void* stream) { return cross_attn(a, false, stream); }
+extern "C" int nsp_cross_attn_bwd(const nsp_cross_attn_params* a, void* stream) { return cross_attn(a, true, stream); }

@@ -2148,6 +2148,320 @@ def lstm_cell_step(gates, h_prev, c_prev, update=None):
 
 
 # --------------------------------------------------------------------------
+# decoder operators: attention over a paged cache / over encoder states, sampling (csrc/paged_attn.hip, csrc/sample.hip)
+# --------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_DECODE_PACK = _struct.Struct('<31qd').pack         # nsp_decode_attn_params
+_APPEND_PACK = _struct.Struct('<28q').pack          # nsp_paged_append_params
+_SAMPLE_PACK = _struct.Struct('<12q3d').pack        # nsp_sample_params
+_DECODE_WS = {}                                     # call sizes -> workspace bytes (a pure function of them)
+
+
+def _one_device(*tensors):
+    """every tensor is where the kernels run, and on one device"""
+    _require_device(*tensors)
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError('tensors on different devices: %s and %s' % (dev, t.device))
+    return dev
+
+
+class _on(object):
+    """make `dev` the current device around a launch when it is not (its stream is then that device's current one)"""
+
+    def __new__(cls, dev):
+        if dev.type != 'cuda' or dev.index is None or dev.index == torch._C._cuda_getDevice():
+            return _NULL_CTX
+        return torch.cuda.device(dev)
+
+
+class _NoCtx(object):
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *a):
+        return False
+
+
+_NULL_CTX = _NoCtx()
+
+
+def _vec_ok(t):
+    """rows the kernels can read 16 bytes at a time: last dimension contiguous, the other strides multiples of 8"""
+    if t.data_ptr() % 16:
+        return False
+    st, sz = t.stride(), t.shape
+    if st[-1] != 1 and sz[-1] != 1:
+        return False
+    for i in range(len(st) - 1):
+        if st[i] % 8 and sz[i] > 1:
+            return False
+    return True
+
+
+def _vec(t):
+    return t if _vec_ok(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _int32_vec(t, n, what):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError('%s: int32 [%d] expected, got %s %s' % (what, n, t.dtype, tuple(t.shape)))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _head_size_ok(D):
+    if D % 8 or not 0 < D <= 128:
+        raise ValueError('head size %d: multiples of 8 up to 128 are supported' % D)
+
+
+def _check_pages(k_pages, v_pages, block_table, B, Hkv, D):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError('k_pages / v_pages: two [n_pages, heads, page, d] tensors of one shape and type expected')
+    if k_pages.shape[1] != Hkv or k_pages.shape[3] != D or k_pages.shape[2] < 1:
+        raise ValueError('pages of shape %s do not hold %d heads of size %d' % (tuple(k_pages.shape), Hkv, D))
+    if not (_vec_ok(k_pages) and _vec_ok(v_pages)):
+        raise ValueError('pages: contiguous last dimension, 16-byte aligned, other strides multiples of 8 elements expected')
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError('block_table: int32 [%d, pages] expected, got %s %s' % (B, block_table.dtype, tuple(block_table.shape)))
+    if block_table.shape[1] * k_pages.shape[2] > 0x7fff0000:
+        raise ValueError('more than 2^31 positions in a block table row')
+
+
+def _decode_attn(dev, q, out, k, v, table, lens, k_new, v_new, B, H, Hkv, D, Tq, page, n_pages, width, qs, ks, vs, ns, scale):
+    key = (B, H, Hkv, Tq, D, width * page)
+    nb = _DECODE_WS.get(key)
+    if nb is None:
+        if len(_DECODE_WS) > 4096:
+            _DECODE_WS.clear()
+        nb = _DECODE_WS[key] = _lib.lib().nsp_decode_attn_workspace_bytes(*key)
+    with _on(dev):
+        ws = torch.empty((nb // 4,), device=dev, dtype=torch.float32) if nb else None
+        _check(_lib.lib().nsp_decode_attn(_DECODE_PACK(
+            q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr() if table is not None else 0,
+            lens.data_ptr() if lens is not None else 0, k_new.data_ptr() if k_new is not None else 0,
+            v_new.data_ptr() if v_new is not None else 0, ws.data_ptr() if ws is not None else 0,
+            B, H, Hkv, D, Tq, page, n_pages, width, _DTYPES[q.dtype], *qs, *ks, *vs, *ns, scale), _stream()),
+            'nsp_decode_attn')
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=None, scale=None):
+    """Attention of one new token per sequence over a paged key / value cache (inference, no autograd).
+
+    q `[B,H,d]`; k_pages / v_pages `[n_pages,Hkv,page,d]` (any strides with a contiguous last dimension; H a multiple of
+    Hkv: query head h reads key head h // (H / Hkv)); block_table int32 `[B,pages]`: page of positions page*i ..; lens int32
+    `[B]`: keys in the cache.  All fp32 or all bf16 -> `[B,H,d]` of that type, softmax(scale q k^T) v with scale = d^-1/2
+    by default.  k_new / v_new `[B,Hkv,d]`: the new tokens' own keys and values, stored at position lens[b] in the same
+    launch and attended to as well (`lens` itself is left to the caller).
+
+    A sequence without any key gets zeros.  lens[b] < 0 marks an unused row of a padded batch (zeros, nothing stored).
+    Table entries behind a sequence's last page are not read; an entry outside [0, n_pages) is an absent page: its keys do
+    not count and a new token that would lie there, or behind the table, is neither stored nor attended to.  No two rows may
+    share the page that a new token is stored to."""
+    dev = _one_device(q, k_pages, v_pages, block_table, lens, k_new, v_new)
+    if q.dim() != 3 or q.dtype not in _DTYPES:
+        raise ValueError('q: fp32 or bf16 [B,H,d] expected, got %s %s' % (q.dtype, tuple(q.shape)))
+    B, H, D = q.shape
+    Hkv = k_pages.shape[1] if k_pages.dim() == 4 else 0
+    if Hkv < 1 or H % Hkv or H < 1:
+        raise ValueError('%d query heads over %d key heads' % (H, Hkv))
+    _head_size_ok(D)
+    if k_pages.dtype != q.dtype:
+        raise ValueError('q is %s, the cache %s' % (q.dtype, k_pages.dtype))
+    _check_pages(k_pages, v_pages, block_table, B, Hkv, D)
+    lens = _int32_vec(lens, B, 'lens')
+    if (k_new is None) != (v_new is None):
+        raise ValueError('k_new and v_new come together')
+    ns = (0, 0, 0, 0)
+    if k_new is not None:
+        for t in (k_new, v_new):
+            if tuple(t.shape) != (B, Hkv, D) or t.dtype != q.dtype:
+                raise ValueError('k_new / v_new: %s [%d,%d,%d] expected, got %s %s' % (q.dtype, B, Hkv, D, t.dtype, tuple(t.shape)))
+        k_new, v_new = _vec(k_new), _vec(v_new)
+        ns = (k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1))
+    if B == 0 or block_table.shape[1] == 0 or k_pages.shape[0] == 0:      # no sequence, or no key and no room
+        return torch.zeros((B, H, D), device=dev, dtype=q.dtype)
+    out = torch.empty((B, H, D), device=dev, dtype=q.dtype)
+    q = _vec(q)
+    block_table = block_table if block_table.is_contiguous() else block_table.contiguous()
+    qs, ks, vs = q.stride(), k_pages.stride(), v_pages.stride()
+    return _decode_attn(dev, q, out, k_pages, v_pages, block_table, lens, k_new, v_new, B, H, Hkv, D, 1, k_pages.shape[2],
+                        k_pages.shape[0], block_table.shape[1], (qs[0], 0, qs[1]), (ks[0], ks[2], ks[1]),
+                        (vs[0], vs[2], vs[1]), ns, D ** -0.5 if scale is None else float(scale))
+
+
+def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
+    """Write the keys and values of several tokens per sequence (a prompt) into a paged cache, in place.
+
+    k / v `[B,n,Hkv,d]` fp32 or bf16, the cache fp32 or bf16 (fp32 into bf16 rounds to nearest even; bf16 into fp32 is not
+    offered); token t of row b goes to position starts[b] + t of its block_table row for t < counts[b] (all n without
+    counts).  starts[b] < 0, absent pages (entries outside [0, n_pages)) and positions behind the table: nothing is written.
+    No position may be written twice by one call."""
+    dev = _one_device(k, v, k_pages, v_pages, block_table, starts, counts)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DTYPES:
+        raise ValueError('k / v: two fp32 or bf16 [B,n,Hkv,d] tensors of one shape and type expected')
+    B, n, Hkv, D = k.shape
+    _head_size_ok(D)
+    _check_pages(k_pages, v_pages, block_table, B, Hkv, D)
+    if k_pages.dtype not in _DTYPES or (k.dtype == torch.bfloat16 and k_pages.dtype != torch.bfloat16):
+        raise ValueError('%s into a %s cache' % (k.dtype, k_pages.dtype))
+    starts = _int32_vec(starts, B, 'starts')
+    counts = _int32_vec(counts, B, 'counts') if counts is not None else None
+    if B == 0 or n == 0 or block_table.shape[1] == 0 or k_pages.shape[0] == 0:
+        return
+    k, v = _vec(k), _vec(v)
+    block_table = block_table if block_table.is_contiguous() else block_table.contiguous()
+    ks, vs, kp, vp = k.stride(), v.stride(), k_pages.stride(), v_pages.stride()
+    with _on(dev):
+        _check(_lib.lib().nsp_paged_append(_APPEND_PACK(
+            k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), starts.data_ptr(),
+            counts.data_ptr() if counts is not None else 0, B, n, Hkv, D, k_pages.shape[2], k_pages.shape[0],
+            block_table.shape[1], _DTYPES[k.dtype], _DTYPES[k_pages.dtype], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+            kp[0], kp[2], kp[1], vp[0], vp[2], vp[1]), _stream()), 'nsp_paged_append')
+
+
+_CROSS_PACK = _struct.Struct('<31q2Q2d').pack       # nsp_cross_attn_params
+
+
+def _cross_call(name, dev, q, k, v, dout, out, o_lo, dq, dk, dv, stats, dsum, klens, sizes, scale, p, seed, offset):
+    def at(t):
+        return t.data_ptr() if t is not None else 0
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    gs = dout.stride() if dout is not None else (0, 0, 0, 0)
+    with _on(dev):
+        _check(getattr(_lib.lib(), name)(_CROSS_PACK(
+            at(q), at(k), at(v), at(dout), at(out), at(o_lo), at(dq), at(dk), at(dv), at(stats), at(dsum), at(klens), *sizes,
+            _DTYPES[q.dtype], qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], gs[0], gs[1], gs[2], seed, offset,
+            scale, p), _stream()), name)
+
+
+class CrossAttnFn(torch.autograd.Function):
+    """cross_attention with its backward (csrc/cross_attn.hip); arguments as checked there."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, klens, scale, p, seed, offset):
+        B, Tq, H, D = q.shape
+        Tk, Hkv = k.shape[1], k.shape[2]
+        dev = q.device
+        sizes = (B, H, Hkv, D, Tq, Tk)
+        ctx.empty = B == 0 or Tq == 0 or Tk == 0      # nothing to read: zeros, with zero gradients
+        if ctx.empty:
+            ctx.save_for_backward(q, k, v)
+            return torch.zeros((B, Tq, H, D), device=dev, dtype=q.dtype)
+        out = torch.empty((B, Tq, H, D), device=dev, dtype=q.dtype)
+        q, k, v = _vec(q), _vec(k), _vec(v)
+        need = any(ctx.needs_input_grad[:3])
+        stats = torch.empty((2, B, H, Tq), device=dev, dtype=torch.float32) if need else None
+        o_lo = torch.empty_like(out) if need and q.dtype == torch.bfloat16 else None
+        _cross_call('nsp_cross_attn_fwd', dev, q, k, v, None, out, o_lo, None, None, None, stats, None, klens, sizes, scale, p,
+                    seed, offset)
+        ctx.save_for_backward(q, k, v, klens, out, o_lo, stats)
+        ctx.cfg = (sizes, scale, p, seed, offset)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        if ctx.empty:
+            return tuple(torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * 5
+        q, k, v, klens, out, o_lo, stats = ctx.saved_tensors
+        (B, H, Hkv, D, Tq, Tk), scale, p, seed, offset = ctx.cfg
+        dev = q.device
+        dout = _vec(dout if dout.dtype == q.dtype else dout.to(q.dtype))
+        dq = torch.empty((B, Tq, H, D), device=dev, dtype=q.dtype)
+        dk = torch.empty((B, Tk, Hkv, D), device=dev, dtype=q.dtype)
+        dv = torch.empty((B, Tk, Hkv, D), device=dev, dtype=q.dtype)
+        dsum = torch.empty((B, H, Tq), device=dev, dtype=torch.float32)
+        _cross_call('nsp_cross_attn_bwd', dev, q, k, v, dout, out, o_lo, dq, dk, dv, stats, dsum, klens, ctx.cfg[0], scale, p,
+                    seed, offset)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
+    """Attention of target tokens over encoder states of another length: q `[B,Tq,H,d]`, k / v `[B,Tk,Hkv,d]` (query head h reads
+    key head h // (H / Hkv)), all fp32 or all bf16, any strides -> `[B,Tq,H,d]` of that type.  Differentiable in q, k and v
+    (once); gradients of shared heads are summed in fp32 and rounded once.
+
+    Key j is visible to the queries of row b if j < klens[b] (int32 `[B]`; None: all); a row without a visible key averages
+    all Tk values and passes no gradient through its scores, as AttentionFn does with its finite mask.  What lies behind
+    klens[b] in k and v is not read.  scale > 0, d^-1/2 by default.  dropout_p: dropout of the probabilities with a mask of its
+    own site (next_dropout_seed), regenerated in backward.
+
+    Without gradients and dropout, calls of up to 16 query rows per key head (Tq * H / Hkv) take the kernel that splits the
+    keys over workgroups: the single-token form of decoding."""
+    dev = _one_device(q, k, v, klens)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError('q [B,Tq,H,d] and k / v [B,Tk,Hkv,d], all fp32 or all bf16, expected: got %s %s, %s %s, %s %s' % (
+            q.dtype, tuple(q.shape), k.dtype, tuple(k.shape), v.dtype, tuple(v.shape)))
+    B, Tq, H, D = q.shape
+    Tk, Hkv = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D or Hkv < 1 or H < 1 or H % Hkv:
+        raise ValueError('q %s does not go with k %s' % (tuple(q.shape), tuple(k.shape)))
+    _head_size_ok(D)
+    if klens is not None:
+        klens = _int32_vec(klens, B, 'klens')
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and 0.0 <= dropout_p < 1.0):
+        raise ValueError('scale %r, dropout_p %r' % (scale, dropout_p))
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    if not grad and dropout_p == 0 and Tq * (H // Hkv) <= 16 and B > 0 and Tq > 0 and Tk > 0:
+        out = torch.empty((B, Tq, H, D), device=dev, dtype=q.dtype)
+        q, k, v = _vec(q), _vec(k), _vec(v)
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        return _decode_attn(dev, q, out, k, v, None, klens, None, None, B, H, Hkv, D, Tq, 1, 0, Tk, qs[:3], ks[:3], vs[:3],
+                            (0, 0, 0, 0), scale)
+    seed, offset = next_dropout_seed() if dropout_p > 0 else (0, 0)
+    return CrossAttnFn.apply(q, k, v, klens, scale, float(dropout_p), seed, offset)
+
+
+def _sample_setting(x, dtype, rows, dev, what):
+    """(device address or 0, value) of a per-row tensor or a number"""
+    if not torch.is_tensor(x):
+        return None, (int(x) if dtype == torch.int32 else float(x))
+    _one_device(x)
+    if x.device != dev or x.dtype != dtype or x.dim() != 1 or x.shape[0] != rows:
+        raise ValueError('%s: a number or %s [%d] on %s expected, got %s %s' % (what, dtype, rows, dev, x.dtype, tuple(x.shape)))
+    return (x if x.is_contiguous() else x.contiguous()), 0
+
+
+def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token per row from the given random numbers: logits fp32 or bf16 `[rows,V]`, u fp32 `[rows]` in [0,1) -> int32
+    `[rows]`.  temperature, top_k, top_p and min_p are numbers or per-row tensors (fp32, top_k int32).
+
+    Order the entries by falling logit, the lower index first among equals; w_i = exp((x_i - x_max) / temperature).  Kept are
+    the first top_k entries (0 or >= V: all), of these the ones with less than top_p x their mass before them, of these the
+    ones with w_i >= min_p; the first always.  The token is the first kept index whose mass together with the kept indices
+    before it exceeds u x the kept mass.  temperature <= 0 is the arg-max (as argmax_rows).  A NaN logit counts as -inf, a
+    +inf logit takes all the mass; rows without a logit above -inf give their first entry."""
+    dev = _one_device(logits, u)
+    if logits.dim() != 2 or logits.dtype not in _DTYPES or logits.shape[1] < 1:
+        raise ValueError('logits: fp32 or bf16 [rows,V] expected, got %s %s' % (logits.dtype, tuple(logits.shape)))
+    rows, V = logits.shape
+    if V > 1 << 18:
+        raise ValueError('vocabularies up to 2^18 are supported, got %d' % V)
+    if u.dtype != torch.float32 or u.dim() != 1 or u.shape[0] != rows:
+        raise ValueError('u: fp32 [%d] expected, got %s %s' % (rows, u.dtype, tuple(u.shape)))
+    t, t_all = _sample_setting(temperature, torch.float32, rows, dev, 'temperature')
+    k, k_all = _sample_setting(top_k, torch.int32, rows, dev, 'top_k')
+    tp, tp_all = _sample_setting(top_p, torch.float32, rows, dev, 'top_p')
+    mp, mp_all = _sample_setting(min_p, torch.float32, rows, dev, 'min_p')
+    out = torch.empty((rows,), device=dev, dtype=torch.int32)
+    if rows == 0:
+        return out
+    if (logits.stride(1) != 1 and V > 1) or (logits.stride(0) < V and rows > 1):
+        logits = logits.contiguous()
+    u = u if u.is_contiguous() else u.contiguous()
+    ld = logits.stride(0)
+    with _on(dev):
+        _check(_lib.lib().nsp_sample_rows(_SAMPLE_PACK(
+            logits.data_ptr(), u.data_ptr(), t.data_ptr() if t is not None else 0, k.data_ptr() if k is not None else 0,
+            tp.data_ptr() if tp is not None else 0, mp.data_ptr() if mp is not None else 0, out.data_ptr(), rows, V,
+            ld if rows > 1 else V, _DTYPES[logits.dtype], min(max(k_all, 0), V), t_all, tp_all, mp_all), _stream()),
+            'nsp_sample_rows')
+    return out
+
+
+# --------------------------------------------------------------------------
 # monotonic (chunkwise) attention training: the scans of MoChA / MMA (csrc/mocha.hip)
 # --------------------------------------------------------------------------
 class MonoAlphaFn(torch.autograd.Function):

@@ -1,0 +1,371 @@
+"""Bodies of the decoder-operator tests (tests/test_decoder_ops_emu_cpu.py on the host emulator of the kernels,
+tests/test_decoder_ops_gpu.py on the device): every case against a plain implementation in 64 bits.
+
+Tolerances are bounds by arithmetic, per output element.  With e(t) = finfo(t).eps / 2 the largest relative error of one
+rounding to t:
+  score s = scale q.k in fp32, D products and sums:      |ds| <= (D + 4) e(f32) scale sum_d |q_d k_d|
+  probability p = exp(s - max) / sum, n terms:           |dp| / p <= 2 max|ds| + (n + 16) e(f32)
+  bf16 probabilities enter products as high + low parts (decode) -> e(bf16)^2, or as one bf16 (training) -> e(bf16)
+  the result is rounded to the output type once:         e(t) |result|
+and an error of the terms of sum_j p_j v_j is at most that relative error times sum_j p_j |v_j|."""
+import math
+
+import torch
+
+E32 = torch.finfo(torch.float32).eps / 2
+E16 = torch.finfo(torch.bfloat16).eps / 2
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def attention_ref(q, k, v, n, scale=None):
+    """q [R,D], k / v [T,D] of one head in their own types, the first n keys visible -> (out [R,D], |dp|/p bound [R,1],
+    sum_j p_j |v_j| [R,D]) in 64 bits; n <= 0: all keys alike; no key: zeros"""
+    q, k, v = q.double(), k.double(), v.double()
+    D = q.shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    if k.shape[0] == 0:
+        return torch.zeros_like(q), torch.zeros(q.shape[0], 1, dtype=torch.float64), torch.zeros_like(q)
+    if n <= 0:
+        P = torch.full((q.shape[0], k.shape[0]), 1.0 / k.shape[0], dtype=torch.float64)
+        ds = torch.zeros(q.shape[0], 1, dtype=torch.float64)
+    else:
+        k, v = k[:n], v[:n]
+        P = torch.softmax(q @ k.t() * scale, dim=1)
+        ds = (D + 4) * E32 * abs(scale) * (q.abs() @ k.abs().t()).max(dim=1, keepdim=True).values
+    return P @ v, 2 * ds + (k.shape[0] + 16) * E32, P @ v.abs()
+
+
+def check_close(got, ref, tol, what):
+    got = got.detach().double().cpu()
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    assert torch.isfinite(got).all(), what
+    bad = (got - ref).abs() > tol
+    assert not bad.any(), '%s: %d of %d outside, worst %.3g of its tolerance' % (
+        what, int(bad.sum()), bad.numel(), float(((got - ref).abs() / tol.clamp(min=1e-300)).max()))
+
+
+def make_pages(B, need, page, Hkv, D, dtype, dev, gen, layout='heads_first', extra=2):
+    """a cache whose unused slots hold NaN, and the pages of the sequences in a random order; table entries behind a
+    sequence's pages are -1"""
+    total = sum(need) + extra
+    order = torch.randperm(total, generator=gen)
+    width = max(1, max(need))
+    table = torch.full((B, width), -1, dtype=torch.int32)
+    at = 0
+    for b in range(B):
+        table[b, :need[b]] = order[at:at + need[b]].to(torch.int32)
+        at += need[b]
+    shape = (total, Hkv, page, D) if layout == 'heads_first' else (total, page, Hkv, D)
+    pages = []
+    for _ in range(2):
+        x = torch.full(shape, float('nan'), dtype=dtype)
+        pages.append(x if layout == 'heads_first' else x.transpose(1, 2))
+    return pages[0], pages[1], table
+
+
+def put(pages, table, b, j, page, x):
+    pages[int(table[b, j // page]), :, j % page] = x
+
+
+def paged_case(ops, dev, dtype, B, H, Hkv, D, page, lens, append, layout='heads_first', seed=0, q_std=2.0, scale=None):
+    gen = torch.Generator().manual_seed(seed)
+    need = [(max(n, 0) + (1 if append and n >= 0 else 0) + page - 1) // page for n in lens]
+    kp, vp, table = make_pages(B, need, page, Hkv, D, dtype, dev, gen, layout)
+    keys = [torch.randn(max(n, 0), Hkv, D, generator=gen).to(dtype) for n in lens]
+    vals = [torch.randn(max(n, 0), Hkv, D, generator=gen).to(dtype) for n in lens]
+    for b in range(B):
+        for j in range(max(lens[b], 0)):
+            put(kp, table, b, j, page, keys[b][j])
+            put(vp, table, b, j, page, vals[b][j])
+    q = (torch.randn(B, H, D, generator=gen) * q_std).to(dtype)
+    kn, vn = torch.randn(B, Hkv, D, generator=gen).to(dtype), torch.randn(B, Hkv, D, generator=gen).to(dtype)
+    want_k, want_v = kp.clone(), vp.clone()
+    kpd, vpd = kp.to(dev), vp.to(dev)
+    if layout != 'heads_first':       # (the transposed storage must survive the move)
+        kpd, vpd = kp.transpose(1, 2).contiguous().to(dev).transpose(1, 2), vp.transpose(1, 2).contiguous().to(dev).transpose(1, 2)
+    out = ops.paged_attention(q.to(dev), kpd, vpd, table.to(dev), torch.tensor(lens, dtype=torch.int32).to(dev),
+                              k_new=kn.to(dev) if append else None, v_new=vn.to(dev) if append else None, scale=scale)
+    assert out.dtype == dtype
+    G = H // Hkv
+    for b in range(B):
+        K, V = keys[b], vals[b]
+        if append and lens[b] >= 0:
+            K, V = torch.cat([K, kn[b:b + 1]]), torch.cat([V, vn[b:b + 1]])
+            put(want_k, table, b, lens[b], page, kn[b])
+            put(want_v, table, b, lens[b], page, vn[b])
+        for h in range(Hkv):
+            ref, dp, av = attention_ref(q[b, h * G:(h + 1) * G], K[:, h], V[:, h], K.shape[0], scale)
+            split = E16 * E16 if dtype == torch.bfloat16 else 0.0
+            check_close(out[b, h * G:(h + 1) * G], ref, half_step(dtype) * ref.abs() + (dp + split) * av * (1 + half_step(dtype)),
+                        'b=%d head group %d' % (b, h))
+    # the cache: the new tokens and nothing else (NaN slots stay NaN)
+    for got, want in ((kpd, want_k), (vpd, want_v)):
+        assert torch.equal(torch.nan_to_num(got.cpu().float(), nan=-77.0), torch.nan_to_num(want.float(), nan=-77.0))
+    return out
+
+
+def append_case(ops, dev, src, dtype, B, n, Hkv, D, page, starts, counts, layout='heads_first', seed=0, strided=True):
+    gen = torch.Generator().manual_seed(seed)
+    need = [(max(s, 0) + c + page - 1) // page if s >= 0 else 0 for s, c in zip(starts, counts)]
+    kp, vp, table = make_pages(B, need, page, Hkv, D, dtype, dev, gen, layout)
+    kv = torch.randn(B, n, 2, Hkv, D, generator=gen).to(src)
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    if not strided:
+        k, v = k.contiguous(), v.contiguous()
+    want_k, want_v = kp.clone(), vp.clone()
+    for b in range(B):
+        if starts[b] >= 0:
+            for t in range(min(n, counts[b])):
+                put(want_k, table, b, starts[b] + t, page, k[b, t].to(dtype))
+                put(want_v, table, b, starts[b] + t, page, v[b, t].to(dtype))
+    if layout == 'heads_first':
+        kpd, vpd = kp.to(dev), vp.to(dev)
+    else:
+        kpd, vpd = (x.transpose(1, 2).contiguous().to(dev).transpose(1, 2) for x in (kp, vp))
+    kvd = kv.to(dev)
+    kd, vd = (kvd[:, :, 0], kvd[:, :, 1]) if strided else (k.to(dev), v.to(dev))
+    ops.paged_append(kd, vd, kpd, vpd, table.to(dev), torch.tensor(starts, dtype=torch.int32).to(dev),
+                     torch.tensor(counts, dtype=torch.int32).to(dev))
+    for got, want in ((kpd, want_k), (vpd, want_v)):
+        assert torch.equal(torch.nan_to_num(got.cpu().float(), nan=-77.0), torch.nan_to_num(want.float(), nan=-77.0))
+
+
+def sample_ref(x, u, t, k, tp, mp):
+    """one row, in Python floats (64 bits), straight from the definition"""
+    x = [(-math.inf if math.isnan(v) else v) for v in x.double().tolist()]
+    V = len(x)
+    order = sorted(range(V), key=lambda i: (-x[i], i))
+    top = x[order[0]]
+    if not t > 0 or top == -math.inf:
+        return order[0]
+    k = V if k <= 0 or k > V else k
+    w = [1.0 if v == top else (math.exp((v - top) / t) if top != math.inf else 0.0) for v in x]
+    kept = order[:k]
+    if tp < 1:
+        whole, before, n = math.fsum(w[i] for i in kept), [], 0
+        acc = 0.0
+        for i in kept:
+            if n > 0 and not acc < tp * whole:
+                break
+            acc += w[i]
+            n += 1
+        kept = kept[:max(n, 1)]
+    kept = [kept[0]] + [i for i in kept[1:] if w[i] >= mp]
+    kept.sort()
+    whole, acc = math.fsum(w[i] for i in kept), 0.0
+    for i in kept:
+        acc += w[i]
+        if acc > u * whole:
+            return i
+    return max(i for i in kept if w[i] > 0)
+
+
+def f32(x):
+    return torch.tensor(x, dtype=torch.float32).double().item()
+
+
+def sample_case(ops, dev, x, u, t=1.0, k=0, tp=1.0, mp=0.0):
+    """settings: numbers or per-row lists"""
+    rows = x.shape[0]
+
+    def per_row(s, as_int=False):
+        return [int(v) if as_int else f32(v) for v in (s if isinstance(s, (list, tuple)) else [s] * rows)]
+
+    def arg(s, dt):
+        return torch.tensor(s, dtype=dt).to(dev) if isinstance(s, (list, tuple)) else s
+    got = ops.sample_rows(x.to(dev), torch.tensor(u, dtype=torch.float32).to(dev), arg(t, torch.float32), arg(k, torch.int32),
+                          arg(tp, torch.float32), arg(mp, torch.float32))
+    assert got.dtype == torch.int32 and tuple(got.shape) == (rows,)
+    T, K, TP, MP, U = per_row(t), per_row(k, True), per_row(tp), per_row(mp), per_row(u)
+    want = [sample_ref(x[b], U[b], T[b], K[b], TP[b], MP[b]) for b in range(rows)]
+    assert got.cpu().tolist() == want, (got.cpu().tolist(), want)
+
+
+def cross_ref(q, k, v, dout, klens, dtype, scale=None, keep=None):
+    """forward and formula gradients in 64 bits, with a bound for every element.  keep [B,H,Tq,Tk]: dropout factors (0 or
+    1 / (1 - p)).  -> {'out': (ref, tol), 'dq': ..., 'dk': ..., 'dv': ...}"""
+    q, k, v = q.double(), k.double(), v.double()
+    dout = dout.double() if dout is not None else None
+    B, Tq, H, D = q.shape
+    Tk, Hkv = k.shape[1], k.shape[2]
+    G = H // Hkv
+    scale = D ** -0.5 if scale is None else scale
+    eo = half_step(dtype)
+    ep = E16 if dtype == torch.bfloat16 else 0.0          # P, dS as operands of the second products
+    z = torch.zeros_like
+    out, t_out = z(q), z(q)
+    dq, t_dq, dk, t_dk, dv, t_dv = z(q), z(q), z(k), z(k), z(v), z(v)
+    for b in range(B):
+        n = Tk if klens is None else min(int(klens[b]), Tk)
+        uniform = n <= 0
+        n = Tk if uniform else n
+        for h in range(H):
+            g = h // G
+            qh, kh, vh = q[b, :, h], k[b, :n, g], v[b, :n, g]
+            S = z(qh @ kh.t()) if uniform else qh @ kh.t() * scale
+            P = torch.softmax(S, dim=1)
+            ds = z(S[:, :1]) if uniform else (D + 4) * E32 * scale * (qh.abs() @ kh.abs().t()).max(1, keepdim=True).values
+            dp = 2 * ds + (n + 16) * E32
+            kp = keep[b, h, :, :n].double() if keep is not None else torch.ones_like(P)
+            Pd = P * kp
+            O, aO = Pd @ vh, Pd @ vh.abs()
+            out[b, :, h] = O
+            t_out[b, :, h] = eo * O.abs() + (dp + ep + 2 * E32) * aO * (1 + eo)
+            if dout is None:
+                continue
+            dO = dout[b, :, h]
+            dv[b, :n, g] += Pd.t() @ dO
+            t_dv[b, :n, g] += (Pd * (dp + ep + (Tq * G + 16) * E32)).t() @ dO.abs()
+            if uniform:
+                continue
+            dP = (dO @ vh.t()) * kp
+            Dv = (P * dP).sum(1, keepdim=True)
+            dS = P * (dP - Dv)
+            e_dP = (D + 4) * E32 * (dO.abs() @ vh.abs().t()) * kp
+            e_D = (dO.abs() * ((dp + ep) * aO + (eo * eo + (D + 4) * E32) * O.abs())).sum(1, keepdim=True)
+            e_dS = P * (dp * (dP - Dv).abs() + e_dP + e_D) + (ep + 2 * E32) * dS.abs()
+            dq[b, :, h] = scale * (dS @ kh)
+            t_dq[b, :, h] = scale * ((e_dS + (n + 16) * E32 * dS.abs()) @ kh.abs())
+            dk[b, :n, g] += scale * (dS.t() @ qh)
+            t_dk[b, :n, g] += scale * ((e_dS + (Tq * G + 16) * E32 * dS.abs()).t() @ qh.abs())
+    r = {'out': (out, t_out)}
+    if dout is not None:
+        for name, x, t in (('dq', dq, t_dq), ('dk', dk, t_dk), ('dv', dv, t_dv)):
+            r[name] = (x, t * (1 + eo) + eo * x.abs())
+    return r
+
+
+def cross_case(ops, dev, dtype, B, H, Hkv, D, Tq, Tk, klens, grad=True, layout='packed', seed=0, scale=None, q_std=2.0,
+               poison=True):
+    """layout: 'packed' = k and v views of one stacked projection, 'heads' = [B,H,T,d] storage, 'dense'"""
+    gen = torch.Generator().manual_seed(seed)
+    q = (torch.randn(B, Tq, H, D, generator=gen) * q_std).to(dtype)
+    kv = torch.randn(B, Tk, 2, Hkv, D, generator=gen).to(dtype)
+    dout = torch.randn(B, Tq, H, D, generator=gen).to(dtype) if grad else None
+    ref = cross_ref(q, kv[:, :, 0], kv[:, :, 1], dout, klens, dtype, scale)
+    if poison and klens is not None:          # what lies behind an utterance's end: NaN and infinities
+        for b in range(B):
+            if 0 < klens[b] < Tk:
+                kv[b, klens[b]:, 0] = float('nan')
+                kv[b, klens[b]:, 1] = float('inf')
+    if layout == 'packed':
+        kvd, qd = kv.to(dev), q.to(dev)
+        kd, vd = kvd[:, :, 0], kvd[:, :, 1]
+    elif layout == 'heads':
+        qd = q.transpose(1, 2).contiguous().to(dev).transpose(1, 2)
+        kd, vd = (kv[:, :, i].transpose(1, 2).contiguous().to(dev).transpose(1, 2) for i in (0, 1))
+    else:
+        qd, kd, vd = q.to(dev), kv[:, :, 0].contiguous().to(dev), kv[:, :, 1].contiguous().to(dev)
+    lens = torch.tensor(klens, dtype=torch.int32).to(dev) if klens is not None else None
+    if grad:
+        qd, kd, vd = (x.detach().requires_grad_(True) for x in (qd, kd, vd))
+    out = ops.cross_attention(qd, kd, vd, lens, scale=scale)
+    assert out.dtype == dtype and out.shape == q.shape
+    check_close(out, *ref['out'], 'out')
+    if grad:
+        for name, x in zip(('dq', 'dk', 'dv'), torch.autograd.grad(out, (qd, kd, vd), dout.to(dev))):
+            assert x.dtype == dtype
+            check_close(x, *ref[name], name)
+    return out
+
+
+def absent_pages_case(ops, dev, dtype, page):
+    """entries outside [0, n_pages) inside a sequence: their keys do not count; a new token on such a page or behind the table
+    is neither stored nor attended to; a length behind the table counts as the table"""
+    gen = torch.Generator().manual_seed(3)
+    B, Hkv, D, width = 4, 2, 32, 4
+    kp = torch.randn(9, Hkv, page, D, generator=gen).to(dtype)
+    vp = torch.randn(9, Hkv, page, D, generator=gen).to(dtype)
+    kp[0] = vp[0] = float('nan')                     # what a clamped entry would read
+    table = torch.tensor([[3, -1, 4, 5], [99, 2, -7, 6], [-1, -1, -1, -1], [1, 7, 8, 9]], dtype=torch.int32)
+    lens = [3 * page - 1, 2 * page, page, 40 * page]
+    q = torch.randn(B, Hkv, D, generator=gen).to(dtype)
+    kn, vn = torch.randn(B, Hkv, D, generator=gen).to(dtype), torch.randn(B, Hkv, D, generator=gen).to(dtype)
+    kd, vd = kp.to(dev), vp.to(dev)
+    out = ops.paged_attention(q.to(dev), kd, vd, table.to(dev), torch.tensor(lens, dtype=torch.int32).to(dev), kn.to(dev), vn.to(dev))
+    for b in range(B):
+        n = min(lens[b], width * page)
+        seen = [j for j in range(n) if 0 <= int(table[b, j // page]) < 9]
+        new = lens[b] < width * page and 0 <= int(table[b, lens[b] // page]) < 9
+        for h in range(Hkv):
+            K = [kp[int(table[b, j // page]), h, j % page] for j in seen] + ([kn[b, h]] if new else [])
+            V = [vp[int(table[b, j // page]), h, j % page] for j in seen] + ([vn[b, h]] if new else [])
+            K = torch.stack(K) if K else torch.zeros(0, D)
+            V = torch.stack(V) if V else torch.zeros(0, D)
+            ref, dp, av = attention_ref(q[b, h:h + 1], K, V, K.shape[0])
+            check_close(out[b, h:h + 1], ref, half_step(dtype) * ref.abs() + (dp + E16 * E16) * av * (1 + half_step(dtype)), 'b=%d' % b)
+        if new:
+            put(kp, table, b, lens[b], page, kn[b])
+            put(vp, table, b, lens[b], page, vn[b])
+    for got, want in ((kd, kp), (vd, vp)):
+        assert torch.equal(torch.nan_to_num(got.cpu().float(), nan=-77.0), torch.nan_to_num(want.float(), nan=-77.0))
+
+
+def dropout_case(ops, dev, dtype, B=2, H=2, Tq=7, Tk=70, D=32, p=0.3):
+    """the factors are read off with values that are rows of the identity; then out and gradients against 64 bits with them,
+    and against the mask AttentionFn draws from the same site"""
+    gen = torch.Generator().manual_seed(11)
+    klens = [Tk, Tk - 13]
+    q, k = torch.randn(B, Tq, H, D, generator=gen), torch.randn(B, Tk, H, D, generator=gen)
+    v, dout = torch.randn(B, Tk, H, D, generator=gen), torch.randn(B, Tq, H, D, generator=gen)
+    lens = torch.tensor(klens, dtype=torch.int32).to(dev)
+    # the mask of this site, from the materialised softmax: q = 0 makes every visible probability 1 / klen
+    mode = ops.get_compute_mode()
+    ops.set_compute_mode('f32')
+    ops.manual_dropout_seed(5)
+    keep = torch.zeros(B, H, Tq, Tk)
+    for j0 in range(0, Tk, D):
+        eye = torch.zeros(B, Tk, H, D)
+        for j in range(j0, min(j0 + D, Tk)):
+            eye[:, j, :, j - j0] = 1.0
+        ops.manual_dropout_seed(5)
+        cv, _ = ops.AttentionFn.apply(torch.zeros(B, Tq, H, D).to(dev), None, k.to(dev), eye.to(dev), None, lens,
+                                      {'dropout': p, 'training': True})
+        cv = cv.detach().cpu().view(B, Tq, H, D)
+        for b in range(B):
+            keep[b, :, :, j0:j0 + D] = (cv[b] * klens[b]).permute(1, 0, 2)[:, :, :min(D, Tk - j0)]
+    ops.set_compute_mode(mode)
+    kept = keep > 0.5
+    share = float(kept[0].float().mean())
+    assert abs(share - (1 - p)) < 0.1, share
+    keep = kept.double() / (1 - p)
+    q, k, v, dout = (x.to(dtype) for x in (q, k, v, dout))
+    ref = cross_ref(q, k, v, dout, klens, dtype, keep=keep)
+    qd, kd, vd = (x.to(dev).requires_grad_(True) for x in (q, k, v))
+    ops.manual_dropout_seed(5)
+    out = ops.cross_attention(qd, kd, vd, lens, dropout_p=p)
+    check_close(out, *ref['out'], 'out')
+    for name, x in zip(('dq', 'dk', 'dv'), torch.autograd.grad(out, (qd, kd, vd), dout.to(dev))):
+        check_close(x, *ref[name], name)
+
+
+def difference_case(ops, dev):
+    """directional derivatives: the kernel's difference quotient against its gradient.  The quotient's own truncation is taken
+    from the same quotient in 64 bits; its rounding is at most the outputs' tolerance over the step."""
+    gen = torch.Generator().manual_seed(7)
+    B, Tq, Tk, H, Hkv, D, h = 2, 6, 37, 4, 2, 16, 2.0 ** -5
+    klens = [37, 20]
+    lens = torch.tensor(klens, dtype=torch.int32).to(dev)
+    x = [torch.randn(B, Tq, H, D, generator=gen), torch.randn(B, Tk, Hkv, D, generator=gen), torch.randn(B, Tk, Hkv, D, generator=gen)]
+    d = [torch.randn(t.shape, generator=gen).mul_(64).round_().div_(64) for t in x]
+    x = [t.mul_(256).round_().div_(256) for t in x]                 # x +- h d without a rounding
+    w = torch.randn(B, Tq, H, D, generator=gen)
+    dev_x = [t.clone().to(dev).requires_grad_(True) for t in x]
+    grads = torch.autograd.grad(ops.cross_attention(*dev_x, lens), dev_x, w.to(dev))
+    g64 = cross_ref(*x, w, klens, torch.float32)
+    for i in range(3):
+        lo, hi = list(x), list(x)
+        lo[i], hi[i] = x[i] - h * d[i], x[i] + h * d[i]
+        with torch.enable_grad():
+            got = [ops.cross_attention(*[t.clone().to(dev).requires_grad_(True) for t in y], lens).detach().double().cpu() for y in (lo, hi)]
+        ref = [cross_ref(*y, None, klens, torch.float32)['out'] for y in (lo, hi)]
+        quot = float(((got[1] - got[0]) * w).sum() / (2 * h))
+        quot64 = float(((ref[1][0] - ref[0][0]) * w).sum() / (2 * h))
+        slope, (r, t) = float((grads[i].double().cpu() * d[i]).sum()), g64[('dq', 'dk', 'dv')[i]]
+        slope64 = float((r * d[i]).sum())
+        tol = abs(quot64 - slope64) + float(((ref[0][1] + ref[1][1]) * w.abs()).sum()) / (2 * h) + float((t * d[i].abs()).sum())
+        assert abs(quot - slope) <= tol, (i, quot, slope, tol)
+        assert tol < 0.2 * abs(slope64), (i, tol, slope64)

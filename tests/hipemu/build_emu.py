@@ -19,7 +19,8 @@ ASAN = os.environ.get('NSP_EMU_ASAN', '0') == '1'
 OUT = os.path.join(HERE, '_build_asan' if ASAN else '_build')
 LIB = os.path.join(OUT, 'libnsp_emu.so')
 EMULATED_SOURCES = ['norm_subsample.hip', 'elementwise.hip', 'xent.hip', 'decode.hip', 'layernorm.hip', 'ctc.hip',
-                    'dwconv.hip', 'rnnt.hip', 'rnnt_fused.hip', 'gemm.hip', 'attention.hip', 'lstm.hip', 'conv2d.hip', 'gemm_bf16.hip', 'flash_attn.hip', 'mocha.hip', 'decoder_step.hip']
+                    'dwconv.hip', 'rnnt.hip', 'rnnt_fused.hip', 'gemm.hip', 'attention.hip', 'lstm.hip', 'conv2d.hip', 'gemm_bf16.hip', 'flash_attn.hip', 'mocha.hip', 'decoder_step.hip',
+                    'paged_attn.hip', 'sample.hip', 'cross_attn.hip']
 CXX_CANDIDATES = ['/opt/rocm/lib/llvm/bin/clang++', 'clang++']
 
 
@@ -49,7 +50,8 @@ def _rewrite(src, dst):
     text = re.sub(r'asm volatile\("s_waitcnt vmcnt\((\d+)\)"\s*:::\s*"memory"\);', r'hipemu_waitcnt_vm(\1);', text)
     text = re.sub(r'asm volatile\("s_waitcnt[^;]*;', '/* s_waitcnt (lgkmcnt): no-op on the host */;', text)
     text = text.replace('__attribute__((address_space(1)))', '').replace('__attribute__((address_space(3)))', '')
-    text = text.replace('#include "common.h"', '#include "%s"' % os.path.join(CSRC, 'common.h'))
+    for hdr in ('common.h', 'attn_frag.h'):
+        text = text.replace('#include "%s"' % hdr, '#include "%s"' % os.path.join(CSRC, hdr))
     with open(dst, 'w') as fh:
         fh.write(text)
 
@@ -71,7 +73,7 @@ def build():
 
 def _build_locked(cxx):
     srcs = [os.path.join(CSRC, s) for s in EMULATED_SOURCES] + [os.path.join(HERE, 'emu_runtime.cpp')]
-    deps = srcs + [os.path.join(HERE, 'include', 'hip', 'hip_runtime.h'), os.path.join(CSRC, 'common.h'),
+    deps = srcs + [os.path.join(HERE, 'include', 'hip', 'hip_runtime.h'), os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'attn_frag.h'),
                    os.path.join(ROOT, 'include', 'nsp_hip.h')]
     h = hashlib.sha1()
     for f in deps:

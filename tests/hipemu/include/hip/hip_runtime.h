@@ -431,6 +431,9 @@ static inline float atomicAdd(float* p, float v) {
   return f;
 }
 
+static inline int atomicAdd(int* p, int v) { return __atomic_fetch_add(p, v, __ATOMIC_RELAXED); }
+static inline unsigned long long atomicAdd(unsigned long long* p, unsigned long long v) { return __atomic_fetch_add(p, v, __ATOMIC_RELAXED); }
+
 namespace hipemu {
 static inline void fiber_entry() {
   Wave* w = wave;
