@@ -833,12 +833,12 @@ typedef struct {
   const void* q; const void* k; const void* v; const void* dout;
   void* out; void* o_lo; void* dq; void* dk; void* dv;
   float* stats; float* dsum; const int* klens;
+  long long g_sb, g_st, g_sh;
+  unsigned long long seed, offset;
   long long B, H, Hkv, D, Tq, Tk, dtype;
   long long q_sb, q_st, q_sh;
   long long k_sb, k_st, k_sh;
   long long v_sb, v_st, v_sh;
-  long long g_sb, g_st, g_sh;
-  unsigned long long seed, offset;
   double scale, dropout_p;
 } nsp_cross_attn_params;
 int nsp_cross_attn_fwd(const nsp_cross_attn_params* p, void* stream);

@@ -10,22 +10,22 @@
 // answer now and then.  Masses are therefore fixed-point integers, w x 2^44 from a 64-bit exponential: integer sums have no
 // order, and borders move by less than 2^-44 of the largest mass per entry.
 //
-// One workgroup of 16 waves per row.  A row of up to 32768 logits is read once and stays in LDS, a longer one is read again
-// by each pass (from L2).  The k-th entry and the entry that completes top_p are found with one histogram of 2048
-// bins that are linear in the logit between the row's extremes, a scan, and an exact ranking of the few entries of the bin
+// One workgroup per row: 4 waves for rows of up to 1024 logits, where latency is all, else 16.  A row is read once and stays in
+// LDS, up to 11000 logits with their masses, so that the 64-bit exponential runs once per entry; rows behind 32768 logits
+// are read again by each pass (from L2).  The k-th entry and the entry that completes top_p are found with one histogram
+// whose bins are linear in the logit between the row's extremes, a scan, and an exact ranking of the few entries of the bin
 // that the border falls in; rows with too many entries in that bin (equal logits) take a radix descent over (logit, index).
-// What bounds the call is latency: a handful of workgroup-wide reductions of about half a microsecond each.
+// What bounds the call is latency: about twenty barriers, and scans over a wave, which therefore run on DPP lane moves
+// (8 cycles a step, where a shuffle through LDS takes about 130).
 #include "common.h"
 
 namespace {
 
 typedef unsigned long long u64;
-constexpr int ST = 1024;      // threads
-constexpr int NW = ST / 64;   // waves
-constexpr int BINS = 2048;
-constexpr int ROW_CHUNKS = 8; // chunks of 4096 logits that fit the LDS (128 KB) beside `Shared`
-constexpr int CAND = 512;    // entries that are ranked one against the other
+constexpr int CAND = 512;     // entries that are ranked one against the other
 constexpr int FRAC = 44;      // bits behind the point of a mass; V <= 2^18 keeps every sum below 2^62
+// what of the row the LDS holds
+enum { NOTHING = 0, LOGITS = 1, LOGITS_AND_MASSES = 2 };
 
 struct SampleArgs {
   const void* x;
@@ -86,81 +86,129 @@ __device__ __forceinline__ double sample_weight(float x, const RowScale& r) {
 }
 __device__ __forceinline__ u64 sample_mass(double w) { return (u64)(w * (double)(1ull << FRAC) + 0.5); }
 
-__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+struct Mass4 {
+  u64 m[4];
+};
+__device__ __forceinline__ Mass4 sample_mass4(float a, float b, float c, float d, const RowScale& rs) {
+  return Mass4{{sample_mass(sample_weight(a, rs)), sample_mass(sample_weight(b, rs)), sample_mass(sample_weight(c, rs)),
+                sample_mass(sample_weight(d, rs))}};
 }
-__device__ __forceinline__ u64 wave_max_u64(u64 v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 w = __shfl_xor(v, o, 64);
-    v = w > v ? w : v;
-  }
-  return v;
-}
-// sum over the lanes below
-__device__ __forceinline__ u64 wave_before_u64(u64 v, int lane) {
-  u64 s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 w = __shfl_up(s, o, 64);
-    if (lane >= o) s += w;
-  }
-  return s - v;
+// (for kernels that compute masses in several places: one copy of the code, everything in registers)
+__device__ __attribute__((noinline)) Mass4 sample_mass4_call(float a, float b, float c, float d, float xmax, double inv_t) {
+  return sample_mass4(a, b, c, d, RowScale{xmax, inv_t});
 }
 
-// the row's entries: thread t holds indices 4 ST c + 4 t + j of chunk c.  IN_LDS: read once, kept in LDS
-template <typename T, bool IN_LDS>
+// the value `CTRL` lanes below (DPP), 0 where there is none
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 lane_move(u64 v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xF, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xF, true);
+  return ((u64)(unsigned)hi << 32) | (unsigned)lo;
+}
+enum { ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143 };
+// sum over this lane and the ones below; lane 63 has the wave's
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+  v += lane_move<ROW_SHR + 1, 0xF>(v);
+  v += lane_move<ROW_SHR + 2, 0xF>(v);
+  v += lane_move<ROW_SHR + 4, 0xF>(v);
+  v += lane_move<ROW_SHR + 8, 0xF>(v);
+  v += lane_move<ROW_BCAST15, 0xA>(v);
+  v += lane_move<ROW_BCAST31, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ u64 max_u64(u64 a, u64 b) { return a > b ? a : b; }
+// maximum, in lane 63
+__device__ __forceinline__ u64 wave_max(u64 v) {
+  v = max_u64(v, lane_move<ROW_SHR + 1, 0xF>(v));
+  v = max_u64(v, lane_move<ROW_SHR + 2, 0xF>(v));
+  v = max_u64(v, lane_move<ROW_SHR + 4, 0xF>(v));
+  v = max_u64(v, lane_move<ROW_SHR + 8, 0xF>(v));
+  v = max_u64(v, lane_move<ROW_BCAST15, 0xA>(v));
+  v = max_u64(v, lane_move<ROW_BCAST31, 0xC>(v));
+  return v;
+}
+
+// the row's entries: thread t holds indices 4 ST c + 4 t + j of chunk c.  A thread reads back from LDS only what it wrote.
+template <typename T, int ST, int KEEP>
 struct Row {
   const T* p;
-  f32x4* buf;
+  f32x4* buf;        // [chunks][ST]
+  ulonglong2* mbuf;  // [chunks][ST][2]
+  RowScale rs;
   int V, chunks, tid;
-  __device__ __forceinline__ void fetch(int c, float (&y)[4]) const {
+  __device__ __forceinline__ void load(int c, float (&y)[4]) const {
     const int i0 = c * (4 * ST) + 4 * tid;
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[j] = i0 + j < V ? sample_load(p + i0 + j) : 0.f;
   }
-  __device__ __forceinline__ void init() {
-    if constexpr (IN_LDS) {      // (a thread reads back only what it wrote)
-#pragma unroll 4
-      for (int c = 0; c < chunks; ++c) {
-        float y[4];
-        fetch(c, y);
-        buf[c * ST + tid] = f32x4{y[0], y[1], y[2], y[3]};
-      }
+  __device__ __forceinline__ void get(int c, float (&y)[4]) const {
+    if constexpr (KEEP != NOTHING) {
+      const f32x4 v = buf[c * ST + tid];
+      y[0] = v[0]; y[1] = v[1]; y[2] = v[2]; y[3] = v[3];
+    } else {
+      load(c, y);
     }
   }
-  template <class F>
-  __device__ __forceinline__ void each_chunk(F f) {   // f(chunk, x[4], first index)
+  // masses of the entries that are not below `floor`
+  __device__ __forceinline__ void compute(const float (&y)[4], int i0, u64 floor, u64 (&m)[4]) const {
+    m[0] = m[1] = m[2] = m[3] = 0;
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) any = any || (i0 + j < V && sample_entry(y[j], i0 + j) >= floor);
+    if (any) {
+      const Mass4 w = KEEP == LOGITS_AND_MASSES ? sample_mass4(y[0], y[1], y[2], y[3], rs)
+                                                : sample_mass4_call(y[0], y[1], y[2], y[3], rs.xmax, rs.inv_t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m[j] = i0 + j < V && sample_entry(y[j], i0 + j) >= floor ? w.m[j] : 0;
+    }
+  }
+  // LOGITS_AND_MASSES: the masses the later passes find in LDS
+  __device__ __forceinline__ void keep_masses(u64 floor) {
+    if constexpr (KEEP == LOGITS_AND_MASSES) {
 #pragma unroll 1
-    for (int c = 0; c < chunks; ++c) {
-      float y[4];
-      if constexpr (IN_LDS) {
-        const f32x4 v = buf[c * ST + tid];
-        y[0] = v[0]; y[1] = v[1]; y[2] = v[2]; y[3] = v[3];
-      } else {
-        fetch(c, y);
+      for (int c = 0; c < chunks; ++c) {
+        const int i0 = c * (4 * ST) + 4 * tid;
+        if (i0 >= V) break;
+        float y[4];
+        u64 m[4];
+        get(c, y);
+        compute(y, i0, floor, m);
+        mbuf[2 * (c * ST + tid)] = make_ulonglong2(m[0], m[1]);
+        mbuf[2 * (c * ST + tid) + 1] = make_ulonglong2(m[2], m[3]);
       }
-      f(c, y, c * (4 * ST) + 4 * tid);
     }
   }
-  template <class F>
-  __device__ __forceinline__ void each(F f) {         // f(x, index) for the entries that there are
-    const int n = V;
-    each_chunk([&](int, float (&y)[4], int i0) {
+  __device__ __forceinline__ void masses(int c, const float (&y)[4], int i0, u64 floor, u64 (&m)[4]) const {
+    if constexpr (KEEP == LOGITS_AND_MASSES) {
+      const ulonglong2 a = mbuf[2 * (c * ST + tid)], b = mbuf[2 * (c * ST + tid) + 1];
+      m[0] = a.x; m[1] = a.y; m[2] = b.x; m[3] = b.y;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (i0 + j < n) f(y[j], i0 + j);
-    });
+        if (sample_entry(y[j], i0 + j) < floor) m[j] = 0;
+    } else {
+      compute(y, i0, floor, m);
+    }
+  }
+  // f(chunk, x[4], first index), for the chunks where this thread has an entry (WHOLE: for all, whole waves)
+  template <bool WHOLE, class F>
+  __device__ __forceinline__ void each_chunk(F f) {
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c) {
+      const int i0 = c * (4 * ST) + 4 * tid;
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      if (i0 < V) get(c, y);
+      else if (!WHOLE) break;
+      f(c, y, i0);
+    }
   }
 };
 
+template <int ST>
 struct Shared {
-  u64 hist[BINS];     // counts or masses per bin
+  u64 hist[2 * ST];   // counts or masses per bin
   u64 cand[CAND];     // entries of the border's bin
   u64 cmass[CAND];
-  u64 red[NW], red2[NW];
+  u64 red[16], red2[16];
   u64 before;
   int bin, count;
 };
@@ -168,17 +216,17 @@ struct Shared {
 // The bin (0 = the first of the order) that the border falls in: the last non-empty one with less than the border before it,
 // where `base` is what lies before bin 0.  The border is `target` entries, or the mass `lim` (frac > 0: frac x the bins' whole).
 // -> sh.bin, sh.before (base included); returns lim
-template <bool MASS>
-__device__ __forceinline__ double find_bin(Shared& sh, u64 base, u64 target, double lim, double frac, int tid) {
+template <int ST, bool MASS>
+__device__ __forceinline__ double find_bin(Shared<ST>& sh, u64 base, u64 target, double lim, double frac, int tid) {
   const int lane = tid & 63, wave = tid >> 6;
   const u64 a = sh.hist[2 * tid], b = sh.hist[2 * tid + 1];
-  const u64 inw = wave_before_u64(a + b, lane);
-  if (lane == 63) sh.red[wave] = inw + a + b;
+  const u64 to = wave_scan(a + b);
+  if (lane == 63) sh.red[wave] = to;
   if (tid == 0) { sh.bin = 0; sh.before = base; }
   __syncthreads();
   u64 off = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) {
+  for (int w = 0; w < ST / 64; ++w) {
     const u64 s = sh.red[w];
     off += w < wave ? s : 0;
     all += s;
@@ -186,7 +234,7 @@ __device__ __forceinline__ double find_bin(Shared& sh, u64 base, u64 target, dou
   if (MASS && frac > 0.) lim = frac * (double)all;
   auto below = [&](u64 s) -> bool { return MASS ? (double)(base + s) < lim : base + s < target; };
   // sums before the bins rise: a kept bin is the last one if the sum behind it is not below the border, or is the whole
-  const u64 s0 = off + inw, s1 = s0 + a, s2 = s1 + b;
+  const u64 s2 = off + to, s1 = s2 - b, s0 = s1 - a;
   if (b > 0 && below(s1) && (!below(s2) || s2 == all)) { sh.bin = 2 * tid + 1; sh.before = base + s1; }
   else if (a > 0 && below(s0) && (!below(s1) || s1 == all)) { sh.bin = 2 * tid; sh.before = base + s0; }
   __syncthreads();
@@ -195,73 +243,77 @@ __device__ __forceinline__ double find_bin(Shared& sh, u64 base, u64 target, dou
 
 // The last kept entry when entries >= floor take part with weight 1 (count: the first `target` stay) or their mass (those
 // with less than frac x the whole before them stay).
-template <typename T, bool IN_LDS, bool MASS>
-__device__ u64 last_kept(Shared& sh, Row<T, IN_LDS>& row, const RowScale& rs, u64 floor, float bin_scale, u64 target, double frac) {
+template <typename T, int ST, int KEEP, bool MASS>
+__device__ __forceinline__ u64 last_kept(Shared<ST>& sh, Row<T, ST, KEEP>& row, u64 floor, float bin_scale, u64 target, double frac) {
+  constexpr int BINS = 2 * ST, LOG_BINS = ST == 1024 ? 11 : 9;
   const int tid = row.tid;
-  auto weight = [&](float x) -> u64 { return MASS ? sample_mass(sample_weight(x, rs)) : 1ull; };
   auto bin_of = [&](float x) -> int {
-    const float y = (rs.xmax - x) * bin_scale;            // falls as x rises, rounding included
+    const float y = (row.rs.xmax - x) * bin_scale;        // falls as x rises, rounding included
     return y < (float)(BINS - 1) ? (int)y : BINS - 1;      // (-inf, NaN: last)
+  };
+  auto each = [&](auto f) {       // f(entry, weight, bin) for the entries that take part
+    row.template each_chunk<false>([&](int c, float (&y)[4], int i0) {
+      u64 m[4];
+      if constexpr (MASS) {
+        row.masses(c, y, i0, floor, m);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m[j] = i0 + j < row.V && sample_entry(y[j], i0 + j) >= floor ? 1ull : 0ull;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (m[j]) f(sample_entry(y[j], i0 + j), m[j], bin_of(y[j]));
+    });
   };
   __syncthreads();
   sh.hist[2 * tid] = 0;
   sh.hist[2 * tid + 1] = 0;
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  row.each([&](float x, int i) {
-    if (sample_entry(x, i) >= floor) {
-      const u64 w = weight(x);
-      if (w) atomicAdd(&sh.hist[bin_of(x)], w);
-    }
-  });
+  each([&](u64, u64 m, int b) { atomicAdd(&sh.hist[b], m); });
   __syncthreads();
-  const double lim = find_bin<MASS>(sh, 0, target, 0., frac, tid);
+  const double lim = find_bin<ST, MASS>(sh, 0, target, 0., frac, tid);
   const int bin = sh.bin;
   const u64 before = sh.before;
-  row.each([&](float x, int i) {
-    if (bin_of(x) == bin && sample_entry(x, i) >= floor) {
-      const u64 w = weight(x);
-      if (w) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < CAND) { sh.cand[at] = sample_entry(x, i); sh.cmass[at] = w; }
-      }
+  each([&](u64 c, u64 m, int b) {
+    if (b == bin) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < CAND) { sh.cand[at] = c; sh.cmass[at] = m; }
     }
   });
   __syncthreads();
   const int n = sh.count;
   if (n <= CAND) {
     // rank every candidate against the others; the last kept one is the smallest entry with less than the border before it
-    u64 mine = ~0ull;
+    u64 kept = 0;                 // (complemented: the maximum is wanted)
     for (int a = tid; a < n; a += ST) {
       const u64 c = sh.cand[a];
       u64 s = before;
       for (int o = 0; o < n; ++o) s += sh.cand[o] > c ? sh.cmass[o] : 0;
-      if (MASS ? (double)s < lim : s < target) mine = c;
+      if (MASS ? (double)s < lim : s < target) kept = max_u64(kept, ~c);
     }
-    mine = ~wave_max_u64(~mine);
-    if ((tid & 63) == 0) sh.red2[tid >> 6] = mine;
+    kept = wave_max(kept);
+    if ((tid & 63) == 63) sh.red2[tid >> 6] = kept;
     __syncthreads();
+    kept = 0;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) mine = sh.red2[w] < mine ? sh.red2[w] : mine;
-    return mine;
+    for (int w = 0; w < ST / 64; ++w) kept = max_u64(kept, sh.red2[w]);
+    return ~kept;
   }
-  // many equal logits: radix descent over the entries of the bin, 11 bits at a time
+  // many equal logits: radix descent over the entries of the bin
   u64 prefix = 0, sum = before;
+#pragma unroll 1
   for (int hi = 32 + IDX_BITS; hi > 0;) {
-    const int bits = hi > 11 ? 11 : hi, lo = hi - bits;
+    const int bits = hi > LOG_BINS ? LOG_BINS : hi, lo = hi - bits;
     __syncthreads();
     sh.hist[2 * tid] = 0;
     sh.hist[2 * tid + 1] = 0;
     __syncthreads();
-    row.each([&](float x, int i) {
-      const u64 c = sample_entry(x, i);
-      if (c >= floor && bin_of(x) == bin && (c >> hi) == prefix) {
-        const u64 w = weight(x);
-        if (w) atomicAdd(&sh.hist[(1 << bits) - 1 - (int)((c >> lo) & ((1u << bits) - 1u))], w);
-      }
+    each([&](u64 c, u64 m, int b) {
+      if (b == bin && (c >> hi) == prefix) atomicAdd(&sh.hist[(1 << bits) - 1 - (int)((c >> lo) & ((1u << bits) - 1u))], m);
     });
     __syncthreads();
-    find_bin<MASS>(sh, sum, target, lim, 0., tid);
+    find_bin<ST, MASS>(sh, sum, target, lim, 0., tid);
     prefix = (prefix << bits) | (u64)((1 << bits) - 1 - sh.bin);
     sum = sh.before;
     hi = lo;
@@ -269,83 +321,95 @@ __device__ u64 last_kept(Shared& sh, Row<T, IN_LDS>& row, const RowScale& rs, u6
   return prefix;
 }
 
-template <typename T, bool IN_LDS>
+template <typename T, int ST, int KEEP>
 __global__ __launch_bounds__(ST) void sample_rows_kernel(const SampleArgs a) {
-  __shared__ Shared sh;
+  constexpr int NW = ST / 64;
+  __shared__ Shared<ST> sh;
   extern __shared__ __attribute__((aligned(16))) float row_buf[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long long b = blockIdx.x;
-  Row<T, IN_LDS> row;
+  Row<T, ST, KEEP> row;
   row.p = reinterpret_cast<const T*>(a.x) + b * a.ld;
   row.V = a.V;
   row.tid = tid;
-  row.buf = reinterpret_cast<f32x4*>(row_buf);
   row.chunks = (a.V + 4 * ST - 1) / (4 * ST);
+  row.buf = reinterpret_cast<f32x4*>(row_buf);
+  row.mbuf = reinterpret_cast<ulonglong2*>(row_buf + (a.V + 3) / 4 * 4);
   const float t = a.t ? a.t[b] : a.t_all, tp = a.tp ? a.tp[b] : a.tp_all, mp = a.mp ? a.mp[b] : a.mp_all;
   const float u = a.u[b];
   int k = a.k ? a.k[b] : a.k_all;
   if (k <= 0 || k > a.V) k = a.V;
-  row.init();
 
-  // first entry of the order, and the smallest finite logit
-  u64 top = 0;
-  float mn = INFINITY;
-  row.each([&](float x, int i) {
-    const u64 c = sample_entry(x, i);
-    top = c > top ? c : top;
-    if (x > -INFINITY && x < mn) mn = x;
-  });
-  top = wave_max_u64(top);
-  mn = -wave_reduce_max(-mn);
-  if (lane == 0) { sh.red[wave] = top; sh.red2[wave] = __float_as_uint(mn); }
+  // the row; the first entry of the order, and the smallest finite logit (as the largest complemented key)
+  u64 top = 0, low = 0;
+#pragma unroll 2
+  for (int c = 0; c < row.chunks; ++c) {
+    const int i0 = c * (4 * ST) + 4 * tid;
+    if (i0 >= a.V) break;
+    float y[4];
+    row.load(c, y);
+    if constexpr (KEEP != NOTHING) row.buf[c * ST + tid] = f32x4{y[0], y[1], y[2], y[3]};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i0 + j < a.V) {
+        top = max_u64(top, sample_entry(y[j], i0 + j));
+        if (y[j] > -INFINITY) low = max_u64(low, (u64)(unsigned)~sample_key(y[j]));
+      }
+    }
+  }
+  top = wave_max(top);
+  low = wave_max(low);
+  if (lane == 63) { sh.red[wave] = top; sh.red2[wave] = low; }
   __syncthreads();
+  top = low = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
-    top = sh.red[w] > top ? sh.red[w] : top;
-    mn = fminf(mn, __uint_as_float((unsigned)sh.red2[w]));
+    top = max_u64(top, sh.red[w]);
+    low = max_u64(low, sh.red2[w]);
   }
   const int first = (1 << IDX_BITS) - 1 - (int)(top & ((1u << IDX_BITS) - 1u));
-  const unsigned tk = (unsigned)(top >> IDX_BITS);
-  RowScale rs;
-  rs.xmax = __uint_as_float(tk ^ ((tk >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+  const unsigned tk = (unsigned)(top >> IDX_BITS), lk = ~(unsigned)low;
+  row.rs.xmax = __uint_as_float(tk ^ ((tk >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+  const float xmin = __uint_as_float(lk ^ ((lk >> 31) ? 0x80000000u : 0xFFFFFFFFu));
   // temperature 0, one entry, nothing but -inf / NaN: the first entry
   if (!(t > 0.f) || k == 1 || !(tp > 0.f) || tk <= 0x007FFFFFu) {
     if (tid == 0) a.out[b] = first;
     return;
   }
-  rs.inv_t = 1.0 / (double)t;
-  const float range = rs.xmax - mn;
-  const float bin_scale = range > 0.f && range < INFINITY ? (float)(BINS - 1) / range : 0.f;
+  row.rs.inv_t = 1.0 / (double)t;
+  const float range = row.rs.xmax - xmin;
+  const float bin_scale = range > 0.f && range < INFINITY ? (float)(2 * ST - 1) / range : 0.f;
 
   u64 floor = 0;
-  if (k < a.V) floor = last_kept<T, IN_LDS, false>(sh, row, rs, 0, bin_scale, (u64)k, 0.);
-  if (tp < 1.f) floor = last_kept<T, IN_LDS, true>(sh, row, rs, floor, bin_scale, 0, (double)tp);
+  if (k < a.V) floor = last_kept<T, ST, KEEP, false>(sh, row, 0, bin_scale, (u64)k, 0.);
+  row.keep_masses(floor);
+  if (tp < 1.f) floor = last_kept<T, ST, KEEP, true>(sh, row, floor, bin_scale, 0, (double)tp);
 
   // kept mass by index: per chunk and wave (256 consecutive indices), in sh.hist
-  const double minw = (double)mp;
-  auto mass = [&](float x, int i) -> u64 {
-    const u64 c = sample_entry(x, i);
-    if (c < floor) return 0ull;
-    const double w = sample_weight(x, rs);
-    return w >= minw || c == top ? sample_mass(w) : 0ull;
+  const double minm = (double)mp * (double)(1ull << FRAC);
+  auto kept_masses = [&](int c, float (&y)[4], int i0, u64 (&m)[4]) {
+    m[0] = m[1] = m[2] = m[3] = 0;
+    if (i0 >= a.V) return;
+    row.masses(c, y, i0, floor, m);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (!((double)m[j] >= minm) && i0 + j != first) m[j] = 0;
   };
   __syncthreads();
   sh.hist[2 * tid] = 0;
   sh.hist[2 * tid + 1] = 0;
   __syncthreads();
-  row.each_chunk([&](int c, float (&y)[4], int i0) {
-    u64 s = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i0 + j < a.V) s += mass(y[j], i0 + j);
-    s = wave_sum_u64(s);
-    if (lane == 0) sh.hist[c * NW + wave] = s;
+  row.template each_chunk<true>([&](int c, float (&y)[4], int i0) {
+    u64 m[4];
+    kept_masses(c, y, i0, m);
+    const u64 s = wave_scan(m[0] + m[1] + m[2] + m[3]);
+    if (lane == 63) sh.hist[c * NW + wave] = s;
   });
   __syncthreads();
-  // the segment of the token: the first whose end exceeds u x the whole (u >= 1: the last with any mass)
+  // the segment of the token: the first whose end exceeds u x the whole (u >= 1, NaN: the last with any mass)
   const u64 ha = sh.hist[2 * tid], hb = sh.hist[2 * tid + 1];
-  const u64 inw = wave_before_u64(ha + hb, lane);
-  if (lane == 63) sh.red[wave] = inw + ha + hb;
+  const u64 to = wave_scan(ha + hb);
+  if (lane == 63) sh.red[wave] = to;
   __syncthreads();
   u64 off = 0, all = 0;
 #pragma unroll
@@ -354,49 +418,47 @@ __global__ __launch_bounds__(ST) void sample_rows_kernel(const SampleArgs a) {
     all += sh.red[w];
   }
   const double want = (double)u * (double)all;
-  const u64 lo = off + inw;
   auto inside = [&](u64 from, u64 m) -> bool {
     return m > 0 && (!((double)from > want) || from == 0) && ((double)(from + m) > want || from + m == all);
   };
-  if (inside(lo, ha)) { sh.bin = 2 * tid; sh.before = lo; }
-  if (inside(lo + ha, hb)) { sh.bin = 2 * tid + 1; sh.before = lo + ha; }
+  const u64 end = off + to;
+  if (inside(end - hb - ha, ha)) { sh.bin = 2 * tid; sh.before = end - hb - ha; }
+  if (inside(end - hb, hb)) { sh.bin = 2 * tid + 1; sh.before = end - hb; }
   __syncthreads();
   const int seg = sh.bin;
   if (wave != seg % NW) return;
-  row.each_chunk([&](int c, float (&y)[4], int i0) {
-    if (c != seg / NW) return;
-    u64 m[4], s = 0;
+  const int c = seg / NW, i0 = c * (4 * ST) + 4 * tid;
+  float y[4] = {0.f, 0.f, 0.f, 0.f};
+  u64 m[4];
+  if (i0 < a.V) row.get(c, y);
+  kept_masses(c, y, i0, m);
+  const u64 s = m[0] + m[1] + m[2] + m[3];
+  u64 at = sh.before + wave_scan(s) - s;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      m[j] = i0 + j < a.V ? mass(y[j], i0 + j) : 0ull;
-      s += m[j];
-    }
-    u64 at = sh.before + wave_before_u64(s, lane);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (inside(at, m[j])) a.out[b] = i0 + j;
-      at += m[j];
-    }
-  });
+  for (int j = 0; j < 4; ++j) {
+    if (inside(at, m[j])) a.out[b] = i0 + j;
+    at += m[j];
+  }
 }
 
-template <typename T>
+template <typename T, int ST, int KEEP>
 int launch_sample(const SampleArgs& a, long long rows, hipStream_t st) {
-  const dim3 grid((unsigned)rows);
-  const int chunks = (a.V + 4 * ST - 1) / (4 * ST);
-  if (chunks <= ROW_CHUNKS) {
-    const size_t bytes = (size_t)chunks * 16 * ST;
-    if (bytes > 32 * 1024) {
-      const hipError_t e = hipFuncSetAttribute((const void*)sample_rows_kernel<T, true>,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, ROW_CHUNKS * 16 * ST);
-      if (e != hipSuccess) return (int)e;
-    }
-    hipLaunchKernelGGL((sample_rows_kernel<T, true>), grid, dim3(ST), bytes, st, a);
-  } else {
-    hipLaunchKernelGGL((sample_rows_kernel<T, false>), grid, dim3(ST), 0, st, a);
+  const size_t v4 = ((size_t)a.V + 3) / 4 * 4, bytes = KEEP == NOTHING ? 0 : KEEP == LOGITS ? v4 * 4 : v4 * 12;
+  if (bytes + sizeof(Shared<ST>) > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)sample_rows_kernel<T, ST, KEEP>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, 132000);
+    if (e != hipSuccess) return (int)e;
   }
+  hipLaunchKernelGGL((sample_rows_kernel<T, ST, KEEP>), dim3((unsigned)rows), dim3(ST), bytes, st, a);
   NSP_LAUNCH_CHECK();
   return NSP_OK;
+}
+template <typename T>
+int launch_sample_v(const SampleArgs& a, long long rows, hipStream_t st) {
+  if (a.V <= 1024) return launch_sample<T, 256, LOGITS_AND_MASSES>(a, rows, st);
+  if (a.V <= 11000) return launch_sample<T, 1024, LOGITS_AND_MASSES>(a, rows, st);   // 132 KB beside the 25 KB of Shared
+  if (a.V <= 32768) return launch_sample<T, 1024, LOGITS>(a, rows, st);
+  return launch_sample<T, 1024, NOTHING>(a, rows, st);
 }
 
 }  // namespace
@@ -412,7 +474,7 @@ extern "C" int nsp_sample_rows(const nsp_sample_params* s, void* stream) {
   a.V = (int)s->V;
   a.k_all = s->k_all > 0x7fffffffLL ? 0x7fffffff : (int)(s->k_all < 0 ? 0 : s->k_all);
   a.t_all = (float)s->t_all; a.tp_all = (float)s->tp_all; a.mp_all = (float)s->mp_all;
-  if (s->dtype == NSP_DT_F32) return launch_sample<float>(a, s->rows, (hipStream_t)stream);
-  if (s->dtype == NSP_DT_BF16) return launch_sample<__bf16>(a, s->rows, (hipStream_t)stream);
+  if (s->dtype == NSP_DT_F32) return launch_sample_v<float>(a, s->rows, (hipStream_t)stream);
+  if (s->dtype == NSP_DT_BF16) return launch_sample_v<__bf16>(a, s->rows, (hipStream_t)stream);
   return NSP_EUNSUPPORTED;
 }

@@ -2151,29 +2151,22 @@ def lstm_cell_step(gates, h_prev, c_prev, update=None):
 # decoder operators: attention over a paged cache / over encoder states, sampling (csrc/paged_attn.hip, csrc/sample.hip)
 # --------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
-_DECODE_PACK = _struct.Struct('<31qd').pack         # nsp_decode_attn_params
-_APPEND_PACK = _struct.Struct('<28q').pack          # nsp_paged_append_params
-_SAMPLE_PACK = _struct.Struct('<12q3d').pack        # nsp_sample_params
-_DECODE_WS = {}                                     # call sizes -> workspace bytes (a pure function of them)
+# The parameter structs are pointers followed by what only depends on the call's sizes, strides and types.  The second part is
+# packed and the call checked once per combination of these (a program makes a few) and kept here under it: checks, strides
+# and struct.pack of a whole call cost more host time than the small kernels take on the device.
+_PLANS = {}
+_DECODE_PTRS, _DECODE_TAIL = _struct.Struct('<9q').pack, _struct.Struct('<22qd').pack        # nsp_decode_attn_params
+_APPEND_PTRS, _APPEND_TAIL = _struct.Struct('<7q').pack, _struct.Struct('<21q').pack         # nsp_paged_append_params
+_CROSS_PTRS, _CROSS_TAIL = _struct.Struct('<12q3q2Q').pack, _struct.Struct('<16q2d').pack    # nsp_cross_attn_params
+_SAMPLE_PACK = _struct.Struct('<12q3d').pack                                                 # nsp_sample_params
 
 
-def _one_device(*tensors):
-    """every tensor is where the kernels run, and on one device"""
-    _require_device(*tensors)
-    dev = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError('tensors on different devices: %s and %s' % (dev, t.device))
-    return dev
-
-
-class _on(object):
-    """make `dev` the current device around a launch when it is not (its stream is then that device's current one)"""
-
-    def __new__(cls, dev):
-        if dev.type != 'cuda' or dev.index is None or dev.index == torch._C._cuda_getDevice():
-            return _NULL_CTX
-        return torch.cuda.device(dev)
+def _plan(key, make, *args):
+    plan = make(*args)
+    if len(_PLANS) > 4096:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
 
 
 class _NoCtx(object):
@@ -2187,10 +2180,20 @@ class _NoCtx(object):
 _NULL_CTX = _NoCtx()
 
 
-def _vec_ok(t):
+def _on(dev):
+    """context that makes device number `dev` current around a launch when it is not (whose stream is then that device's
+    current one)"""
+    if dev < 0 or dev == torch._C._cuda_getDevice():
+        return _NULL_CTX
+    return torch.cuda.device(dev)
+
+
+def _devices_differ(*tensors):
+    raise ValueError('tensors on different devices: %s' % ', '.join(str(t.device) for t in tensors if t is not None))
+
+
+def _vec_strides(t):
     """rows the kernels can read 16 bytes at a time: last dimension contiguous, the other strides multiples of 8"""
-    if t.data_ptr() % 16:
-        return False
     st, sz = t.stride(), t.shape
     if st[-1] != 1 and sz[-1] != 1:
         return False
@@ -2201,49 +2204,74 @@ def _vec_ok(t):
 
 
 def _vec(t):
-    return t if _vec_ok(t) else t.clone(memory_format=torch.contiguous_format)
+    """t, or a copy the kernels can read 16 bytes at a time"""
+    return t if t.data_ptr() % 16 == 0 and _vec_strides(t) else t.clone(memory_format=torch.contiguous_format)
 
 
-def _int32_vec(t, n, what):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n:
-        raise ValueError('%s: int32 [%d] expected, got %s %s' % (what, n, t.dtype, tuple(t.shape)))
-    return t if t.is_contiguous() else t.contiguous()
+def _need(t, dtype, shape, what):
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError('%s: %s %s expected, got %s %s' % (what, dtype, list(shape), t.dtype, list(t.shape)))
 
 
-def _head_size_ok(D):
+def _need_head_size(D):
     if D % 8 or not 0 < D <= 128:
         raise ValueError('head size %d: multiples of 8 up to 128 are supported' % D)
 
 
-def _check_pages(k_pages, v_pages, block_table, B, Hkv, D):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
-        raise ValueError('k_pages / v_pages: two [n_pages, heads, page, d] tensors of one shape and type expected')
+def _need_pages(k_pages, v_pages, block_table, B, Hkv, D):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.dtype not in _DTYPES:
+        raise ValueError('k_pages / v_pages: two fp32 or bf16 [n_pages, heads, page, d] tensors of one shape and type expected')
     if k_pages.shape[1] != Hkv or k_pages.shape[3] != D or k_pages.shape[2] < 1:
         raise ValueError('pages of shape %s do not hold %d heads of size %d' % (tuple(k_pages.shape), Hkv, D))
-    if not (_vec_ok(k_pages) and _vec_ok(v_pages)):
-        raise ValueError('pages: contiguous last dimension, 16-byte aligned, other strides multiples of 8 elements expected')
+    if not (_vec_strides(k_pages) and _vec_strides(v_pages)):
+        raise ValueError('pages: contiguous last dimension, other strides multiples of 8 elements expected')
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError('block_table: int32 [%d, pages] expected, got %s %s' % (B, block_table.dtype, tuple(block_table.shape)))
     if block_table.shape[1] * k_pages.shape[2] > 0x7fff0000:
         raise ValueError('more than 2^31 positions in a block table row')
 
 
-def _decode_attn(dev, q, out, k, v, table, lens, k_new, v_new, B, H, Hkv, D, Tq, page, n_pages, width, qs, ks, vs, ns, scale):
-    key = (B, H, Hkv, Tq, D, width * page)
-    nb = _DECODE_WS.get(key)
-    if nb is None:
-        if len(_DECODE_WS) > 4096:
-            _DECODE_WS.clear()
-        nb = _DECODE_WS[key] = _lib.lib().nsp_decode_attn_workspace_bytes(*key)
-    with _on(dev):
-        ws = torch.empty((nb // 4,), device=dev, dtype=torch.float32) if nb else None
-        _check(_lib.lib().nsp_decode_attn(_DECODE_PACK(
-            q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr() if table is not None else 0,
-            lens.data_ptr() if lens is not None else 0, k_new.data_ptr() if k_new is not None else 0,
-            v_new.data_ptr() if v_new is not None else 0, ws.data_ptr() if ws is not None else 0,
-            B, H, Hkv, D, Tq, page, n_pages, width, _DTYPES[q.dtype], *qs, *ks, *vs, *ns, scale), _stream()),
-            'nsp_decode_attn')
-    return out
+def _need_aligned(*pages):
+    for t in pages:
+        if t.data_ptr() % 16:
+            raise ValueError('pages: 16-byte aligned memory expected')
+
+
+def _decode_tail(B, H, Hkv, D, Tq, page, n_pages, width, dtype, qs, ks, vs, ns, scale):
+    """-> (constant part of nsp_decode_attn_params, workspace floats)"""
+    nb = _lib.lib().nsp_decode_attn_workspace_bytes(B, H, Hkv, Tq, D, width * page)
+    return _DECODE_TAIL(B, H, Hkv, D, Tq, page, n_pages, width, _DTYPES[dtype], *qs, *ks, *vs, *ns, scale), nb // 4
+
+
+def _paged_plan(q, k_pages, v_pages, block_table, lens, k_new, v_new, scale):
+    if q.dim() != 3 or q.dtype not in _DTYPES:
+        raise ValueError('q: fp32 or bf16 [B,H,d] expected, got %s %s' % (q.dtype, tuple(q.shape)))
+    B, H, D = q.shape
+    Hkv = k_pages.shape[1] if k_pages.dim() == 4 else 0
+    if Hkv < 1 or H % Hkv or H < 1:
+        raise ValueError('%d query heads over %d key heads' % (H, Hkv))
+    _need_head_size(D)
+    if k_pages.dtype != q.dtype:
+        raise ValueError('q is %s, the cache %s' % (q.dtype, k_pages.dtype))
+    _need_pages(k_pages, v_pages, block_table, B, Hkv, D)
+    _need(lens, torch.int32, (B,), 'lens')
+    if (k_new is None) != (v_new is None):
+        raise ValueError('k_new and v_new come together')
+    ns = (0, 0, 0, 0)
+    as_is = _vec_strides(q) and block_table.is_contiguous() and lens.is_contiguous()
+    if k_new is not None:
+        _need(k_new, q.dtype, (B, Hkv, D), 'k_new')
+        _need(v_new, q.dtype, (B, Hkv, D), 'v_new')
+        as_is = as_is and _vec_strides(k_new) and _vec_strides(v_new)
+        ns = (k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1))
+    scale = D ** -0.5 if scale is None else float(scale)
+    if B == 0 or block_table.shape[1] == 0 or k_pages.shape[0] == 0:
+        return 'zeros', None, 0               # no sequence, or no key and no room
+    if not as_is:
+        return 'copy', None, 0
+    qs, ks, vs = q.stride(), k_pages.stride(), v_pages.stride()
+    return ('call',) + _decode_tail(B, H, Hkv, D, 1, k_pages.shape[2], k_pages.shape[0], block_table.shape[1], q.dtype,
+                                    (qs[0], 0, qs[1]), (ks[0], ks[2], ks[1]), (vs[0], vs[2], vs[1]), ns, scale)
 
 
 def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=None, scale=None):
@@ -2259,36 +2287,59 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
     Table entries behind a sequence's last page are not read; an entry outside [0, n_pages) is an absent page: its keys do
     not count and a new token that would lie there, or behind the table, is neither stored nor attended to.  No two rows may
     share the page that a new token is stored to."""
-    dev = _one_device(q, k_pages, v_pages, block_table, lens, k_new, v_new)
-    if q.dim() != 3 or q.dtype not in _DTYPES:
-        raise ValueError('q: fp32 or bf16 [B,H,d] expected, got %s %s' % (q.dtype, tuple(q.shape)))
-    B, H, D = q.shape
-    Hkv = k_pages.shape[1] if k_pages.dim() == 4 else 0
-    if Hkv < 1 or H % Hkv or H < 1:
-        raise ValueError('%d query heads over %d key heads' % (H, Hkv))
-    _head_size_ok(D)
-    if k_pages.dtype != q.dtype:
-        raise ValueError('q is %s, the cache %s' % (q.dtype, k_pages.dtype))
-    _check_pages(k_pages, v_pages, block_table, B, Hkv, D)
-    lens = _int32_vec(lens, B, 'lens')
-    if (k_new is None) != (v_new is None):
-        raise ValueError('k_new and v_new come together')
-    ns = (0, 0, 0, 0)
-    if k_new is not None:
-        for t in (k_new, v_new):
-            if tuple(t.shape) != (B, Hkv, D) or t.dtype != q.dtype:
-                raise ValueError('k_new / v_new: %s [%d,%d,%d] expected, got %s %s' % (q.dtype, B, Hkv, D, t.dtype, tuple(t.shape)))
-        k_new, v_new = _vec(k_new), _vec(v_new)
-        ns = (k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1))
-    if B == 0 or block_table.shape[1] == 0 or k_pages.shape[0] == 0:      # no sequence, or no key and no room
-        return torch.zeros((B, H, D), device=dev, dtype=q.dtype)
-    out = torch.empty((B, H, D), device=dev, dtype=q.dtype)
-    q = _vec(q)
-    block_table = block_table if block_table.is_contiguous() else block_table.contiguous()
-    qs, ks, vs = q.stride(), k_pages.stride(), v_pages.stride()
-    return _decode_attn(dev, q, out, k_pages, v_pages, block_table, lens, k_new, v_new, B, H, Hkv, D, 1, k_pages.shape[2],
-                        k_pages.shape[0], block_table.shape[1], (qs[0], 0, qs[1]), (ks[0], ks[2], ks[1]),
-                        (vs[0], vs[2], vs[1]), ns, D ** -0.5 if scale is None else float(scale))
+    _require_device(q)
+    dev = q.get_device()
+    if k_pages.get_device() != dev or v_pages.get_device() != dev or block_table.get_device() != dev or lens.get_device() != dev:
+        _devices_differ(q, k_pages, v_pages, block_table, lens)
+    if k_new is None or v_new is None:
+        key = ('paged', q.shape, q.stride(), q.dtype, k_pages.shape, k_pages.stride(), k_pages.dtype, v_pages.shape,
+               v_pages.stride(), v_pages.dtype, block_table.shape, block_table.stride(), block_table.dtype, lens.shape,
+               lens.stride(), lens.dtype, scale, k_new is None, v_new is None)
+        kn = vn = 0
+    else:
+        if k_new.get_device() != dev or v_new.get_device() != dev:
+            _devices_differ(q, k_new, v_new)
+        key = ('paged', q.shape, q.stride(), q.dtype, k_pages.shape, k_pages.stride(), k_pages.dtype, v_pages.shape,
+               v_pages.stride(), v_pages.dtype, block_table.shape, block_table.stride(), block_table.dtype, lens.shape,
+               lens.stride(), lens.dtype, scale, k_new.shape, k_new.stride(), k_new.dtype, v_new.shape, v_new.stride(), v_new.dtype)
+        kn, vn = k_new.data_ptr(), v_new.data_ptr()
+    how, tail, ws_floats = _PLANS.get(key) or _plan(key, _paged_plan, q, k_pages, v_pages, block_table, lens, k_new, v_new, scale)
+    if how == 'zeros':
+        return torch.zeros(q.shape, device=q.device, dtype=q.dtype)
+    qa, ka, va = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
+    if how == 'copy' or (qa | ka | va | kn | vn) & 15:
+        _need_aligned(k_pages, v_pages)
+        return paged_attention(_vec(q), k_pages, v_pages, block_table.contiguous(), lens.contiguous(),
+                               None if k_new is None else _vec(k_new), None if v_new is None else _vec(v_new), scale)
+    with _on(dev):
+        out = q.new_empty(q.shape)
+        ws = q.new_empty((ws_floats,), dtype=torch.float32) if ws_floats else None
+        _check(_lib.lib().nsp_decode_attn(_DECODE_PTRS(
+            qa, out.data_ptr(), ka, va, block_table.data_ptr(), lens.data_ptr(), kn, vn, ws.data_ptr() if ws_floats else 0) + tail,
+            _stream()), 'nsp_decode_attn')
+    return out
+
+
+def _append_plan(k, v, k_pages, v_pages, block_table, starts, counts):
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DTYPES:
+        raise ValueError('k / v: two fp32 or bf16 [B,n,Hkv,d] tensors of one shape and type expected')
+    B, n, Hkv, D = k.shape
+    _need_head_size(D)
+    _need_pages(k_pages, v_pages, block_table, B, Hkv, D)
+    if k.dtype == torch.bfloat16 and k_pages.dtype != torch.bfloat16:
+        raise ValueError('%s into a %s cache' % (k.dtype, k_pages.dtype))
+    _need(starts, torch.int32, (B,), 'starts')
+    if counts is not None:
+        _need(counts, torch.int32, (B,), 'counts')
+    if B == 0 or n == 0 or block_table.shape[1] == 0 or k_pages.shape[0] == 0:
+        return 'nothing', None
+    if not (_vec_strides(k) and _vec_strides(v) and block_table.is_contiguous() and starts.is_contiguous()
+            and (counts is None or counts.is_contiguous())):
+        return 'copy', None
+    ks, vs, kp, vp = k.stride(), v.stride(), k_pages.stride(), v_pages.stride()
+    return 'call', _APPEND_TAIL(B, n, Hkv, D, k_pages.shape[2], k_pages.shape[0], block_table.shape[1], _DTYPES[k.dtype],
+                                _DTYPES[k_pages.dtype], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kp[0], kp[2], kp[1],
+                                vp[0], vp[2], vp[1])
 
 
 def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
@@ -2298,83 +2349,102 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
     offered); token t of row b goes to position starts[b] + t of its block_table row for t < counts[b] (all n without
     counts).  starts[b] < 0, absent pages (entries outside [0, n_pages)) and positions behind the table: nothing is written.
     No position may be written twice by one call."""
-    dev = _one_device(k, v, k_pages, v_pages, block_table, starts, counts)
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DTYPES:
-        raise ValueError('k / v: two fp32 or bf16 [B,n,Hkv,d] tensors of one shape and type expected')
-    B, n, Hkv, D = k.shape
-    _head_size_ok(D)
-    _check_pages(k_pages, v_pages, block_table, B, Hkv, D)
-    if k_pages.dtype not in _DTYPES or (k.dtype == torch.bfloat16 and k_pages.dtype != torch.bfloat16):
-        raise ValueError('%s into a %s cache' % (k.dtype, k_pages.dtype))
-    starts = _int32_vec(starts, B, 'starts')
-    counts = _int32_vec(counts, B, 'counts') if counts is not None else None
-    if B == 0 or n == 0 or block_table.shape[1] == 0 or k_pages.shape[0] == 0:
+    _require_device(k)
+    dev = k.get_device()
+    if v.get_device() != dev or k_pages.get_device() != dev or v_pages.get_device() != dev or \
+            block_table.get_device() != dev or starts.get_device() != dev or (counts is not None and counts.get_device() != dev):
+        _devices_differ(k, v, k_pages, v_pages, block_table, starts, counts)
+    key = ('append', k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, k_pages.shape, k_pages.stride(), k_pages.dtype,
+           v_pages.shape, v_pages.stride(), v_pages.dtype, block_table.shape, block_table.stride(), block_table.dtype,
+           starts.shape, starts.stride(), starts.dtype,
+           None if counts is None else (counts.shape, counts.stride(), counts.dtype))
+    how, tail = _PLANS.get(key) or _plan(key, _append_plan, k, v, k_pages, v_pages, block_table, starts, counts)
+    if how == 'nothing':
         return
-    k, v = _vec(k), _vec(v)
-    block_table = block_table if block_table.is_contiguous() else block_table.contiguous()
-    ks, vs, kp, vp = k.stride(), v.stride(), k_pages.stride(), v_pages.stride()
+    ka, va, kp, vp = k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
+    if how == 'copy' or (ka | va | kp | vp) & 15:
+        _need_aligned(k_pages, v_pages)
+        return paged_append(_vec(k), _vec(v), k_pages, v_pages, block_table.contiguous(), starts.contiguous(),
+                            None if counts is None else counts.contiguous())
     with _on(dev):
-        _check(_lib.lib().nsp_paged_append(_APPEND_PACK(
-            k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), starts.data_ptr(),
-            counts.data_ptr() if counts is not None else 0, B, n, Hkv, D, k_pages.shape[2], k_pages.shape[0],
-            block_table.shape[1], _DTYPES[k.dtype], _DTYPES[k_pages.dtype], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-            kp[0], kp[2], kp[1], vp[0], vp[2], vp[1]), _stream()), 'nsp_paged_append')
-
-
-_CROSS_PACK = _struct.Struct('<31q2Q2d').pack       # nsp_cross_attn_params
-
-
-def _cross_call(name, dev, q, k, v, dout, out, o_lo, dq, dk, dv, stats, dsum, klens, sizes, scale, p, seed, offset):
-    def at(t):
-        return t.data_ptr() if t is not None else 0
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    gs = dout.stride() if dout is not None else (0, 0, 0, 0)
-    with _on(dev):
-        _check(getattr(_lib.lib(), name)(_CROSS_PACK(
-            at(q), at(k), at(v), at(dout), at(out), at(o_lo), at(dq), at(dk), at(dv), at(stats), at(dsum), at(klens), *sizes,
-            _DTYPES[q.dtype], qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], gs[0], gs[1], gs[2], seed, offset,
-            scale, p), _stream()), name)
+        _check(_lib.lib().nsp_paged_append(_APPEND_PTRS(
+            ka, va, kp, vp, block_table.data_ptr(), starts.data_ptr(), 0 if counts is None else counts.data_ptr()) + tail,
+            _stream()), 'nsp_paged_append')
 
 
 class CrossAttnFn(torch.autograd.Function):
-    """cross_attention with its backward (csrc/cross_attn.hip); arguments as checked there."""
+    """cross_attention with its backward (csrc/cross_attn.hip); arguments as checked there.  One buffer holds what backward
+    needs beside the inputs and the output: stats [2,B,H,Tq] and backward's scratch [B,H,Tq] (fp32), and for bf16 what the
+    rounding of the output left."""
 
     @staticmethod
-    def forward(ctx, q, k, v, klens, scale, p, seed, offset):
-        B, Tq, H, D = q.shape
-        Tk, Hkv = k.shape[1], k.shape[2]
-        dev = q.device
-        sizes = (B, H, Hkv, D, Tq, Tk)
-        ctx.empty = B == 0 or Tq == 0 or Tk == 0      # nothing to read: zeros, with zero gradients
-        if ctx.empty:
+    def forward(ctx, q, k, v, klens, tail, seed, need):
+        out = q.new_empty(q.shape)
+        rows = out.numel()
+        if k.numel() == 0 or rows == 0:       # nothing to read: zeros, with zero gradients
+            ctx.empty = True
             ctx.save_for_backward(q, k, v)
-            return torch.zeros((B, Tq, H, D), device=dev, dtype=q.dtype)
-        out = torch.empty((B, Tq, H, D), device=dev, dtype=q.dtype)
-        q, k, v = _vec(q), _vec(k), _vec(v)
-        need = any(ctx.needs_input_grad[:3])
-        stats = torch.empty((2, B, H, Tq), device=dev, dtype=torch.float32) if need else None
-        o_lo = torch.empty_like(out) if need and q.dtype == torch.bfloat16 else None
-        _cross_call('nsp_cross_attn_fwd', dev, q, k, v, None, out, o_lo, None, None, None, stats, None, klens, sizes, scale, p,
-                    seed, offset)
-        ctx.save_for_backward(q, k, v, klens, out, o_lo, stats)
-        ctx.cfg = (sizes, scale, p, seed, offset)
+            return out.zero_()
+        buf, at, lo = None, 0, 0
+        if need:
+            half = q.dtype == torch.bfloat16
+            D = q.shape[3]
+            lo = (12 * (rows // D) + 15) // 16 * 16
+            buf = q.new_empty(((lo + 2 * rows if half else lo) // 4,), dtype=torch.float32)
+            at = buf.data_ptr()
+            lo = at + lo if half else 0
+        with _on(q.get_device()):
+            _check(_lib.lib().nsp_cross_attn_fwd(_CROSS_PTRS(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), lo, 0, 0, 0, at, 0,
+                0 if klens is None else klens.data_ptr(), 0, 0, 0, seed, 0) + tail, _stream()), 'nsp_cross_attn_fwd')
+        if need:
+            ctx.empty, ctx.tail, ctx.seed = False, tail, seed
+            ctx.save_for_backward(q, k, v, klens, out, buf)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         if ctx.empty:
-            return tuple(torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * 5
-        q, k, v, klens, out, o_lo, stats = ctx.saved_tensors
-        (B, H, Hkv, D, Tq, Tk), scale, p, seed, offset = ctx.cfg
-        dev = q.device
-        dout = _vec(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-        dq = torch.empty((B, Tq, H, D), device=dev, dtype=q.dtype)
-        dk = torch.empty((B, Tk, Hkv, D), device=dev, dtype=q.dtype)
-        dv = torch.empty((B, Tk, Hkv, D), device=dev, dtype=q.dtype)
-        dsum = torch.empty((B, H, Tq), device=dev, dtype=torch.float32)
-        _cross_call('nsp_cross_attn_bwd', dev, q, k, v, dout, out, o_lo, dq, dk, dv, stats, dsum, klens, ctx.cfg[0], scale, p,
-                    seed, offset)
-        return dq, dk, dv, None, None, None, None, None
+            return tuple(torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * 4
+        q, k, v, klens, out, buf = ctx.saved_tensors
+        if dout.dtype != q.dtype or not dout.is_contiguous() or dout.data_ptr() & 15:
+            dout = _vec(dout.to(q.dtype))
+        g0, g1, g2, _ = dout.stride()
+        dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
+        n = q.numel() // q.shape[3]
+        at = buf.data_ptr()
+        with _on(q.get_device()):
+            _check(_lib.lib().nsp_cross_attn_bwd(_CROSS_PTRS(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(),
+                at + (12 * n + 15) // 16 * 16 if q.dtype == torch.bfloat16 else 0, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                at, at + 8 * n, 0 if klens is None else klens.data_ptr(), g0, g1, g2, ctx.seed, 0) + ctx.tail, _stream()),
+                'nsp_cross_attn_bwd')
+        return dq, dk, dv, None, None, None, None
+
+
+def _cross_plan(q, k, v, klens, scale, dropout_p):
+    """-> (can the strides be read, constant part for the training kernels, the same for the single-token kernel if it may take
+    the call, its workspace floats)"""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError('q [B,Tq,H,d] and k / v [B,Tk,Hkv,d], all fp32 or all bf16, expected: got %s %s, %s %s, %s %s' % (
+            q.dtype, tuple(q.shape), k.dtype, tuple(k.shape), v.dtype, tuple(v.shape)))
+    B, Tq, H, D = q.shape
+    Tk, Hkv = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D or Hkv < 1 or H < 1 or H % Hkv:
+        raise ValueError('q %s does not go with k %s' % (tuple(q.shape), tuple(k.shape)))
+    _need_head_size(D)
+    if klens is not None:
+        _need(klens, torch.int32, (B,), 'klens')
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale) and 0.0 <= dropout_p < 1.0):
+        raise ValueError('scale %r, dropout_p %r' % (scale, dropout_p))
+    if not (_vec_strides(q) and _vec_strides(k) and _vec_strides(v) and (klens is None or klens.is_contiguous())):
+        return False, None, None, 0
+    st = [t.stride()[:3] for t in (q, k, v)]
+    tail = _CROSS_TAIL(B, H, Hkv, D, Tq, Tk, _DTYPES[q.dtype], *st[0], *st[1], *st[2], scale, dropout_p)
+    few = dropout_p == 0 and Tq * (H // Hkv) <= 16 and B > 0 and Tq > 0 and Tk > 0
+    one, floats = _decode_tail(B, H, Hkv, D, Tq, 1, 0, Tk, q.dtype, *st, (0, 0, 0, 0), scale) if few else (None, 0)
+    return True, tail, one, floats
 
 
 def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
@@ -2389,39 +2459,36 @@ def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
 
     Without gradients and dropout, calls of up to 16 query rows per key head (Tq * H / Hkv) take the kernel that splits the
     keys over workgroups: the single-token form of decoding."""
-    dev = _one_device(q, k, v, klens)
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError('q [B,Tq,H,d] and k / v [B,Tk,Hkv,d], all fp32 or all bf16, expected: got %s %s, %s %s, %s %s' % (
-            q.dtype, tuple(q.shape), k.dtype, tuple(k.shape), v.dtype, tuple(v.shape)))
-    B, Tq, H, D = q.shape
-    Tk, Hkv = k.shape[1], k.shape[2]
-    if k.shape[0] != B or k.shape[3] != D or Hkv < 1 or H < 1 or H % Hkv:
-        raise ValueError('q %s does not go with k %s' % (tuple(q.shape), tuple(k.shape)))
-    _head_size_ok(D)
-    if klens is not None:
-        klens = _int32_vec(klens, B, 'klens')
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not (scale > 0 and 0.0 <= dropout_p < 1.0):
-        raise ValueError('scale %r, dropout_p %r' % (scale, dropout_p))
-    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    if not grad and dropout_p == 0 and Tq * (H // Hkv) <= 16 and B > 0 and Tq > 0 and Tk > 0:
-        out = torch.empty((B, Tq, H, D), device=dev, dtype=q.dtype)
-        q, k, v = _vec(q), _vec(k), _vec(v)
-        qs, ks, vs = q.stride(), k.stride(), v.stride()
-        return _decode_attn(dev, q, out, k, v, None, klens, None, None, B, H, Hkv, D, Tq, 1, 0, Tk, qs[:3], ks[:3], vs[:3],
-                            (0, 0, 0, 0), scale)
-    seed, offset = next_dropout_seed() if dropout_p > 0 else (0, 0)
-    return CrossAttnFn.apply(q, k, v, klens, scale, float(dropout_p), seed, offset)
+    _require_device(q)
+    dev = q.get_device()
+    if k.get_device() != dev or v.get_device() != dev or (klens is not None and klens.get_device() != dev):
+        _devices_differ(q, k, v, klens)
+    key = ('cross', q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype,
+           None if klens is None else (klens.shape, klens.stride(), klens.dtype), scale, dropout_p)
+    as_is, tail, one, floats = _PLANS.get(key) or _plan(key, _cross_plan, q, k, v, klens, scale, dropout_p)
+    qa, ka, va = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if not as_is or (qa | ka | va) & 15:
+        return cross_attention(_vec(q), _vec(k), _vec(v), klens if klens is None else klens.contiguous(), scale, dropout_p)
+    need = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
+    if one is not None and not need:
+        with _on(dev):
+            out = q.new_empty(q.shape)
+            ws = q.new_empty((floats,), dtype=torch.float32) if floats else None
+            _check(_lib.lib().nsp_decode_attn(_DECODE_PTRS(
+                qa, out.data_ptr(), ka, va, 0, 0 if klens is None else klens.data_ptr(), 0, 0, ws.data_ptr() if floats else 0)
+                + one, _stream()), 'nsp_decode_attn')
+        return out
+    return CrossAttnFn.apply(q, k, v, klens, tail, next_dropout_seed()[0] if dropout_p > 0 else 0, need)
 
 
 def _sample_setting(x, dtype, rows, dev, what):
-    """(device address or 0, value) of a per-row tensor or a number"""
+    """(device address or 0, value) of a per-row tensor or a number; a tensor has to stay alive over the launch"""
     if not torch.is_tensor(x):
-        return None, (int(x) if dtype == torch.int32 else float(x))
-    _one_device(x)
-    if x.device != dev or x.dtype != dtype or x.dim() != 1 or x.shape[0] != rows:
-        raise ValueError('%s: a number or %s [%d] on %s expected, got %s %s' % (what, dtype, rows, dev, x.dtype, tuple(x.shape)))
-    return (x if x.is_contiguous() else x.contiguous()), 0
+        return 0, x
+    if x.get_device() != dev or x.dtype != dtype or x.dim() != 1 or x.shape[0] != rows or not x.is_contiguous():
+        raise ValueError('%s: a number or a contiguous %s [%d] beside the logits expected, got %s %s on %s' % (
+            what, dtype, rows, x.dtype, tuple(x.shape), x.device))
+    return x.data_ptr(), 0
 
 
 def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -2433,31 +2500,33 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     ones with w_i >= min_p; the first always.  The token is the first kept index whose mass together with the kept indices
     before it exceeds u x the kept mass.  temperature <= 0 is the arg-max (as argmax_rows).  A NaN logit counts as -inf, a
     +inf logit takes all the mass; rows without a logit above -inf give their first entry."""
-    dev = _one_device(logits, u)
+    _require_device(logits)
+    dev = logits.get_device()
     if logits.dim() != 2 or logits.dtype not in _DTYPES or logits.shape[1] < 1:
         raise ValueError('logits: fp32 or bf16 [rows,V] expected, got %s %s' % (logits.dtype, tuple(logits.shape)))
     rows, V = logits.shape
     if V > 1 << 18:
         raise ValueError('vocabularies up to 2^18 are supported, got %d' % V)
-    if u.dtype != torch.float32 or u.dim() != 1 or u.shape[0] != rows:
-        raise ValueError('u: fp32 [%d] expected, got %s %s' % (rows, u.dtype, tuple(u.shape)))
+    if u.get_device() != dev:
+        _devices_differ(logits, u)
+    _need(u, torch.float32, (rows,), 'u')
     t, t_all = _sample_setting(temperature, torch.float32, rows, dev, 'temperature')
     k, k_all = _sample_setting(top_k, torch.int32, rows, dev, 'top_k')
     tp, tp_all = _sample_setting(top_p, torch.float32, rows, dev, 'top_p')
     mp, mp_all = _sample_setting(min_p, torch.float32, rows, dev, 'min_p')
-    out = torch.empty((rows,), device=dev, dtype=torch.int32)
-    if rows == 0:
-        return out
-    if (logits.stride(1) != 1 and V > 1) or (logits.stride(0) < V and rows > 1):
-        logits = logits.contiguous()
-    u = u if u.is_contiguous() else u.contiguous()
-    ld = logits.stride(0)
     with _on(dev):
+        out = torch.empty((rows,), device=logits.device, dtype=torch.int32)
+        if rows == 0:
+            return out
+        ld, step = logits.stride()
+        if (step != 1 and V > 1) or (ld < V and rows > 1):
+            logits = logits.contiguous()
+            ld = V
+        if not u.is_contiguous():
+            u = u.contiguous()
         _check(_lib.lib().nsp_sample_rows(_SAMPLE_PACK(
-            logits.data_ptr(), u.data_ptr(), t.data_ptr() if t is not None else 0, k.data_ptr() if k is not None else 0,
-            tp.data_ptr() if tp is not None else 0, mp.data_ptr() if mp is not None else 0, out.data_ptr(), rows, V,
-            ld if rows > 1 else V, _DTYPES[logits.dtype], min(max(k_all, 0), V), t_all, tp_all, mp_all), _stream()),
-            'nsp_sample_rows')
+            logits.data_ptr(), u.data_ptr(), t, k, tp, mp, out.data_ptr(), rows, V, ld if rows > 1 else V,
+            _DTYPES[logits.dtype], min(max(k_all, 0), V), t_all, tp_all, mp_all), _stream()), 'nsp_sample_rows')
     return out
 
 

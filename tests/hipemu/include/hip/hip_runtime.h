@@ -97,6 +97,8 @@ struct int2 { int x, y; };
 static inline float2 make_float2(float x, float y) { return float2{x, y}; }
 static inline float4 make_float4(float x, float y, float z, float w) { return float4{x, y, z, w}; }
 static inline int4 make_int4(int x, int y, int z, int w) { return int4{x, y, z, w}; }
+struct ulonglong2 { unsigned long long x, y; };
+static inline ulonglong2 make_ulonglong2(unsigned long long x, unsigned long long y) { return ulonglong2{x, y}; }
 static inline int2 make_int2(int x, int y) { return int2{x, y}; }
 struct alignas(16) uint4 { unsigned x, y, z, w; };
 static inline uint4 make_uint4(unsigned x, unsigned y, unsigned z, unsigned w) { return uint4{x, y, z, w}; }
@@ -239,8 +241,24 @@ static inline int hipemu_src_quad(int lane, int ctrl) {
   if (ctrl == 0x141) return (lane & ~7) | (7 - (lane & 7));
   return (lane & ~3) | ((ctrl >> (2 * (lane & 3))) & 3);
 }
-static inline int __builtin_amdgcn_update_dpp(int /*old*/, int src, int ctrl, int /*row_mask*/, int /*bank_mask*/, bool /*bound_ctrl*/) {
-  return hipemu_shfl(src, hipemu_src_quad, ctrl);
+// + row_shr:n (0x110 | n: lane l reads lane l - n of its row), row_bcast:15 (0x142: lane 15 of the row before) and
+// row_bcast:31 (0x143: lane 31, into rows 2 and 3); lanes without a source read 0 (bound_ctrl), rows outside row_mask get `old`
+static inline int __builtin_amdgcn_update_dpp(int old, int src, int ctrl, int row_mask, int /*bank_mask*/, bool /*bound_ctrl*/) {
+  const int lane = hipemu::tid_flat & 63, row = lane >> 4;
+  int v;
+  if (ctrl > 0x110 && ctrl < 0x120) {
+    v = hipemu_shfl(src, hipemu_src_up, ctrl & 15);
+    if ((lane & 15) < (ctrl & 15)) v = 0;
+  } else if (ctrl == 0x142) {
+    v = hipemu_shfl(src, hipemu_src_idx, row > 0 ? 16 * row - 1 : 0);
+    if (row == 0) v = 0;
+  } else if (ctrl == 0x143) {
+    v = hipemu_shfl(src, hipemu_src_idx, 31);
+    if (row < 2) v = 0;
+  } else {
+    v = hipemu_shfl(src, hipemu_src_quad, ctrl);
+  }
+  return ((row_mask >> row) & 1) ? v : old;
 }
 
 // ---- MFMA as a wave collective (register layouts: cdna_hip_programming.md, "Fragment layout") ----
