@@ -10,19 +10,19 @@
 // answer now and then.  Masses are therefore fixed-point integers, w x 2^44 from a 64-bit exponential: integer sums have no
 // order, and borders move by less than 2^-44 of the largest mass per entry.
 //
-// One workgroup per row: 4 waves for rows of up to 1024 logits, where latency is all, else 16.  A row is read once and stays in
-// LDS, up to 11000 logits with their masses, so that the 64-bit exponential runs once per entry; rows behind 32768 logits
+// One workgroup per row: 4 waves for rows of up to 1024 logits, where latency is all, else 8.  A row is read once and stays in
+// LDS, up to 10800 logits with their masses, so that the 64-bit exponential runs once per entry; rows behind 30000 logits
 // are read again by each pass (from L2).  The k-th entry and the entry that completes top_p are found with one histogram
 // whose bins are linear in the logit between the row's extremes, a scan, and an exact ranking of the few entries of the bin
 // that the border falls in; rows with too many entries in that bin (equal logits) take a radix descent over (logit, index).
-// What bounds the call is latency: about twenty barriers, and scans over a wave, which therefore run on DPP lane moves
-// (8 cycles a step, where a shuffle through LDS takes about 130).
+// What bounds the call is latency: about a dozen barriers, and scans over a wave, which therefore run on DPP lane moves
+// (a step takes a few cycles, where a shuffle through LDS takes about 130), and the issue of what every wave has to do.
 #include "common.h"
 
 namespace {
 
 typedef unsigned long long u64;
-constexpr int CAND = 512;     // entries that are ranked one against the other
+constexpr int CAND = 256;     // entries that are ranked one against the other
 constexpr int FRAC = 44;      // bits behind the point of a mass; V <= 2^18 keeps every sum below 2^62
 // what of the row the LDS holds
 enum { NOTHING = 0, LOGITS = 1, LOGITS_AND_MASSES = 2 };
@@ -41,8 +41,18 @@ struct SampleArgs {
   float t_all, tp_all, mp_all;
 };
 
-__device__ __forceinline__ float sample_load(const float* p) { return *p; }
-__device__ __forceinline__ float sample_load(const __bf16* p) { return (float)*p; }
+// four consecutive logits at any address (the memory system takes unaligned vectors)
+typedef __attribute__((ext_vector_type(4), aligned(4))) float f32x4_any;
+typedef __attribute__((ext_vector_type(4), aligned(2))) unsigned short u16x4_any;
+__device__ __forceinline__ void sample_load4(const float* p, float (&y)[4]) {
+  const f32x4_any v = *reinterpret_cast<const f32x4_any*>(p);
+  y[0] = v[0]; y[1] = v[1]; y[2] = v[2]; y[3] = v[3];
+}
+__device__ __forceinline__ void sample_load4(const __bf16* p, float (&y)[4]) {
+  const u16x4_any v = *reinterpret_cast<const u16x4_any*>(p);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = __uint_as_float((unsigned)v[j] << 16);
+}
 
 // order-preserving image of a logit (-0 counts as 0; a NaN is below everything), and of an entry: larger = earlier
 __device__ __forceinline__ unsigned sample_key(float x) {
@@ -55,12 +65,19 @@ __device__ __forceinline__ u64 sample_entry(float x, int i) {
   return ((u64)sample_key(x) << IDX_BITS) | (u64)((1 << IDX_BITS) - 1 - i);
 }
 
-// exp(d), d <= 0, to better than 2^-46 of its value: exp(d) = 2^n exp(f), |f| <= ln 2 / 2, Taylor to the 12th power
-__device__ __forceinline__ double sample_exp(double d) {
-  const double n = rint(d * 1.4426950408889634074);
+struct RowScale {
+  float xmax;
+  double inv_t;
+};
+// The mass of a logit: exp(d) x 2^44 rounded to a whole number, d = (x - xmax) / T <= 0; relative error of the exponential below
+// 2^-47.  exp(d) = 2^n exp(f), |f| <= ln 2 / 2, Taylor to the 11th power; n and the final rounding come from additions of
+// 1.5 x 2^52 and 2^52, whose low bits then are the whole number (gfx950 has no conversion from 64-bit floats to 64-bit integers).
+__device__ __forceinline__ u64 sample_mass(float x, const RowScale& r) {
+  const double d = x == r.xmax ? 0. : ((double)x - (double)r.xmax) * r.inv_t;
+  const double t = fma(d, 1.4426950408889634074, 6755399441055744.0);
+  const double n = t - 6755399441055744.0;
   const double f = fma(n, -2.3190468138462995584e-17, fma(n, -0.69314718055994528623, d));
-  double s = 1.0 / 479001600.0;
-  s = fma(s, f, 1.0 / 39916800.0);
+  double s = 1.0 / 39916800.0;
   s = fma(s, f, 1.0 / 3628800.0);
   s = fma(s, f, 1.0 / 362880.0);
   s = fma(s, f, 1.0 / 40320.0);
@@ -72,26 +89,17 @@ __device__ __forceinline__ double sample_exp(double d) {
   s = fma(s, f, 0.5);
   s = fma(s, f, 1.0);
   s = fma(s, f, 1.0);
-  return ldexp(s, (int)n);
+  const int e = (int)(unsigned)__builtin_bit_cast(u64, t);         // n
+  const double scale = __builtin_bit_cast(double, (u64)(unsigned)(e + FRAC + 1023) << 52);
+  const u64 m = __builtin_bit_cast(u64, fma(s, scale, 4503599627370496.0)) & ((1ull << 52) - 1);
+  return d > -40.0 ? m : 0ull;       // (below 2^-57: no mass; also a NaN)
 }
-
-struct RowScale {
-  float xmax;
-  double inv_t;
-};
-__device__ __forceinline__ double sample_weight(float x, const RowScale& r) {
-  if (x == r.xmax) return 1.0;
-  const double d = ((double)x - (double)r.xmax) * r.inv_t;
-  return d > -40.0 ? sample_exp(d) : 0.0;       // (below 2^-57: no mass; also a NaN)
-}
-__device__ __forceinline__ u64 sample_mass(double w) { return (u64)(w * (double)(1ull << FRAC) + 0.5); }
 
 struct Mass4 {
   u64 m[4];
 };
 __device__ __forceinline__ Mass4 sample_mass4(float a, float b, float c, float d, const RowScale& rs) {
-  return Mass4{{sample_mass(sample_weight(a, rs)), sample_mass(sample_weight(b, rs)), sample_mass(sample_weight(c, rs)),
-                sample_mass(sample_weight(d, rs))}};
+  return Mass4{{sample_mass(a, rs), sample_mass(b, rs), sample_mass(c, rs), sample_mass(d, rs)}};
 }
 // (for kernels that compute masses in several places: one copy of the code, everything in registers)
 __device__ __attribute__((noinline)) Mass4 sample_mass4_call(float a, float b, float c, float d, float xmax, double inv_t) {
@@ -136,10 +144,14 @@ struct Row {
   ulonglong2* mbuf;  // [chunks][ST][2]
   RowScale rs;
   int V, chunks, tid;
-  __device__ __forceinline__ void load(int c, float (&y)[4]) const {
+  __device__ __forceinline__ void load(int c, float (&y)[4]) const {      // (indices behind the row: anything)
     const int i0 = c * (4 * ST) + 4 * tid;
+    if (i0 + 3 < V) {
+      sample_load4(p + i0, y);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = i0 + j < V ? sample_load(p + i0 + j) : 0.f;
+      for (int j = 0; j < 4; ++j) y[j] = i0 + j < V ? (float)p[i0 + j] : 0.f;
+    }
   }
   __device__ __forceinline__ void get(int c, float (&y)[4]) const {
     if constexpr (KEEP != NOTHING) {
@@ -149,17 +161,20 @@ struct Row {
       load(c, y);
     }
   }
-  // masses of the entries that are not below `floor`
+  // masses of the entries that are not below `floor`, 0 for the others
   __device__ __forceinline__ void compute(const float (&y)[4], int i0, u64 floor, u64 (&m)[4]) const {
-    m[0] = m[1] = m[2] = m[3] = 0;
-    bool any = false;
+    bool in[4], any = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) any = any || (i0 + j < V && sample_entry(y[j], i0 + j) >= floor);
+    for (int j = 0; j < 4; ++j) {
+      in[j] = i0 + j < V && sample_entry(y[j], i0 + j) >= floor;
+      any = any || in[j];
+      m[j] = 0;
+    }
     if (any) {
       const Mass4 w = KEEP == LOGITS_AND_MASSES ? sample_mass4(y[0], y[1], y[2], y[3], rs)
                                                 : sample_mass4_call(y[0], y[1], y[2], y[3], rs.xmax, rs.inv_t);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m[j] = i0 + j < V && sample_entry(y[j], i0 + j) >= floor ? w.m[j] : 0;
+      for (int j = 0; j < 4; ++j) m[j] = in[j] ? w.m[j] : 0;
     }
   }
   // LOGITS_AND_MASSES: the masses the later passes find in LDS
@@ -178,13 +193,16 @@ struct Row {
       }
     }
   }
+  // the masses again, for the floor of keep_masses or (RISEN) a higher one
+  template <bool RISEN>
   __device__ __forceinline__ void masses(int c, const float (&y)[4], int i0, u64 floor, u64 (&m)[4]) const {
     if constexpr (KEEP == LOGITS_AND_MASSES) {
       const ulonglong2 a = mbuf[2 * (c * ST + tid)], b = mbuf[2 * (c * ST + tid) + 1];
       m[0] = a.x; m[1] = a.y; m[2] = b.x; m[3] = b.y;
+      if constexpr (RISEN) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (sample_entry(y[j], i0 + j) < floor) m[j] = 0;
+        for (int j = 0; j < 4; ++j) m[j] = sample_entry(y[j], i0 + j) < floor ? 0 : m[j];
+      }
     } else {
       compute(y, i0, floor, m);
     }
@@ -205,100 +223,92 @@ struct Row {
 
 template <int ST>
 struct Shared {
-  u64 hist[2 * ST];   // counts or masses per bin
-  u64 cand[CAND];     // entries of the border's bin
+  u64 hist[3][2 * ST];   // counts per bin, masses per bin, masses per segment of the row
+  u64 cand[CAND];        // entries of the border's bin
   u64 cmass[CAND];
-  u64 red[16], red2[16];
-  u64 before;
-  int bin, count;
+  u64 red[4][16];        // (one for each use: no barrier in front of the next)
+  u64 before[3], last[2];
+  int bin[3], count[2];
 };
+
+// sums over the waves below (off) and over all (all) from each wave's own, `to` in its lane 63; one barrier
+template <int ST>
+__device__ __forceinline__ void block_sums(u64* red, u64 to, int tid, u64& off, u64& all) {
+  constexpr int NW = ST / 64;
+  const int lane = tid & 63, wave = tid >> 6;
+  if (lane == 63) red[wave] = to;
+  __syncthreads();
+  u64 s = lane < NW ? red[lane] : 0;
+  s += lane_move<ROW_SHR + 1, 0xF>(s);
+  s += lane_move<ROW_SHR + 2, 0xF>(s);
+  if (NW > 4) s += lane_move<ROW_SHR + 4, 0xF>(s);
+  all = __shfl(s, NW - 1, 64);
+  off = __shfl(s, wave > 0 ? wave - 1 : 0, 64);
+  if (wave == 0) off = 0;
+}
 
 // The bin (0 = the first of the order) that the border falls in: the last non-empty one with less than the border before it,
 // where `base` is what lies before bin 0.  The border is `target` entries, or the mass `lim` (frac > 0: frac x the bins' whole).
-// -> sh.bin, sh.before (base included); returns lim
+// -> sh.bin[W], sh.before[W] (base included); returns lim
 template <int ST, bool MASS>
 __device__ __forceinline__ double find_bin(Shared<ST>& sh, u64 base, u64 target, double lim, double frac, int tid) {
-  const int lane = tid & 63, wave = tid >> 6;
-  const u64 a = sh.hist[2 * tid], b = sh.hist[2 * tid + 1];
+  constexpr int W = MASS ? 1 : 0;
+  const u64 a = sh.hist[W][2 * tid], b = sh.hist[W][2 * tid + 1];
   const u64 to = wave_scan(a + b);
-  if (lane == 63) sh.red[wave] = to;
-  if (tid == 0) { sh.bin = 0; sh.before = base; }
-  __syncthreads();
-  u64 off = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < ST / 64; ++w) {
-    const u64 s = sh.red[w];
-    off += w < wave ? s : 0;
-    all += s;
-  }
+  u64 off, all;
+  block_sums<ST>(sh.red[W], to, tid, off, all);
   if (MASS && frac > 0.) lim = frac * (double)all;
   auto below = [&](u64 s) -> bool { return MASS ? (double)(base + s) < lim : base + s < target; };
   // sums before the bins rise: a kept bin is the last one if the sum behind it is not below the border, or is the whole
   const u64 s2 = off + to, s1 = s2 - b, s0 = s1 - a;
-  if (b > 0 && below(s1) && (!below(s2) || s2 == all)) { sh.bin = 2 * tid + 1; sh.before = base + s1; }
-  else if (a > 0 && below(s0) && (!below(s1) || s1 == all)) { sh.bin = 2 * tid; sh.before = base + s0; }
+  if (b > 0 && below(s1) && (!below(s2) || s2 == all)) { sh.bin[W] = 2 * tid + 1; sh.before[W] = base + s1; }
+  else if (a > 0 && below(s0) && (!below(s1) || s1 == all)) { sh.bin[W] = 2 * tid; sh.before[W] = base + s0; }
   __syncthreads();
   return lim;
 }
 
-// The last kept entry when entries >= floor take part with weight 1 (count: the first `target` stay) or their mass (those
-// with less than frac x the whole before them stay).
+// The last kept entry when all entries take part with weight 1 (count: the first `target` stay), or the ones >= floor with their
+// mass (those with less than frac x the whole before them stay).  sh.hist[W], sh.count[W] and sh.last[W] come cleared.
 template <typename T, int ST, int KEEP, bool MASS>
 __device__ __forceinline__ u64 last_kept(Shared<ST>& sh, Row<T, ST, KEEP>& row, u64 floor, float bin_scale, u64 target, double frac) {
-  constexpr int BINS = 2 * ST, LOG_BINS = ST == 1024 ? 11 : 9;
+  constexpr int BINS = 2 * ST, LOG_BINS = ST == 512 ? 10 : 9, W = MASS ? 1 : 0;
+  static_assert(BINS == 1 << LOG_BINS, "bins");
   const int tid = row.tid;
-  auto bin_of = [&](float x) -> int {
-    const float y = (row.rs.xmax - x) * bin_scale;        // falls as x rises, rounding included
-    return y < (float)(BINS - 1) ? (int)y : BINS - 1;      // (-inf, NaN: last)
-  };
-  auto each = [&](auto f) {       // f(entry, weight, bin) for the entries that take part
+  auto each = [&](auto f) {       // f(x, index, weight, bin) for the entries that take part
     row.template each_chunk<false>([&](int c, float (&y)[4], int i0) {
-      u64 m[4];
-      if constexpr (MASS) {
-        row.masses(c, y, i0, floor, m);
-      } else {
+      u64 m[4] = {1, 1, 1, 1};
+      if constexpr (MASS) row.template masses<false>(c, y, i0, floor, m);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = i0 + j < row.V && sample_entry(y[j], i0 + j) >= floor ? 1ull : 0ull;
+      for (int j = 0; j < 4; ++j) {
+        const float z = (row.rs.xmax - y[j]) * bin_scale;             // falls as x rises, rounding included
+        const int b = z < (float)(BINS - 1) ? (int)z : BINS - 1;       // (-inf, NaN: last)
+        if (MASS ? m[j] > 0 : i0 + j < row.V) f(y[j], i0 + j, m[j], b);
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (m[j]) f(sample_entry(y[j], i0 + j), m[j], bin_of(y[j]));
     });
   };
-  __syncthreads();
-  sh.hist[2 * tid] = 0;
-  sh.hist[2 * tid + 1] = 0;
-  if (tid == 0) sh.count = 0;
-  __syncthreads();
-  each([&](u64, u64 m, int b) { atomicAdd(&sh.hist[b], m); });
+  each([&](float, int, u64 m, int b) { atomicAdd(&sh.hist[W][b], m); });
   __syncthreads();
   const double lim = find_bin<ST, MASS>(sh, 0, target, 0., frac, tid);
-  const int bin = sh.bin;
-  const u64 before = sh.before;
-  each([&](u64 c, u64 m, int b) {
+  const int bin = sh.bin[W];
+  const u64 before = sh.before[W];
+  each([&](float x, int i, u64 m, int b) {
     if (b == bin) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < CAND) { sh.cand[at] = c; sh.cmass[at] = m; }
+      const int at = atomicAdd(&sh.count[W], 1);
+      if (at < CAND) { sh.cand[at] = sample_entry(x, i); sh.cmass[at] = m; }
     }
   });
   __syncthreads();
-  const int n = sh.count;
+  const int n = sh.count[W];
   if (n <= CAND) {
     // rank every candidate against the others; the last kept one is the smallest entry with less than the border before it
-    u64 kept = 0;                 // (complemented: the maximum is wanted)
-    for (int a = tid; a < n; a += ST) {
-      const u64 c = sh.cand[a];
+    if (tid < n) {
+      const u64 c = sh.cand[tid];
       u64 s = before;
       for (int o = 0; o < n; ++o) s += sh.cand[o] > c ? sh.cmass[o] : 0;
-      if (MASS ? (double)s < lim : s < target) kept = max_u64(kept, ~c);
+      if (MASS ? (double)s < lim : s < target) atomicMin(&sh.last[W], c);
     }
-    kept = wave_max(kept);
-    if ((tid & 63) == 63) sh.red2[tid >> 6] = kept;
     __syncthreads();
-    kept = 0;
-#pragma unroll
-    for (int w = 0; w < ST / 64; ++w) kept = max_u64(kept, sh.red2[w]);
-    return ~kept;
+    return sh.last[W];
   }
   // many equal logits: radix descent over the entries of the bin
   u64 prefix = 0, sum = before;
@@ -306,18 +316,20 @@ __device__ __forceinline__ u64 last_kept(Shared<ST>& sh, Row<T, ST, KEEP>& row, 
   for (int hi = 32 + IDX_BITS; hi > 0;) {
     const int bits = hi > LOG_BINS ? LOG_BINS : hi, lo = hi - bits;
     __syncthreads();
-    sh.hist[2 * tid] = 0;
-    sh.hist[2 * tid + 1] = 0;
+    sh.hist[W][2 * tid] = 0;
+    sh.hist[W][2 * tid + 1] = 0;
     __syncthreads();
-    each([&](u64 c, u64 m, int b) {
-      if (b == bin && (c >> hi) == prefix) atomicAdd(&sh.hist[(1 << bits) - 1 - (int)((c >> lo) & ((1u << bits) - 1u))], m);
+    each([&](float x, int i, u64 m, int b) {
+      const u64 c = sample_entry(x, i);
+      if (b == bin && (c >> hi) == prefix) atomicAdd(&sh.hist[W][(1 << bits) - 1 - (int)((c >> lo) & ((1u << bits) - 1u))], m);
     });
     __syncthreads();
     find_bin<ST, MASS>(sh, sum, target, lim, 0., tid);
-    prefix = (prefix << bits) | (u64)((1 << bits) - 1 - sh.bin);
-    sum = sh.before;
+    prefix = (prefix << bits) | (u64)((1 << bits) - 1 - sh.bin[W]);
+    sum = sh.before[W];
     hi = lo;
   }
+  __syncthreads();
   return prefix;
 }
 
@@ -340,9 +352,17 @@ __global__ __launch_bounds__(ST) void sample_rows_kernel(const SampleArgs a) {
   int k = a.k ? a.k[b] : a.k_all;
   if (k <= 0 || k > a.V) k = a.V;
 
+  // while the row is on its way
+#pragma unroll
+  for (int w = 0; w < 3; ++w) sh.hist[w][2 * tid] = sh.hist[w][2 * tid + 1] = 0;
+  if (tid < 2) {
+    sh.count[tid] = 0;
+    sh.last[tid] = ~0ull;
+  }
+
   // the row; the first entry of the order, and the smallest finite logit (as the largest complemented key)
   u64 top = 0, low = 0;
-#pragma unroll 2
+#pragma unroll 4
   for (int c = 0; c < row.chunks; ++c) {
     const int i0 = c * (4 * ST) + 4 * tid;
     if (i0 >= a.V) break;
@@ -359,13 +379,13 @@ __global__ __launch_bounds__(ST) void sample_rows_kernel(const SampleArgs a) {
   }
   top = wave_max(top);
   low = wave_max(low);
-  if (lane == 63) { sh.red[wave] = top; sh.red2[wave] = low; }
+  if (lane == 63) { sh.red[2][wave] = top; sh.red[3][wave] = low; }
   __syncthreads();
   top = low = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
-    top = max_u64(top, sh.red[w]);
-    low = max_u64(low, sh.red2[w]);
+    top = max_u64(top, sh.red[2][w]);
+    low = max_u64(low, sh.red[3][w]);
   }
   const int first = (1 << IDX_BITS) - 1 - (int)(top & ((1u << IDX_BITS) - 1u));
   const unsigned tk = (unsigned)(top >> IDX_BITS), lk = ~(unsigned)low;
@@ -385,47 +405,37 @@ __global__ __launch_bounds__(ST) void sample_rows_kernel(const SampleArgs a) {
   row.keep_masses(floor);
   if (tp < 1.f) floor = last_kept<T, ST, KEEP, true>(sh, row, floor, bin_scale, 0, (double)tp);
 
-  // kept mass by index: per chunk and wave (256 consecutive indices), in sh.hist
-  const double minm = (double)mp * (double)(1ull << FRAC);
+  // kept mass by index: per chunk and wave (256 consecutive indices), in sh.hist[2]; min_p as a mass (NaN: all but the first out)
+  const double least = ceil((double)mp * (double)(1ull << FRAC));
+  const u64 min_mass = least <= 0. ? 0ull : least < 9e15 ? (u64)least : ~0ull;
   auto kept_masses = [&](int c, float (&y)[4], int i0, u64 (&m)[4]) {
     m[0] = m[1] = m[2] = m[3] = 0;
     if (i0 >= a.V) return;
-    row.masses(c, y, i0, floor, m);
+    row.template masses<true>(c, y, i0, floor, m);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (!((double)m[j] >= minm) && i0 + j != first) m[j] = 0;
+    for (int j = 0; j < 4; ++j) m[j] = m[j] >= min_mass || i0 + j == first ? m[j] : 0;
   };
-  __syncthreads();
-  sh.hist[2 * tid] = 0;
-  sh.hist[2 * tid + 1] = 0;
-  __syncthreads();
   row.template each_chunk<true>([&](int c, float (&y)[4], int i0) {
     u64 m[4];
     kept_masses(c, y, i0, m);
     const u64 s = wave_scan(m[0] + m[1] + m[2] + m[3]);
-    if (lane == 63) sh.hist[c * NW + wave] = s;
+    if (lane == 63) sh.hist[2][c * NW + wave] = s;
   });
   __syncthreads();
   // the segment of the token: the first whose end exceeds u x the whole (u >= 1, NaN: the last with any mass)
-  const u64 ha = sh.hist[2 * tid], hb = sh.hist[2 * tid + 1];
+  const u64 ha = sh.hist[2][2 * tid], hb = sh.hist[2][2 * tid + 1];
   const u64 to = wave_scan(ha + hb);
-  if (lane == 63) sh.red[wave] = to;
-  __syncthreads();
-  u64 off = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    off += w < wave ? sh.red[w] : 0;
-    all += sh.red[w];
-  }
+  u64 off, all;
+  block_sums<ST>(sh.red[2], to, tid, off, all);
   const double want = (double)u * (double)all;
   auto inside = [&](u64 from, u64 m) -> bool {
     return m > 0 && (!((double)from > want) || from == 0) && ((double)(from + m) > want || from + m == all);
   };
   const u64 end = off + to;
-  if (inside(end - hb - ha, ha)) { sh.bin = 2 * tid; sh.before = end - hb - ha; }
-  if (inside(end - hb, hb)) { sh.bin = 2 * tid + 1; sh.before = end - hb; }
+  if (inside(end - hb - ha, ha)) { sh.bin[2] = 2 * tid; sh.before[2] = end - hb - ha; }
+  if (inside(end - hb, hb)) { sh.bin[2] = 2 * tid + 1; sh.before[2] = end - hb; }
   __syncthreads();
-  const int seg = sh.bin;
+  const int seg = sh.bin[2];
   if (wave != seg % NW) return;
   const int c = seg / NW, i0 = c * (4 * ST) + 4 * tid;
   float y[4] = {0.f, 0.f, 0.f, 0.f};
@@ -433,7 +443,7 @@ __global__ __launch_bounds__(ST) void sample_rows_kernel(const SampleArgs a) {
   if (i0 < a.V) row.get(c, y);
   kept_masses(c, y, i0, m);
   const u64 s = m[0] + m[1] + m[2] + m[3];
-  u64 at = sh.before + wave_scan(s) - s;
+  u64 at = sh.before[2] + wave_scan(s) - s;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (inside(at, m[j])) a.out[b] = i0 + j;
@@ -446,7 +456,7 @@ int launch_sample(const SampleArgs& a, long long rows, hipStream_t st) {
   const size_t v4 = ((size_t)a.V + 3) / 4 * 4, bytes = KEEP == NOTHING ? 0 : KEEP == LOGITS ? v4 * 4 : v4 * 12;
   if (bytes + sizeof(Shared<ST>) > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)sample_rows_kernel<T, ST, KEEP>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, 132000);
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, 130000);
     if (e != hipSuccess) return (int)e;
   }
   hipLaunchKernelGGL((sample_rows_kernel<T, ST, KEEP>), dim3((unsigned)rows), dim3(ST), bytes, st, a);
@@ -456,9 +466,9 @@ int launch_sample(const SampleArgs& a, long long rows, hipStream_t st) {
 template <typename T>
 int launch_sample_v(const SampleArgs& a, long long rows, hipStream_t st) {
   if (a.V <= 1024) return launch_sample<T, 256, LOGITS_AND_MASSES>(a, rows, st);
-  if (a.V <= 11000) return launch_sample<T, 1024, LOGITS_AND_MASSES>(a, rows, st);   // 132 KB beside the 25 KB of Shared
-  if (a.V <= 32768) return launch_sample<T, 1024, LOGITS>(a, rows, st);
-  return launch_sample<T, 1024, NOTHING>(a, rows, st);
+  if (a.V <= 10800) return launch_sample<T, 512, LOGITS_AND_MASSES>(a, rows, st);   // 127 KB beside the 29 KB of Shared
+  if (a.V <= 30000) return launch_sample<T, 512, LOGITS>(a, rows, st);
+  return launch_sample<T, 512, NOTHING>(a, rows, st);
 }
 
 }  // namespace
