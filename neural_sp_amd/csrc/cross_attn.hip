@@ -231,15 +231,16 @@ __device__ __forceinline__ void x_load_rows(typename AttnElem<T>::chunk (&f)[N][
   }
 }
 
-// score tile: s[f][kf] rows = streamed rows 16 kf + 4 g + e, column = owned row
-template <typename T, int DP, int N, int KF, int NS>
+// score tile: s[f][kf] rows = streamed rows 16 kf + 4 g + e, column = owned row; init(f, kf) is added (the matrix instruction's
+// accumulator starts with it)
+template <typename T, int DP, int N, int KF, int NS, class I>
 __device__ __forceinline__ void x_product(f32x4 (&s)[N][KF], const unsigned char* tile,
-                                          const typename AttnElem<T>::chunk (&own)[N][NS], int r, int g) {
+                                          const typename AttnElem<T>::chunk (&own)[N][NS], int r, int g, I init) {
   typedef XTile<T, DP> X;
 #pragma unroll
   for (int kf = 0; kf < KF; ++kf) {
 #pragma unroll
-    for (int f = 0; f < N; ++f) s[f][kf] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int f = 0; f < N; ++f) s[f][kf] = init(f, kf);
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const auto a = X::rows(tile, 16 * kf, i, r, g);
@@ -248,9 +249,12 @@ __device__ __forceinline__ void x_product(f32x4 (&s)[N][KF], const unsigned char
     }
   }
 }
+struct XZero {
+  __device__ __forceinline__ f32x4 operator()(int, int) const { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+};
 
 template <typename T, int DP, int NQ, bool DROP>
-__global__ __launch_bounds__(256) void cross_fwd_kernel(const XArgs p) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
   constexpr int KF = X::KT / 16;
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES];
@@ -292,26 +296,44 @@ __global__ __launch_bounds__(256) void cross_fwd_kernel(const XArgs p) {
       X::dma(Kn + X::BYTES, vb, p.v_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
     }
     f32x4 s[NQ][KF];
-    x_product<T, DP, NQ>(s, Kc, Q, r, g);
-    const bool whole = (kt + 1) * X::KT <= klen;
+    x_product<T, DP, NQ>(s, Kc, Q, r, g, XZero());
+    if (uniform || (kt + 1) * X::KT > klen) {
+#pragma unroll
+      for (int f = 0; f < NQ; ++f)
+#pragma unroll
+        for (int kf = 0; kf < KF; ++kf)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (uniform) s[f][kf][e] = 0.f;
+            if (kt * X::KT + 16 * kf + 4 * g + e >= klen) s[f][kf][e] = -INFINITY;
+          }
+    }
+    // The reference maximum moves only when a score exceeds it by 2^8: exponentials then stay below 2^8 (exact in range for both
+    // types, and bf16 keeps its relative precision), and after the first tiles nothing is rescaled any more.
+    float mx[NQ];
+    bool move = false;
 #pragma unroll
     for (int f = 0; f < NQ; ++f) {
-      float mx = -INFINITY;
+      mx[f] = s[f][0][0];
 #pragma unroll
       for (int kf = 0; kf < KF; ++kf)
+        mx[f] = fmaxf(fmaxf(fmaxf(mx[f], s[f][kf][0]), fmaxf(s[f][kf][1], s[f][kf][2])), s[f][kf][3]);
+      mx[f] = attn_max4(mx[f]) * p.sl2;    // (scale > 0: the maximum commutes with it; a tile has a visible key: finite)
+      move = move || !(mx[f] <= m[f] + 8.f);
+    }
+    if (__any(move)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (uniform) s[f][kf][e] = 0.f;
-          if (!whole && kt * X::KT + 16 * kf + 4 * g + e >= klen) s[f][kf][e] = -INFINITY;
-          mx = fmaxf(mx, s[f][kf][e]);
-        }
-      // (scale > 0: the maximum commutes with it; a tile always has a visible key, so it is finite)
-      const float mn = fmaxf(m[f], attn_max4(mx) * p.sl2);
-      const float alpha = __builtin_amdgcn_exp2f(m[f] - mn);
-      m[f] = mn;
-      l[f] *= alpha;
+      for (int f = 0; f < NQ; ++f) {
+        const float mn = fmaxf(m[f], mx[f]);
+        const float alpha = __builtin_amdgcn_exp2f(m[f] - mn);
+        m[f] = mn;
+        l[f] *= alpha;
 #pragma unroll
-      for (int i = 0; i < X::NB; ++i) o[f][i] *= alpha;
+        for (int i = 0; i < X::NB; ++i) o[f][i] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < NQ; ++f) {
       const int qi = min(q0 + 16 * f + r, p.Tq - 1);
       const unsigned long long row =
           DROP ? p.offset + (unsigned long long)((((long long)b * p.H + h) * p.Tq + qi) * p.Tk) : 0ull;
@@ -321,7 +343,7 @@ __global__ __launch_bounds__(256) void cross_fwd_kernel(const XArgs p) {
         if constexpr (DROP) nsp_keep_scale4(p.seed, row + (unsigned long long)(kt * X::KT + 16 * kf + 4 * g), p.drop, keep);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -mn));
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -m[f]));
           l[f] += x;
           s[f][kf][e] = DROP ? x * keep[e] : x;
         }
@@ -348,7 +370,7 @@ __global__ __launch_bounds__(256) void cross_fwd_kernel(const XArgs p) {
 }
 
 template <typename T, int DP, int NQ, bool DROP>
-__global__ __launch_bounds__(256) void cross_dq_kernel(const XArgs p) {
+__global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
   constexpr int KF = X::KT / 16;
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES];
@@ -393,6 +415,7 @@ __global__ __launch_bounds__(256) void cross_dq_kernel(const XArgs p) {
       const int qi = min(q0 + 16 * f + r, p.Tq - 1);
       m[f] = p.stats[srow + qi];
       inv[f] = p.stats[(long long)p.B * p.H * p.Tq + srow + qi];
+      if constexpr (sizeof(T) == 2) m[f] -= __log2f(inv[f]);      // (one rounding of the exponent more, far below bf16's)
       if (g == 0 && q0 + 16 * f + r < p.Tq) p.dsum[srow + qi] = ds[f];
 #pragma unroll
       for (int i = 0; i < X::NB; ++i) acc[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -413,9 +436,10 @@ __global__ __launch_bounds__(256) void cross_dq_kernel(const XArgs p) {
       X::dma(Kn + X::BYTES, vb, p.v_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
     }
     f32x4 s[NQ][KF], dp[NQ][KF];
-    x_product<T, DP, NQ>(s, Kc, Q, r, g);
-    x_product<T, DP, NQ>(dp, Kc + X::BYTES, dO, r, g);
-    const bool whole = (kt + 1) * X::KT <= klen;
+    x_product<T, DP, NQ>(s, Kc, Q, r, g, XZero());
+    // dP - D in one go (with dropout D comes after the mask)
+    x_product<T, DP, NQ>(dp, Kc + X::BYTES, dO, r, g,
+                         [&](int f, int) -> f32x4 { return DROP ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{-ds[f], -ds[f], -ds[f], -ds[f]}; });
 #pragma unroll
     for (int f = 0; f < NQ; ++f) {
       const int qi = min(q0 + 16 * f + r, p.Tq - 1);
@@ -426,13 +450,20 @@ __global__ __launch_bounds__(256) void cross_dq_kernel(const XArgs p) {
         if constexpr (DROP) nsp_keep_scale4(p.seed, row + (unsigned long long)(kt * X::KT + 16 * kf + 4 * g), p.drop, keep);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -m[f])) * inv[f];
-          const float dpe = DROP ? dp[f][kf][e] * keep[e] : dp[f][kf][e];
-          x *= dpe - ds[f];
-          if (!whole && kt * X::KT + 16 * kf + 4 * g + e >= klen) x = 0.f;
-          s[f][kf][e] = x;
+          float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -m[f]));
+          if constexpr (sizeof(T) == 4) x *= inv[f];
+          s[f][kf][e] = x * (DROP ? fmaf(dp[f][kf][e], keep[e], -ds[f]) : dp[f][kf][e]);
         }
       }
+    }
+    if ((kt + 1) * X::KT > klen) {
+#pragma unroll
+      for (int f = 0; f < NQ; ++f)
+#pragma unroll
+        for (int kf = 0; kf < KF; ++kf)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (kt * X::KT + 16 * kf + 4 * g + e >= klen) s[f][kf][e] = 0.f;
     }
     x_accumulate<DP, NQ>(acc, Kc, s, T(0), r, g);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -446,33 +477,33 @@ __global__ __launch_bounds__(256) void cross_dq_kernel(const XArgs p) {
   }
 }
 
-template <typename T, int DP, bool DROP>
-__global__ __launch_bounds__(256) void cross_dkv_kernel(const XArgs p) {
+template <typename T, int DP, int NK, bool DROP>
+__global__ __launch_bounds__(256, DP == 128 && NK == 2 ? 1 : 2) void cross_dkv_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
   constexpr int QF = X::KT / 16;
   // tiles, then per buffer KT maxima, KT reciprocal sums, KT values of D
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES + 2 * 3 * X::KT * 4];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int G = p.H / p.Hkv, nkt = (p.Tk + 63) / 64;
+  const int G = p.H / p.Hkv, nkt = (p.Tk + 64 * NK - 1) / (64 * NK);
   int grp, item;
   if (!x_place(p.B * p.Hkv, nkt, grp, item)) return;
   const int b = grp / p.Hkv, hkv = grp % p.Hkv;
   int klen = p.klens ? min(p.klens[b], p.Tk) : p.Tk;
   const bool uniform = klen <= 0;
   if (uniform) klen = p.Tk;
-  const int k0 = item * 64 + wave * 16, key = k0 + r;
-  T* dkr = reinterpret_cast<T*>(p.dk) + (((long long)b * p.Tk + key) * p.Hkv + hkv) * p.D;
-  T* dvr = reinterpret_cast<T*>(p.dv) + (((long long)b * p.Tk + key) * p.Hkv + hkv) * p.D;
-  f32x4 dk[1][X::NB], dv[1][X::NB];
+  const int k0 = (item * 4 + wave) * (16 * NK);
+  f32x4 dk[NK][X::NB], dv[NK][X::NB];
 #pragma unroll
-  for (int i = 0; i < X::NB; ++i) dk[0][i] = dv[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (item * 64 < klen && p.Tq > 0) {      // (uniform over the workgroup; keys behind klen get zeros)
+  for (int f = 0; f < NK; ++f)
+#pragma unroll
+    for (int i = 0; i < X::NB; ++i) dk[f][i] = dv[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (item * (64 * NK) < klen && p.Tq > 0) {      // (uniform over the workgroup; keys behind klen get zeros)
     const int chunks = p.D / X::E::CE, nqt = (p.Tq + X::KT - 1) / X::KT, n = G * nqt;
-    typename X::E::chunk K[1][X::NS], V[1][X::NS];
-    x_load_rows<T, 1>(K, reinterpret_cast<const T*>(p.k) + (long long)b * p.k_sb + (long long)hkv * p.k_sh, p.k_st, k0, klen,
+    typename X::E::chunk K[NK][X::NS], V[NK][X::NS];
+    x_load_rows<T, NK>(K, reinterpret_cast<const T*>(p.k) + (long long)b * p.k_sb + (long long)hkv * p.k_sh, p.k_st, k0, klen,
                           p.D, r, g);
-    x_load_rows<T, 1>(V, reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh, p.v_st, k0, klen,
+    x_load_rows<T, NK>(V, reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh, p.v_st, k0, klen,
                           p.D, r, g);
     const T* qb = reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)hkv * G * p.q_sh;
     const T* gb = reinterpret_cast<const T*>(p.dout) + (long long)b * p.g_sb + (long long)hkv * G * p.g_sh;
@@ -481,9 +512,11 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const XArgs p) {
     auto stat = [&](int it) -> float {     // this thread's statistic of tile it
       const int which = (int)threadIdx.x / X::KT, q = (it % nqt) * X::KT + (int)threadIdx.x % X::KT;
       if (which >= 3) return 0.f;
-      if (which == 1 && q >= p.Tq) return 0.f;      // rows behind the last query: probability 0
       const long long at = srow + (long long)(it / nqt) * p.Tq + min(q, p.Tq - 1);
-      return which == 0 ? p.stats[at] : which == 1 ? p.stats[nst + at] : p.dsum[at];
+      if (which == 2) return p.dsum[at];
+      if (q >= p.Tq) return which == 0 ? INFINITY : 0.f;      // rows behind the last query: probability 0
+      if constexpr (sizeof(T) == 2) return which == 0 ? p.stats[at] - __log2f(p.stats[nst + at]) : 0.f;
+      return p.stats[(which == 0 ? 0 : nst) + at];
     };
     auto fetch = [&](unsigned char* to, int it) {
       const int hq = it / nqt, row0 = (it % nqt) * X::KT;
@@ -503,42 +536,62 @@ __global__ __launch_bounds__(256) void cross_dkv_kernel(const XArgs p) {
         next = stat(it + 1);
         fetch(lds + ((it + 1) & 1) * (2 * X::BYTES), it + 1);
       }
-      f32x4 s[1][QF], dp[1][QF];
-      x_product<T, DP, 1>(s, Qc, K, r, g);
-      x_product<T, DP, 1>(dp, Qc + X::BYTES, V, r, g);
+      f32x4 s[NK][QF], dp[NK][QF];
+      x_product<T, DP, NK>(s, Qc, K, r, g, XZero());
+      x_product<T, DP, NK>(dp, Qc + X::BYTES, V, r, g, [&](int, int qf) -> f32x4 {
+        return DROP ? f32x4{0.f, 0.f, 0.f, 0.f} : -*reinterpret_cast<const f32x4*>(sc + 2 * X::KT + 16 * qf + 4 * g);
+      });
+      if (uniform) {
+#pragma unroll
+        for (int f = 0; f < NK; ++f)
+#pragma unroll
+          for (int qf = 0; qf < QF; ++qf) s[f][qf] = f32x4{0.f, 0.f, 0.f, 0.f};      // (exponent 0 - 0, see the forward kernel)
+      }
 #pragma unroll
       for (int qf = 0; qf < QF; ++qf) {
         const f32x4 m4 = *reinterpret_cast<const f32x4*>(sc + 16 * qf + 4 * g);
         const f32x4 i4 = *reinterpret_cast<const f32x4*>(sc + X::KT + 16 * qf + 4 * g);
         const f32x4 d4 = *reinterpret_cast<const f32x4*>(sc + 2 * X::KT + 16 * qf + 4 * g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(uniform ? 0.f : fmaf(s[0][qf][e], p.sl2, -m4[e])) * i4[e];
-          float keep = 1.f;
-          if constexpr (DROP) {
-            const int qi = min((it % nqt) * X::KT + 16 * qf + 4 * g + e, p.Tq - 1);
-            keep = nsp_keep_scale(p.seed, p.offset + (unsigned long long)((srow + (long long)(it / nqt) * p.Tq + qi) * p.Tk + key), p.drop);
+        for (int f = 0; f < NK; ++f)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = __builtin_amdgcn_exp2f(fmaf(s[f][qf][e], p.sl2, -m4[e]));
+            if constexpr (sizeof(T) == 4) x *= i4[e];
+            if constexpr (DROP) {
+              const int qi = min((it % nqt) * X::KT + 16 * qf + 4 * g + e, p.Tq - 1);
+              const float keep = nsp_keep_scale(
+                  p.seed, p.offset + (unsigned long long)((srow + (long long)(it / nqt) * p.Tq + qi) * p.Tk + k0 + 16 * f + r), p.drop);
+              dp[f][qf][e] = x * fmaf(dp[f][qf][e], keep, -d4[e]);
+              s[f][qf][e] = x * keep;
+            } else {
+              dp[f][qf][e] *= x;
+              s[f][qf][e] = x;
+            }
           }
-          const float dpe = DROP ? dp[0][qf][e] * keep : dp[0][qf][e];
-          dp[0][qf][e] = uniform ? 0.f : x * (dpe - d4[e]);
-          s[0][qf][e] = DROP ? x * keep : x;
-        }
       }
-      x_accumulate<DP, 1>(dv, Qc + X::BYTES, s, T(0), r, g);
-      x_accumulate<DP, 1>(dk, Qc, dp, T(0), r, g);
+      x_accumulate<DP, NK>(dv, Qc + X::BYTES, s, T(0), r, g);
+      x_accumulate<DP, NK>(dk, Qc, dp, T(0), r, g);
       if (it + 1 < n && (int)threadIdx.x < 3 * X::KT) st[((it + 1) & 1) * (3 * X::KT) + threadIdx.x] = next;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
     }
   }
-  if (key < p.Tk) {
-    const bool in = key < klen;
-    if (!in) {
 #pragma unroll
-      for (int i = 0; i < X::NB; ++i) dk[0][i] = dv[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int f = 0; f < NK; ++f) {
+    const int key = k0 + 16 * f + r;
+    if (key >= p.Tk) continue;
+    const long long at = (((long long)b * p.Tk + key) * p.Hkv + hkv) * p.D;
+    if (key >= klen) {
+#pragma unroll
+      for (int i = 0; i < X::NB; ++i) dk[f][i] = dv[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    x_store<DP, false>(dkr, dk[0], p.scale, p.D, g);
-    x_store<DP, false>(dvr, dv[0], 1.f, p.D, g);
+    if (uniform) {      // the scores of such a row are constants
+#pragma unroll
+      for (int i = 0; i < X::NB; ++i) dk[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    x_store<DP, false>(reinterpret_cast<T*>(p.dk) + at, dk[f], p.scale, p.D, g);
+    x_store<DP, false>(reinterpret_cast<T*>(p.dv) + at, dv[f], 1.f, p.D, g);
   }
 }
 
@@ -552,20 +605,39 @@ int launch_fwd(const XArgs& p, hipStream_t st) {
   return NSP_OK;
 }
 template <typename T, int DP, int NQ, bool DROP>
-int launch_bwd(const XArgs& p, hipStream_t st) {
-  const long long groups = ((long long)p.B * p.Hkv + 7) / 8 * 8;
-  const long long wq = groups * (p.H / p.Hkv) * ((p.Tq + 64 * NQ - 1) / (64 * NQ)), wk = groups * ((p.Tk + 63) / 64);
-  if (wq > 0x7fffffffLL || wk > 0x7fffffffLL) return NSP_EUNSUPPORTED;
-  hipLaunchKernelGGL((cross_dq_kernel<T, DP, NQ, DROP>), dim3((unsigned)wq), dim3(256), 0, st, p);
+int launch_dq(const XArgs& p, hipStream_t st) {
+  const long long wgs = ((long long)p.B * p.Hkv + 7) / 8 * 8 * (p.H / p.Hkv) * ((p.Tq + 64 * NQ - 1) / (64 * NQ));
+  if (wgs > 0x7fffffffLL) return NSP_EUNSUPPORTED;
+  hipLaunchKernelGGL((cross_dq_kernel<T, DP, NQ, DROP>), dim3((unsigned)wgs), dim3(256), 0, st, p);
   NSP_LAUNCH_CHECK();
-  hipLaunchKernelGGL((cross_dkv_kernel<T, DP, DROP>), dim3((unsigned)wk), dim3(256), 0, st, p);
+  return NSP_OK;
+}
+template <typename T, int DP, int NK, bool DROP>
+int launch_dkv(const XArgs& p, hipStream_t st) {
+  const long long wgs = ((long long)p.B * p.Hkv + 7) / 8 * 8 * ((p.Tk + 64 * NK - 1) / (64 * NK));
+  if (wgs > 0x7fffffffLL) return NSP_EUNSUPPORTED;
+  hipLaunchKernelGGL((cross_dkv_kernel<T, DP, NK, DROP>), dim3((unsigned)wgs), dim3(256), 0, st, p);
   NSP_LAUNCH_CHECK();
   return NSP_OK;
 }
 
+// Two owned 16-row fragments per wave halve the LDS reads per score, which bound the bf16 kernels with one; they pay once the
+// halved number of workgroups still fills the 256 compute units.  fp32 spends eight times as long in the matrix cores and keeps
+// one.
 template <typename T, int DP, bool DROP>
 int launch(const XArgs& p, bool bwd, hipStream_t st) {
-  return bwd ? launch_bwd<T, DP, 1, DROP>(p, st) : launch_fwd<T, DP, 1, DROP>(p, st);
+  if constexpr (sizeof(T) == 2) {
+    const bool two_q = p.Tq > 64 && (long long)p.B * p.H * ((p.Tq + 127) / 128) >= 512;
+    const bool two_k = p.Tk > 64 && (long long)p.B * p.Hkv * ((p.Tk + 127) / 128) >= 512;
+    if (!bwd) return two_q ? launch_fwd<T, DP, 2, DROP>(p, st) : launch_fwd<T, DP, 1, DROP>(p, st);
+    const int rc = two_q ? launch_dq<T, DP, 2, DROP>(p, st) : launch_dq<T, DP, 1, DROP>(p, st);
+    if (rc != NSP_OK) return rc;
+    return two_k ? launch_dkv<T, DP, 2, DROP>(p, st) : launch_dkv<T, DP, 1, DROP>(p, st);
+  } else {
+    if (!bwd) return launch_fwd<T, DP, 1, DROP>(p, st);
+    const int rc = launch_dq<T, DP, 1, DROP>(p, st);
+    return rc != NSP_OK ? rc : launch_dkv<T, DP, 1, DROP>(p, st);
+  }
 }
 template <typename T, bool DROP>
 int launch_d(const XArgs& p, bool bwd, hipStream_t st) {

@@ -217,6 +217,17 @@ template <class T> static inline T __shfl_xor(T v, int m, int = 64) { return hip
 template <class T> static inline T __shfl_down(T v, int d, int = 64) { return hipemu_shfl(v, hipemu_src_down, d); }
 template <class T> static inline T __shfl_up(T v, int d, int = 64) { return hipemu_shfl(v, hipemu_src_up, d); }
 template <class T> static inline T __shfl(T v, int i, int = 64) { return hipemu_shfl(v, hipemu_src_idx, i); }
+// true in any live lane of the wave
+static inline int __any(int pred) {
+  hipemu::Wave& w = *hipemu::wave;
+  w.slot[hipemu::tid_flat & 63] = pred ? 1 : 0;
+  hipemu::wave_barrier();
+  int r = 0;
+  for (int i = 0; i < w.n; ++i) r |= !w.done[i] && w.slot[i] == 1;
+  hipemu::wave_barrier();
+  return r;
+}
+#define __log2f(x) log2f(x)
 // v_permlane16_swap / v_permlane32_swap (vdst, src): odd 16-lane rows (upper 32-lane half) of vdst <-> even rows (lower
 // half) of src; returns {vdst', src'}
 struct hipemu_swap_pair { unsigned v[2]; unsigned operator[](int i) const { return v[i]; } };

@@ -25,6 +25,9 @@ CROSS = [
     dict(B=2, H=16, Hkv=4, D=128, Tq=129, Tk=515, klens=[515, 100]),
     dict(B=1, H=6, Hkv=1, D=40, Tq=1, Tk=3001, klens=[3000]),
     dict(B=1, H=2, Hkv=2, D=64, Tq=700, Tk=64, klens=[64], scale=0.5),
+    dict(B=64, H=8, Hkv=8, D=64, Tq=70, Tk=131, klens=[131 - 2 * i for i in range(64)]),      # two owned fragments per wave
+    dict(B=32, H=16, Hkv=16, D=128, Tq=130, Tk=66, klens=[66 - i for i in range(32)]),
+    dict(B=520, H=2, Hkv=1, D=24, Tq=129, Tk=129, klens=[(i * 5) % 131 for i in range(520)]),
     dict(B=17, H=2, Hkv=1, D=96, Tq=16, Tk=100, klens=[100 - 5 * i for i in range(17)], layout='heads'),
 ]
 
