@@ -21,6 +21,7 @@
 // A row without a visible key is uniform over all Tk keys, as with the finite mask value of attn_softmax_fwd, and passes no
 // gradient through its scores.  Keys behind klens are never read.
 #include "attn_frag.h"
+#include <type_traits>
 
 namespace {
 
@@ -51,20 +52,6 @@ struct XTile {
   static constexpr int NB = DP / 16;                 // 16-row blocks of a transposed accumulator
   static constexpr int BYTES = KT * RB;
   __device__ static __forceinline__ int swz(int row) { return RB >= 128 ? (row & 7) : ((row >> 1) & 3); }
-  // rows row0 .. row0 + KT - 1 of src (limit > 0 rows; later ones re-read the last) into LDS
-  __device__ static __forceinline__ void dma(unsigned char* tile, const T* src, long long ld, int row0, int limit, int chunks,
-                                             int wave, int lane) {
-    constexpr int PIECES = BYTES / 1024;             // 1 KB = one instruction of a wave
-#pragma unroll
-    for (int i = 0; i < PIECES / 4; ++i) {
-      const int piece = wave * (PIECES / 4) + i;
-      const int row = piece * (64 / CPR) + lane / CPR, c = lane % CPR;
-      int sc = c ^ swz(row);
-      sc = min(sc, chunks - 1);                      // (head sizes below DP: the owned operand is zero there)
-      const T* p = src + (long long)min(row0 + row, limit - 1) * ld + sc * E::CE;
-      __builtin_amdgcn_global_load_lds((x_glb_void*)p, (x_lds_void*)(tile + piece * 1024), 16, 0, 0);
-    }
-  }
   // operand of a product over the head size: chunk 4 s + g of row rbase + r
   __device__ static __forceinline__ typename E::chunk rows(const unsigned char* tile, int rbase, int s, int r, int g) {
     const int row = rbase + r;
@@ -72,11 +59,52 @@ struct XTile {
   }
 };
 
+// where a workgroup's tiles come from: a uniform address per tile and 32-bit offsets per lane that stay (strides below 2^24
+// elements), so that the requests of a tile cost no vector arithmetic
+template <typename T, int DP>
+struct XSource {
+  typedef XTile<T, DP> X;
+  static constexpr int P = X::BYTES / 4096;          // instructions (1 KB each) of a wave
+  const unsigned char* base;
+  unsigned ldb, off[P];
+  int wave, lane;
+  __device__ __forceinline__ unsigned chunk_byte(int i, int chunks) const {
+    const int row = (wave * P + i) * (64 / X::CPR) + lane / X::CPR;
+    return (unsigned)min(lane % X::CPR ^ X::swz(row), chunks - 1) * 16u;      // (head sizes below DP: the owned operand is 0 there)
+  }
+  __device__ __forceinline__ int row_of(int i) const { return (wave * P + i) * (64 / X::CPR) + lane / X::CPR; }
+  __device__ __forceinline__ void init(const T* src, long long ld, int chunks, int wave_, int lane_) {
+    base = reinterpret_cast<const unsigned char*>(src);
+    ldb = (unsigned)ld * (unsigned)sizeof(T);
+    wave = wave_;
+    lane = lane_;
+#pragma unroll
+    for (int i = 0; i < P; ++i) off[i] = (unsigned)row_of(i) * ldb + chunk_byte(i, chunks);
+  }
+  // rows row0 .. row0 + KT - 1 into LDS; rows from `limit` (> row0) on re-read the last one
+  __device__ __forceinline__ void request(unsigned char* tile, long long skip, int row0, int limit) const {
+    const unsigned char* at = base + skip + (long long)row0 * ldb;
+    if (row0 + X::KT <= limit) {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        __builtin_amdgcn_global_load_lds((x_glb_void*)(at + off[i]), (x_lds_void*)(tile + (wave * P + i) * 1024), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int row = row_of(i);
+        const unsigned back = (unsigned)(row - min(row, limit - 1 - row0)) * ldb;
+        __builtin_amdgcn_global_load_lds((x_glb_void*)(at + (off[i] - back)), (x_lds_void*)(tile + (wave * P + i) * 1024), 16, 0, 0);
+      }
+    }
+  }
+};
+
 // acc[blk] (rows: dimension x_dim(blk, g, e), column: owned row) += tile^T w for all KT rows of the tile; w[kf][e] = weight of
 // row 16 kf + 4 g + e
-template <int DP, int N>
-__device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], const unsigned char* tile, const f32x4 (&w)[N][2],
-                                             float, int r, int g) {
+template <int OFF, bool SUM, int DP, int N>
+__device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], f32x4 (&)[N], const unsigned char* lds, const unsigned*,
+                                             const f32x4 (&w)[N][2], int r, int g) {
+  const unsigned char* tile = lds + OFF;
   typedef XTile<float, DP> X;
   constexpr int VW = DP / 16;
 #pragma unroll
@@ -106,71 +134,88 @@ __device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], const uns
     }
 }
 
-// four transposed fragments (16 dimensions each, 32 rows): eight reads and their wait in ONE statement, so that no other
-// instruction can touch a destination in between.  (The builtin is modelled as reading memory that an LDS-DMA in flight
-// may write: hipcc would wait for the next tile's DMA in front of it.)
+// Transposed fragments (16 dimensions each, 32 rows): the reads and their wait in ONE statement, so that no other
+// instruction can touch a destination in between.  (The builtin is modelled as reading memory that an LDS-DMA in flight may
+// write: hipcc would wait for the next tile's DMA in front of it.)  A lane has one address per 16 dimensions (per 16 of the first
+// 64: the swizzle leaves 128-byte steps alone); rows, tiles and buffers are offsets in the instruction.
 template <int DP>
-__device__ __forceinline__ const unsigned char* x_tr_addr(const unsigned char* tile, int row, int cbase, int r) {
+__device__ __forceinline__ void x_tr_addr(unsigned (&ta)[4], const unsigned char* lds, int r, int g) {
   typedef XTile<__bf16, DP> X;
-  const int b = r & 3, c = (cbase >> 3) + (b >> 1);
-  return tile + row * X::RB + ((c ^ X::swz(row)) << 4) + (b & 1) * 8;
+  const int row = 4 * g + (r >> 2), b = r & 3;
+#ifdef NSP_HOST_EMULATION
+  const unsigned at = 0;
+#else
+  typedef __attribute__((address_space(3))) unsigned char lds_uchar;
+  const unsigned at = (unsigned)(uintptr_t)((lds_uchar*)const_cast<unsigned char*>(lds));
+#endif
+#pragma unroll
+  for (int i = 0; i < (DP == 32 ? 2 : 4); ++i)
+    ta[i] = at + (unsigned)(row * X::RB + (((2 * i + (b >> 1)) ^ X::swz(row)) << 4) + (b & 1) * 8);
 }
-template <int DP, int NF>
-__device__ __forceinline__ void x_tr_read(bf16x8 (&out)[NF], const unsigned char* tile, int d0, int k0, int r, int g) {
-  const int ra = k0 + 4 * g + (r >> 2), rb = ra + 16;
+template <int OFF, int RB, int NF>
+__device__ __forceinline__ void x_tr_read(bf16x8 (&out)[NF], const unsigned char* lds, const unsigned* ta) {
   bf16x4 lo[NF], hi[NF];
 #ifdef NSP_HOST_EMULATION
   for (int i = 0; i < NF; ++i) {
-    lo[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)x_tr_addr<DP>(tile, ra, d0 + 16 * i, r));
-    hi[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)x_tr_addr<DP>(tile, rb, d0 + 16 * i, r));
+    lo[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OFF));
+    hi[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OFF + 16 * RB));
   }
 #else
-  typedef __attribute__((address_space(3))) unsigned char lds_uchar;
-  unsigned a[2 * NF];
-#pragma unroll
-  for (int i = 0; i < NF; ++i) {
-    a[2 * i] = (unsigned)(uintptr_t)((lds_uchar*)const_cast<unsigned char*>(x_tr_addr<DP>(tile, ra, d0 + 16 * i, r)));
-    a[2 * i + 1] = (unsigned)(uintptr_t)((lds_uchar*)const_cast<unsigned char*>(x_tr_addr<DP>(tile, rb, d0 + 16 * i, r)));
-  }
+  (void)lds;
   if constexpr (NF == 2)
-    asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %2, %6\n\t"
-                 "ds_read_b64_tr_b16 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+                 "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
-                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3])
+                 : "v"(ta[0]), "v"(ta[1]), "i"(OFF), "i"(OFF + 16 * RB)
                  : "memory");
   else
-    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %10\n\t"
-                 "ds_read_b64_tr_b16 %3, %11\n\tds_read_b64_tr_b16 %4, %12\n\tds_read_b64_tr_b16 %5, %13\n\t"
-                 "ds_read_b64_tr_b16 %6, %14\n\tds_read_b64_tr_b16 %7, %15\n\ts_waitcnt lgkmcnt(0)"
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
-                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7])
+                 : "v"(ta[0]), "v"(ta[1]), "v"(ta[2]), "v"(ta[3]), "i"(OFF), "i"(OFF + 16 * RB)
                  : "memory");
 #endif
 #pragma unroll
   for (int i = 0; i < NF; ++i) out[i] = __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7);
 }
-template <int DP, int N>
-__device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], const unsigned char* tile, const f32x4 (&w)[N][4],
-                                             __bf16, int r, int g) {
+// SUM: sum[f] (every element) += the column's weights as rounded, by a product with ones -- the matrix cores have room for it,
+// the vector units, which bound the forward kernel, do not
+template <int OFF, bool SUM, int DP, int N>
+__device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], f32x4 (&sum)[N], const unsigned char* lds,
+                                             const unsigned* ta, const f32x4 (&w)[N][4], int, int) {
+  typedef XTile<__bf16, DP> X;
   constexpr int NF = DP == 32 ? 2 : 4;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  auto half = [&](auto U) {
+    constexpr int u = decltype(U)::value;
     bf16x8 p[N];
 #pragma unroll
     for (int f = 0; f < N; ++f)
 #pragma unroll
       for (int i = 0; i < 8; ++i) p[f][i] = (__bf16)w[f][2 * u + (i >> 2)][i & 3];
+    if constexpr (SUM) {
+      bf16x8 one;
 #pragma unroll
-    for (int d0 = 0; d0 < DP; d0 += 16 * NF) {
+      for (int i = 0; i < 8; ++i) one[i] = (__bf16)1.f;
+#pragma unroll
+      for (int f = 0; f < N; ++f) sum[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(one, p[f], sum[f], 0, 0, 0);
+    }
+    auto block = [&](auto Q) {
+      constexpr int q = decltype(Q)::value;
       bf16x8 t[NF];
-      x_tr_read<DP, NF>(t, tile, d0, 32 * u, r, g);
+      x_tr_read<OFF + 32 * u * X::RB + 128 * q, X::RB, NF>(t, lds, ta);
 #pragma unroll
       for (int i = 0; i < NF; ++i)
 #pragma unroll
         for (int f = 0; f < N; ++f)
-          acc[f][d0 / 16 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t[i], p[f], acc[f][d0 / 16 + i], 0, 0, 0);
-    }
-  }
+          acc[f][4 * q + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t[i], p[f], acc[f][4 * q + i], 0, 0, 0);
+    };
+    block(std::integral_constant<int, 0>());
+    if constexpr (DP == 128) block(std::integral_constant<int, 1>());
+  };
+  half(std::integral_constant<int, 0>());
+  half(std::integral_constant<int, 1>());
 }
 
 // row `dst` (D elements) <- a transposed accumulator's column, times f; LO: what the rounding to T left, as T
@@ -274,26 +319,33 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
   typename X::E::chunk Q[NQ][X::NS];
   x_load_rows<T, NQ>(Q, reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)h * p.q_sh, p.q_st, q0, p.Tq,
                          p.D, r, g);
-  f32x4 o[NQ][X::NB];
+  constexpr bool SUM = sizeof(T) == 2 && !DROP;
+  f32x4 o[NQ][X::NB], sum[NQ];
   float m[NQ], l[NQ];
 #pragma unroll
   for (int f = 0; f < NQ; ++f) {
 #pragma unroll
     for (int i = 0; i < X::NB; ++i) o[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    sum[f] = f32x4{0.f, 0.f, 0.f, 0.f};
     m[f] = -INFINITY;
     l[f] = 0.f;
   }
+  unsigned ta[4];
+  if constexpr (sizeof(T) == 2) x_tr_addr<DP>(ta, lds, r, g);
+  XSource<T, DP> ks, vs;
+  ks.init(kb, p.k_st, chunks, wave, lane);
+  vs.init(vb, p.v_st, chunks, wave, lane);
   const int nkt = (klen + X::KT - 1) / X::KT;
-  X::dma(lds, kb, p.k_st, 0, klen, chunks, wave, lane);
-  X::dma(lds + X::BYTES, vb, p.v_st, 0, klen, chunks, wave, lane);
+  ks.request(lds, 0, 0, klen);
+  vs.request(lds + X::BYTES, 0, 0, klen);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  for (int kt = 0; kt < nkt; ++kt) {
-    const unsigned char* Kc = lds + (kt & 1) * (2 * X::BYTES);
+  auto step = [&](int kt, auto BUF) {
+    constexpr int AT = decltype(BUF)::value * 2 * X::BYTES, NEXT = 2 * X::BYTES - AT;
+    const unsigned char* Kc = lds + AT;
     if (kt + 1 < nkt) {     // the other buffers were last read in iteration kt - 1, behind that iteration's barrier
-      unsigned char* Kn = lds + ((kt + 1) & 1) * (2 * X::BYTES);
-      X::dma(Kn, kb, p.k_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
-      X::dma(Kn + X::BYTES, vb, p.v_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
+      ks.request(lds + NEXT, 0, (kt + 1) * X::KT, klen);
+      vs.request(lds + NEXT + X::BYTES, 0, (kt + 1) * X::KT, klen);
     }
     f32x4 s[NQ][KF];
     x_product<T, DP, NQ>(s, Kc, Q, r, g, XZero());
@@ -328,6 +380,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
         const float alpha = __builtin_amdgcn_exp2f(m[f] - mn);
         m[f] = mn;
         l[f] *= alpha;
+        sum[f] *= alpha;
 #pragma unroll
         for (int i = 0; i < X::NB; ++i) o[f][i] *= alpha;
       }
@@ -344,18 +397,22 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -m[f]));
-          l[f] += x;
+          if constexpr (!SUM) l[f] += x;
           s[f][kf][e] = DROP ? x * keep[e] : x;
         }
       }
     }
-    x_accumulate<DP, NQ>(o, Kc + X::BYTES, s, T(0), r, g);
+    x_accumulate<AT + X::BYTES, SUM, DP, NQ>(o, sum, lds, ta, s, r, g);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+  };
+  for (int kt = 0; kt < nkt; kt += 2) {
+    step(kt, std::integral_constant<int, 0>());
+    if (kt + 1 < nkt) step(kt + 1, std::integral_constant<int, 1>());
   }
 #pragma unroll
   for (int f = 0; f < NQ; ++f) {
-    const float inv = 1.f / attn_sum4(l[f]);
+    const float inv = 1.f / (SUM ? sum[f][0] : attn_sum4(l[f]));
     const int qi = q0 + 16 * f + r;
     if (qi >= p.Tq) continue;
     const long long at = (((long long)b * p.Tq + qi) * p.H + h) * p.D;
@@ -422,18 +479,24 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
     }
   }
   const int nkt = klen <= 0 ? 0 : (klen + X::KT - 1) / X::KT;     // no visible key: no gradient
+  unsigned ta[4];
+  f32x4 none[NQ];
+  if constexpr (sizeof(T) == 2) x_tr_addr<DP>(ta, lds, r, g);
+  XSource<T, DP> ks, vs;
+  ks.init(kb, p.k_st, chunks, wave, lane);
+  vs.init(vb, p.v_st, chunks, wave, lane);
   if (nkt > 0) {
-    X::dma(lds, kb, p.k_st, 0, klen, chunks, wave, lane);
-    X::dma(lds + X::BYTES, vb, p.v_st, 0, klen, chunks, wave, lane);
+    ks.request(lds, 0, 0, klen);
+    vs.request(lds + X::BYTES, 0, 0, klen);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  for (int kt = 0; kt < nkt; ++kt) {
-    const unsigned char* Kc = lds + (kt & 1) * (2 * X::BYTES);
+  auto step = [&](int kt, auto BUF) {
+    constexpr int AT = decltype(BUF)::value * 2 * X::BYTES, NEXT = 2 * X::BYTES - AT;
+    const unsigned char* Kc = lds + AT;
     if (kt + 1 < nkt) {
-      unsigned char* Kn = lds + ((kt + 1) & 1) * (2 * X::BYTES);
-      X::dma(Kn, kb, p.k_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
-      X::dma(Kn + X::BYTES, vb, p.v_st, (kt + 1) * X::KT, klen, chunks, wave, lane);
+      ks.request(lds + NEXT, 0, (kt + 1) * X::KT, klen);
+      vs.request(lds + NEXT + X::BYTES, 0, (kt + 1) * X::KT, klen);
     }
     f32x4 s[NQ][KF], dp[NQ][KF];
     x_product<T, DP, NQ>(s, Kc, Q, r, g, XZero());
@@ -465,9 +528,13 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
           for (int e = 0; e < 4; ++e)
             if (kt * X::KT + 16 * kf + 4 * g + e >= klen) s[f][kf][e] = 0.f;
     }
-    x_accumulate<DP, NQ>(acc, Kc, s, T(0), r, g);
+    x_accumulate<AT, false, DP, NQ>(acc, none, lds, ta, s, r, g);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+  };
+  for (int kt = 0; kt < nkt; kt += 2) {
+    step(kt, std::integral_constant<int, 0>());
+    if (kt + 1 < nkt) step(kt + 1, std::integral_constant<int, 1>());
   }
 #pragma unroll
   for (int f = 0; f < NQ; ++f) {
@@ -478,7 +545,7 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
 }
 
 template <typename T, int DP, int NK, bool DROP>
-__global__ __launch_bounds__(256, DP == 128 && NK == 2 ? 1 : 2) void cross_dkv_kernel(const XArgs p) {
+__global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
   constexpr int QF = X::KT / 16;
   // tiles, then per buffer KT maxima, KT reciprocal sums, KT values of D
@@ -518,23 +585,30 @@ __global__ __launch_bounds__(256, DP == 128 && NK == 2 ? 1 : 2) void cross_dkv_k
       if constexpr (sizeof(T) == 2) return which == 0 ? p.stats[at] - __log2f(p.stats[nst + at]) : 0.f;
       return p.stats[(which == 0 ? 0 : nst) + at];
     };
+    unsigned ta[4];
+    f32x4 none[NK];
+    if constexpr (sizeof(T) == 2) x_tr_addr<DP>(ta, lds, r, g);
+    XSource<T, DP> qs, gs;
+    qs.init(qb, p.q_st, chunks, wave, lane);
+    gs.init(gb, p.g_st, chunks, wave, lane);
     auto fetch = [&](unsigned char* to, int it) {
       const int hq = it / nqt, row0 = (it % nqt) * X::KT;
-      X::dma(to, qb + (long long)hq * p.q_sh, p.q_st, row0, p.Tq, chunks, wave, lane);
-      X::dma(to + X::BYTES, gb + (long long)hq * p.g_sh, p.g_st, row0, p.Tq, chunks, wave, lane);
+      qs.request(to, (long long)hq * p.q_sh * (long long)sizeof(T), row0, p.Tq);
+      gs.request(to + X::BYTES, (long long)hq * p.g_sh * (long long)sizeof(T), row0, p.Tq);
     };
     const float first = stat(0);
     if ((int)threadIdx.x < 3 * X::KT) st[threadIdx.x] = first;
     fetch(lds, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    for (int it = 0; it < n; ++it) {
-      const unsigned char* Qc = lds + (it & 1) * (2 * X::BYTES);
-      const float* sc = st + (it & 1) * (3 * X::KT);
+    auto step = [&](int it, auto BUF) {
+      constexpr int B01 = decltype(BUF)::value, AT = B01 * 2 * X::BYTES, NEXT = 2 * X::BYTES - AT;
+      const unsigned char* Qc = lds + AT;
+      const float* sc = st + B01 * (3 * X::KT);
       float next = 0.f;
       if (it + 1 < n) {
         next = stat(it + 1);
-        fetch(lds + ((it + 1) & 1) * (2 * X::BYTES), it + 1);
+        fetch(lds + NEXT, it + 1);
       }
       f32x4 s[NK][QF], dp[NK][QF];
       x_product<T, DP, NK>(s, Qc, K, r, g, XZero());
@@ -570,11 +644,15 @@ __global__ __launch_bounds__(256, DP == 128 && NK == 2 ? 1 : 2) void cross_dkv_k
             }
           }
       }
-      x_accumulate<DP, NK>(dv, Qc + X::BYTES, s, T(0), r, g);
-      x_accumulate<DP, NK>(dk, Qc, dp, T(0), r, g);
-      if (it + 1 < n && (int)threadIdx.x < 3 * X::KT) st[((it + 1) & 1) * (3 * X::KT) + threadIdx.x] = next;
+      x_accumulate<AT + X::BYTES, false, DP, NK>(dv, none, lds, ta, s, r, g);
+      x_accumulate<AT, false, DP, NK>(dk, none, lds, ta, dp, r, g);
+      if (it + 1 < n && (int)threadIdx.x < 3 * X::KT) st[(1 - B01) * (3 * X::KT) + threadIdx.x] = next;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
+    };
+    for (int it = 0; it < n; it += 2) {
+      step(it, std::integral_constant<int, 0>());
+      if (it + 1 < n) step(it + 1, std::integral_constant<int, 1>());
     }
   }
 #pragma unroll
@@ -628,11 +706,13 @@ template <typename T, int DP, bool DROP>
 int launch(const XArgs& p, bool bwd, hipStream_t st) {
   if constexpr (sizeof(T) == 2) {
     const bool two_q = p.Tq > 64 && (long long)p.B * p.H * ((p.Tq + 127) / 128) >= 512;
-    const bool two_k = p.Tk > 64 && (long long)p.B * p.Hkv * ((p.Tk + 127) / 128) >= 512;
+    const bool two_k = DP <= 64 && p.Tk > 64 && (long long)p.B * p.Hkv * ((p.Tk + 127) / 128) >= 512;
     if (!bwd) return two_q ? launch_fwd<T, DP, 2, DROP>(p, st) : launch_fwd<T, DP, 1, DROP>(p, st);
     const int rc = two_q ? launch_dq<T, DP, 2, DROP>(p, st) : launch_dq<T, DP, 1, DROP>(p, st);
     if (rc != NSP_OK) return rc;
-    return two_k ? launch_dkv<T, DP, 2, DROP>(p, st) : launch_dkv<T, DP, 1, DROP>(p, st);
+    if constexpr (DP <= 64)
+      if (two_k) return launch_dkv<T, DP, 2, DROP>(p, st);
+    return launch_dkv<T, DP, 1, DROP>(p, st);
   } else {
     if (!bwd) return launch_fwd<T, DP, 1, DROP>(p, st);
     const int rc = launch_dq<T, DP, 1, DROP>(p, st);
@@ -650,6 +730,8 @@ int cross_attn(const nsp_cross_attn_params* a, bool bwd, void* stream) {
   if (!a || a->B < 0 || a->Tq < 0 || a->Tk < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->D <= 0) return NSP_EINVAL;
   if (a->D % 8 || a->D > 128 || (a->dtype != NSP_DT_F32 && a->dtype != NSP_DT_BF16)) return NSP_EUNSUPPORTED;
   if (a->B * a->H > 0x7ffffff0LL || a->Tq > 0x7fffff00LL || a->Tk > 0x7fffff00LL || !(a->scale > 0.)) return NSP_EUNSUPPORTED;
+  const long long far = 1 << 24;      // (32-bit offsets inside a tile)
+  if (a->q_st >= far || a->k_st >= far || a->v_st >= far || a->g_st >= far) return NSP_EUNSUPPORTED;
   if (!(a->dropout_p >= 0. && a->dropout_p < 1.)) return NSP_EINVAL;
   if (a->B == 0 || a->Tk == 0 || (a->Tq == 0 && !bwd)) return NSP_OK;     // (nothing to read, or nothing to write but empty rows: the caller's)
   if (!a->k || !a->v || (a->Tq > 0 && (!a->q || !a->out))) return NSP_EINVAL;
