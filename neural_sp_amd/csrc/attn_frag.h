@@ -45,12 +45,14 @@ struct AttnElem<__bf16> {
 
 constexpr float NSP_LOG2E = 1.4426950408889634f;
 
+// (IEEE maximum: a NaN wins, and unlike fmaxf it needs no quieting of its operands first -- one instruction, or half of one)
+__device__ __forceinline__ float attn_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 // max / sum over the four lanes that share r (lanes r, r + 16, r + 32, r + 48): one lane-swap instruction per step
 __device__ __forceinline__ float attn_max4(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  v = attn_max(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  return attn_max(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float attn_sum4(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -51,6 +51,8 @@ struct XTile {
   static constexpr int NS = CPR / 4;                 // steps of a product over the head size
   static constexpr int NB = DP / 16;                 // 16-row blocks of a transposed accumulator
   static constexpr int BYTES = KT * RB;
+  static constexpr int U = KT / 32;                  // 32-row steps of a tile
+  static constexpr int HALF = 32 * RB;
   __device__ static __forceinline__ int swz(int row) { return RB >= 128 ? (row & 7) : ((row >> 1) & 3); }
   // operand of a product over the head size: chunk 4 s + g of row rbase + r
   __device__ static __forceinline__ typename E::chunk rows(const unsigned char* tile, int rbase, int s, int r, int g) {
@@ -99,45 +101,56 @@ struct XSource {
   }
 };
 
-// acc[blk] (rows: dimension x_dim(blk, g, e), column: owned row) += tile^T w for all KT rows of the tile; w[kf][e] = weight of
-// row 16 kf + 4 g + e
-template <int OFF, bool SUM, int DP, int N>
-__device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], f32x4 (&)[N], const unsigned char* lds, const unsigned*,
-                                             const f32x4 (&w)[N][2], int r, int g) {
-  const unsigned char* tile = lds + OFF;
-  typedef XTile<float, DP> X;
-  constexpr int VW = DP / 16;
-#pragma unroll
-  for (int kf = 0; kf < X::KT / 16; ++kf)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = 16 * kf + 4 * g + e;
-      const float* base = reinterpret_cast<const float*>(tile + row * X::RB);
-      float x[VW];
-#pragma unroll
-      for (int i = 0; i < VW; i += (VW < 4 ? VW : 4)) {
-        const int el = r * VW + i, c = el >> 2;
-        const float* p = base + ((c ^ X::swz(row)) << 2) + (el & 3);
-        if constexpr (VW == 2) {
-          const float2 a = *reinterpret_cast<const float2*>(p);
-          x[0] = a.x; x[1] = a.y;
-        } else {
-          const f32x4 a = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[i + j] = a[j];
-        }
-      }
-#pragma unroll
-      for (int f = 0; f < N; ++f)
-#pragma unroll
-        for (int j = 0; j < VW; ++j) acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], w[f][kf][e], acc[f][j], 0, 0, 0);
-    }
-}
+// ---- 32 rows of a tile as the operand of a product that runs over these rows:
+//   acc[f][blk] (rows: 16 dimensions, column: owned row) += sum over the rows  row^T w,  w[f][kf][e] = weight of row 16 kf + 4 g + e
+template <typename T, int DP>
+struct XAcross;
 
-// Transposed fragments (16 dimensions each, 32 rows): the reads and their wait in ONE statement, so that no other
+// fp32: a lane holds one contraction element per instruction and picks its row: dimension blk of row m is m * DP / 16 + blk
+template <int DP>
+struct XAcross<float, DP> {
+  typedef XTile<float, DP> X;
+  static constexpr int VW = DP / 16;
+  template <int OFF>
+  __device__ __forceinline__ void read(const unsigned char*, const unsigned*) {}
+  template <int OA, int OB>
+  __device__ static __forceinline__ void read2(XAcross&, XAcross&, const unsigned char*, const unsigned*) {}
+  template <int OFF, bool SUM, int N>
+  __device__ __forceinline__ void product(f32x4 (&acc)[N][VW], f32x4 (&)[N], const f32x4 (&w)[N][2], const unsigned char* lds, int r,
+                                          int g) const {
+#pragma unroll
+    for (int kf = 0; kf < 2; ++kf)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = 16 * kf + 4 * g + e;
+        const float* base = reinterpret_cast<const float*>(lds + OFF + row * X::RB);
+        float x[VW];
+#pragma unroll
+        for (int i = 0; i < VW; i += (VW < 4 ? VW : 4)) {
+          const int el = r * VW + i, c = el >> 2;
+          const float* p = base + ((c ^ X::swz(row)) << 2) + (el & 3);
+          if constexpr (VW == 2) {
+            const float2 a = *reinterpret_cast<const float2*>(p);
+            x[0] = a.x; x[1] = a.y;
+          } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i + j] = a[j];
+          }
+        }
+#pragma unroll
+        for (int f = 0; f < N; ++f)
+#pragma unroll
+          for (int j = 0; j < VW; ++j) acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], w[f][kf][e], acc[f][j], 0, 0, 0);
+      }
+  }
+};
+
+// bf16: transposing LDS reads, dimension blk of row m is 16 blk + m.  The reads and their wait are ONE statement, so that no other
 // instruction can touch a destination in between.  (The builtin is modelled as reading memory that an LDS-DMA in flight may
-// write: hipcc would wait for the next tile's DMA in front of it.)  A lane has one address per 16 dimensions (per 16 of the first
-// 64: the swizzle leaves 128-byte steps alone); rows, tiles and buffers are offsets in the instruction.
+// write: hipcc would wait for the next tile's DMA in front of it.)  The statement's wait hides behind the matrix instructions
+// issued before it: the callers put it between the score products and what needs their results.  A lane has one address per
+// 16 dimensions (of the first 64: the swizzle leaves 128-byte steps alone); rows, tiles and buffers are offsets in the instruction.
 template <int DP>
 __device__ __forceinline__ void x_tr_addr(unsigned (&ta)[4], const unsigned char* lds, int r, int g) {
   typedef XTile<__bf16, DP> X;
@@ -152,48 +165,108 @@ __device__ __forceinline__ void x_tr_addr(unsigned (&ta)[4], const unsigned char
   for (int i = 0; i < (DP == 32 ? 2 : 4); ++i)
     ta[i] = at + (unsigned)(row * X::RB + (((2 * i + (b >> 1)) ^ X::swz(row)) << 4) + (b & 1) * 8);
 }
-template <int OFF, int RB, int NF>
-__device__ __forceinline__ void x_tr_read(bf16x8 (&out)[NF], const unsigned char* lds, const unsigned* ta) {
-  bf16x4 lo[NF], hi[NF];
+// 4 + 4 fragments of 32 rows x 16 dimensions at byte offsets OA and OB
+template <int OA, int OB, int RB>
+__device__ __forceinline__ void x_tr_read16(bf16x8* a, bf16x8* b, const unsigned char* lds, const unsigned* ta) {
+  bf16x4 al[4], ah[4], bl[4], bh[4];
 #ifdef NSP_HOST_EMULATION
-  for (int i = 0; i < NF; ++i) {
+  for (int i = 0; i < 4; ++i) {
+    al[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OA));
+    ah[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OA + 16 * RB));
+    bl[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OB));
+    bh[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OB + 16 * RB));
+  }
+#else
+  (void)lds;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %16 offset:%20\n\tds_read_b64_tr_b16 %1, %16 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %2, %17 offset:%20\n\tds_read_b64_tr_b16 %3, %17 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %4, %18 offset:%20\n\tds_read_b64_tr_b16 %5, %18 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %6, %19 offset:%20\n\tds_read_b64_tr_b16 %7, %19 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %8, %16 offset:%22\n\tds_read_b64_tr_b16 %9, %16 offset:%23\n\t"
+      "ds_read_b64_tr_b16 %10, %17 offset:%22\n\tds_read_b64_tr_b16 %11, %17 offset:%23\n\t"
+      "ds_read_b64_tr_b16 %12, %18 offset:%22\n\tds_read_b64_tr_b16 %13, %18 offset:%23\n\t"
+      "ds_read_b64_tr_b16 %14, %19 offset:%22\n\tds_read_b64_tr_b16 %15, %19 offset:%23\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(al[0]), "=&v"(ah[0]), "=&v"(al[1]), "=&v"(ah[1]), "=&v"(al[2]), "=&v"(ah[2]), "=&v"(al[3]), "=&v"(ah[3]),
+        "=&v"(bl[0]), "=&v"(bh[0]), "=&v"(bl[1]), "=&v"(bh[1]), "=&v"(bl[2]), "=&v"(bh[2]), "=&v"(bl[3]), "=&v"(bh[3])
+      : "v"(ta[0]), "v"(ta[1]), "v"(ta[2]), "v"(ta[3]), "i"(OA), "i"(OA + 16 * RB), "i"(OB), "i"(OB + 16 * RB)
+      : "memory");
+#endif
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[i] = __builtin_shufflevector(al[i], ah[i], 0, 1, 2, 3, 4, 5, 6, 7);
+    b[i] = __builtin_shufflevector(bl[i], bh[i], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+template <int OFF, int RB>
+__device__ __forceinline__ void x_tr_read8(bf16x8* out, const unsigned char* lds, const unsigned* ta) {
+  bf16x4 lo[4], hi[4];
+#ifdef NSP_HOST_EMULATION
+  for (int i = 0; i < 4; ++i) {
     lo[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OFF));
     hi[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OFF + 16 * RB));
   }
 #else
   (void)lds;
-  if constexpr (NF == 2)
-    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
-                 "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
-                 : "v"(ta[0]), "v"(ta[1]), "i"(OFF), "i"(OFF + 16 * RB)
-                 : "memory");
-  else
-    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
-                 "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
-                 "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
-                 : "v"(ta[0]), "v"(ta[1]), "v"(ta[2]), "v"(ta[3]), "i"(OFF), "i"(OFF + 16 * RB)
-                 : "memory");
+  asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
+               : "v"(ta[0]), "v"(ta[1]), "v"(ta[2]), "v"(ta[3]), "i"(OFF), "i"(OFF + 16 * RB)
+               : "memory");
 #endif
 #pragma unroll
-  for (int i = 0; i < NF; ++i) out[i] = __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7);
+  for (int i = 0; i < 4; ++i) out[i] = __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// SUM: sum[f] (every element) += the column's weights as rounded, by a product with ones -- the matrix cores have room for it,
-// the vector units, which bound the forward kernel, do not
-template <int OFF, bool SUM, int DP, int N>
-__device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], f32x4 (&sum)[N], const unsigned char* lds,
-                                             const unsigned* ta, const f32x4 (&w)[N][4], int, int) {
+template <int OFF, int RB>
+__device__ __forceinline__ void x_tr_read4(bf16x8* out, const unsigned char* lds, const unsigned* ta) {
+  bf16x4 lo[2], hi[2];
+#ifdef NSP_HOST_EMULATION
+  for (int i = 0; i < 2; ++i) {
+    lo[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OFF));
+    hi[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((x_lds_bf16x4*)(lds + ta[i] + OFF + 16 * RB));
+  }
+#else
+  (void)lds;
+  asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+               "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
+               : "v"(ta[0]), "v"(ta[1]), "i"(OFF), "i"(OFF + 16 * RB)
+               : "memory");
+#endif
+#pragma unroll
+  for (int i = 0; i < 2; ++i) out[i] = __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int DP>
+struct XAcross<__bf16, DP> {
   typedef XTile<__bf16, DP> X;
-  constexpr int NF = DP == 32 ? 2 : 4;
-  auto half = [&](auto U) {
-    constexpr int u = decltype(U)::value;
+  bf16x8 t[X::NB];
+  template <int OFF>
+  __device__ __forceinline__ void read(const unsigned char* lds, const unsigned* ta) {
+    if constexpr (DP == 32) x_tr_read4<OFF, X::RB>(t, lds, ta);
+    else if constexpr (DP == 64) x_tr_read8<OFF, X::RB>(t, lds, ta);
+    else x_tr_read16<OFF, OFF + 128, X::RB>(t, t + 4, lds, ta);
+  }
+  template <int OA, int OB>
+  __device__ static __forceinline__ void read2(XAcross& a, XAcross& b, const unsigned char* lds, const unsigned* ta) {
+    if constexpr (DP == 64) {
+      x_tr_read16<OA, OB, X::RB>(a.t, b.t, lds, ta);
+    } else {
+      a.template read<OA>(lds, ta);
+      b.template read<OB>(lds, ta);
+    }
+  }
+  // SUM: sum[f] (every element) += the column's weights as rounded, by a product with ones -- the matrix cores have room for
+  // it, the vector units, which bound the forward kernel, do not
+  template <int OFF, bool SUM, int N>
+  __device__ __forceinline__ void product(f32x4 (&acc)[N][X::NB], f32x4 (&sum)[N], const f32x4 (&w)[N][2], const unsigned char*, int,
+                                          int) const {
     bf16x8 p[N];
 #pragma unroll
     for (int f = 0; f < N; ++f)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[f][i] = (__bf16)w[f][2 * u + (i >> 2)][i & 3];
+      for (int i = 0; i < 8; ++i) p[f][i] = (__bf16)w[f][i >> 2][i & 3];
     if constexpr (SUM) {
       bf16x8 one;
 #pragma unroll
@@ -201,22 +274,12 @@ __device__ __forceinline__ void x_accumulate(f32x4 (&acc)[N][DP / 16], f32x4 (&s
 #pragma unroll
       for (int f = 0; f < N; ++f) sum[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(one, p[f], sum[f], 0, 0, 0);
     }
-    auto block = [&](auto Q) {
-      constexpr int q = decltype(Q)::value;
-      bf16x8 t[NF];
-      x_tr_read<OFF + 32 * u * X::RB + 128 * q, X::RB, NF>(t, lds, ta);
 #pragma unroll
-      for (int i = 0; i < NF; ++i)
+    for (int i = 0; i < X::NB; ++i)
 #pragma unroll
-        for (int f = 0; f < N; ++f)
-          acc[f][4 * q + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t[i], p[f], acc[f][4 * q + i], 0, 0, 0);
-    };
-    block(std::integral_constant<int, 0>());
-    if constexpr (DP == 128) block(std::integral_constant<int, 1>());
-  };
-  half(std::integral_constant<int, 0>());
-  half(std::integral_constant<int, 1>());
-}
+      for (int f = 0; f < N; ++f) acc[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t[i], p[f], acc[f][i], 0, 0, 0);
+  }
+};
 
 // row `dst` (D elements) <- a transposed accumulator's column, times f; LO: what the rounding to T left, as T
 template <int DP, bool LO>
@@ -276,14 +339,14 @@ __device__ __forceinline__ void x_load_rows(typename AttnElem<T>::chunk (&f)[N][
   }
 }
 
-// score tile: s[f][kf] rows = streamed rows 16 kf + 4 g + e, column = owned row; init(f, kf) is added (the matrix instruction's
-// accumulator starts with it)
-template <typename T, int DP, int N, int KF, int NS, class I>
-__device__ __forceinline__ void x_product(f32x4 (&s)[N][KF], const unsigned char* tile,
+// scores of 32 streamed rows: s[f][kf] rows = streamed rows 16 kf + 4 g + e, column = owned row; init(f, kf) is added (the matrix
+// instruction's accumulator starts with it)
+template <typename T, int DP, int N, int NS, class I>
+__device__ __forceinline__ void x_product(f32x4 (&s)[N][2], const unsigned char* tile,
                                           const typename AttnElem<T>::chunk (&own)[N][NS], int r, int g, I init) {
   typedef XTile<T, DP> X;
 #pragma unroll
-  for (int kf = 0; kf < KF; ++kf) {
+  for (int kf = 0; kf < 2; ++kf) {
 #pragma unroll
     for (int f = 0; f < N; ++f) s[f][kf] = init(f, kf);
 #pragma unroll
@@ -301,7 +364,6 @@ struct XZero {
 template <typename T, int DP, int NQ, bool DROP>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
-  constexpr int KF = X::KT / 16;
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -347,18 +409,25 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
       ks.request(lds + NEXT, 0, (kt + 1) * X::KT, klen);
       vs.request(lds + NEXT + X::BYTES, 0, (kt + 1) * X::KT, klen);
     }
-    f32x4 s[NQ][KF];
-    x_product<T, DP, NQ>(s, Kc, Q, r, g, XZero());
+    f32x4 s[X::U][NQ][2];
+#pragma unroll
+    for (int u = 0; u < X::U; ++u) x_product<T, DP, NQ>(s[u], Kc + u * X::HALF, Q, r, g, XZero());
+    __builtin_amdgcn_sched_barrier(0);      // (the products are under way while the values are read)
+    XAcross<T, DP> v[X::U];
+    if constexpr (X::U == 2) XAcross<T, DP>::template read2<AT + X::BYTES, AT + X::BYTES + X::HALF>(v[0], v[X::U - 1], lds, ta);
+    __builtin_amdgcn_sched_barrier(0);
     if (uniform || (kt + 1) * X::KT > klen) {
 #pragma unroll
-      for (int f = 0; f < NQ; ++f)
+      for (int u = 0; u < X::U; ++u)
 #pragma unroll
-        for (int kf = 0; kf < KF; ++kf)
+        for (int f = 0; f < NQ; ++f)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (uniform) s[f][kf][e] = 0.f;
-            if (kt * X::KT + 16 * kf + 4 * g + e >= klen) s[f][kf][e] = -INFINITY;
-          }
+          for (int kf = 0; kf < 2; ++kf)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (uniform) s[u][f][kf][e] = 0.f;
+              if (kt * X::KT + 32 * u + 16 * kf + 4 * g + e >= klen) s[u][f][kf][e] = -INFINITY;
+            }
     }
     // The reference maximum moves only when a score exceeds it by 2^8: exponentials then stay below 2^8 (exact in range for both
     // types, and bf16 keeps its relative precision), and after the first tiles nothing is rescaled any more.
@@ -366,17 +435,19 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
     bool move = false;
 #pragma unroll
     for (int f = 0; f < NQ; ++f) {
-      mx[f] = s[f][0][0];
+      mx[f] = s[0][f][0][0];
 #pragma unroll
-      for (int kf = 0; kf < KF; ++kf)
-        mx[f] = fmaxf(fmaxf(fmaxf(mx[f], s[f][kf][0]), fmaxf(s[f][kf][1], s[f][kf][2])), s[f][kf][3]);
+      for (int u = 0; u < X::U; ++u)
+#pragma unroll
+        for (int kf = 0; kf < 2; ++kf)
+          mx[f] = attn_max(attn_max(attn_max(mx[f], s[u][f][kf][0]), attn_max(s[u][f][kf][1], s[u][f][kf][2])), s[u][f][kf][3]);
       mx[f] = attn_max4(mx[f]) * p.sl2;    // (scale > 0: the maximum commutes with it; a tile has a visible key: finite)
       move = move || !(mx[f] <= m[f] + 8.f);
     }
     if (__any(move)) {
 #pragma unroll
       for (int f = 0; f < NQ; ++f) {
-        const float mn = fmaxf(m[f], mx[f]);
+        const float mn = attn_max(m[f], mx[f]);
         const float alpha = __builtin_amdgcn_exp2f(m[f] - mn);
         m[f] = mn;
         l[f] *= alpha;
@@ -391,18 +462,22 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
       const unsigned long long row =
           DROP ? p.offset + (unsigned long long)((((long long)b * p.H + h) * p.Tq + qi) * p.Tk) : 0ull;
 #pragma unroll
-      for (int kf = 0; kf < KF; ++kf) {
-        float keep[4];
-        if constexpr (DROP) nsp_keep_scale4(p.seed, row + (unsigned long long)(kt * X::KT + 16 * kf + 4 * g), p.drop, keep);
+      for (int u = 0; u < X::U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -m[f]));
-          if constexpr (!SUM) l[f] += x;
-          s[f][kf][e] = DROP ? x * keep[e] : x;
+        for (int kf = 0; kf < 2; ++kf) {
+          float keep[4];
+          if constexpr (DROP)
+            nsp_keep_scale4(p.seed, row + (unsigned long long)(kt * X::KT + 32 * u + 16 * kf + 4 * g), p.drop, keep);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[u][f][kf][e], p.sl2, -m[f]));
+            if constexpr (!SUM) l[f] += x;
+            s[u][f][kf][e] = DROP ? x * keep[e] : x;
+          }
         }
-      }
     }
-    x_accumulate<AT + X::BYTES, SUM, DP, NQ>(o, sum, lds, ta, s, r, g);
+    v[0].template product<AT + X::BYTES, SUM, NQ>(o, sum, s[0], lds, r, g);
+    if constexpr (X::U == 2) v[1].template product<AT + X::BYTES + X::HALF, SUM, NQ>(o, sum, s[1], lds, r, g);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   };
@@ -429,7 +504,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
 template <typename T, int DP, int NQ, bool DROP>
 __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
-  constexpr int KF = X::KT / 16;
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -443,6 +517,17 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
   const T* vb = reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh;
   const int chunks = p.D / X::E::CE;
   const long long srow = ((long long)b * p.H + h) * p.Tq;
+  const int nkt = klen <= 0 ? 0 : (klen + X::KT - 1) / X::KT;     // no visible key: no gradient
+  unsigned ta[4];
+  f32x4 none[NQ];
+  if constexpr (sizeof(T) == 2) x_tr_addr<DP>(ta, lds, r, g);
+  XSource<T, DP> ks, vs;
+  ks.init(kb, p.k_st, chunks, wave, lane);
+  vs.init(vb, p.v_st, chunks, wave, lane);
+  if (nkt > 0) {
+    ks.request(lds, 0, 0, klen);
+    vs.request(lds + X::BYTES, 0, 0, klen);
+  }
   typename X::E::chunk Q[NQ][X::NS], dO[NQ][X::NS];
   x_load_rows<T, NQ>(Q, reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)h * p.q_sh, p.q_st, q0, p.Tq,
                          p.D, r, g);
@@ -478,57 +563,56 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
       for (int i = 0; i < X::NB; ++i) acc[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
-  const int nkt = klen <= 0 ? 0 : (klen + X::KT - 1) / X::KT;     // no visible key: no gradient
-  unsigned ta[4];
-  f32x4 none[NQ];
-  if constexpr (sizeof(T) == 2) x_tr_addr<DP>(ta, lds, r, g);
-  XSource<T, DP> ks, vs;
-  ks.init(kb, p.k_st, chunks, wave, lane);
-  vs.init(vb, p.v_st, chunks, wave, lane);
-  if (nkt > 0) {
-    ks.request(lds, 0, 0, klen);
-    vs.request(lds + X::BYTES, 0, 0, klen);
-  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   auto step = [&](int kt, auto BUF) {
     constexpr int AT = decltype(BUF)::value * 2 * X::BYTES, NEXT = 2 * X::BYTES - AT;
-    const unsigned char* Kc = lds + AT;
     if (kt + 1 < nkt) {
       ks.request(lds + NEXT, 0, (kt + 1) * X::KT, klen);
       vs.request(lds + NEXT + X::BYTES, 0, (kt + 1) * X::KT, klen);
     }
-    f32x4 s[NQ][KF], dp[NQ][KF];
-    x_product<T, DP, NQ>(s, Kc, Q, r, g, XZero());
-    // dP - D in one go (with dropout D comes after the mask)
-    x_product<T, DP, NQ>(dp, Kc + X::BYTES, dO, r, g,
-                         [&](int f, int) -> f32x4 { return DROP ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{-ds[f], -ds[f], -ds[f], -ds[f]}; });
+    auto rows32 = [&](auto UC) {
+      constexpr int u = decltype(UC)::value, R = AT + u * X::HALF;
+      f32x4 s[NQ][2], dp[NQ][2];
+      x_product<T, DP, NQ>(s, lds + R, Q, r, g, XZero());
+      // dP - D in one go (with dropout D comes after the mask)
+      x_product<T, DP, NQ>(dp, lds + R + X::BYTES, dO, r, g, [&](int f, int) -> f32x4 {
+        return DROP ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{-ds[f], -ds[f], -ds[f], -ds[f]};
+      });
+      __builtin_amdgcn_sched_barrier(0);
+      XAcross<T, DP> k;
+      k.template read<R>(lds, ta);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int f = 0; f < NQ; ++f) {
-      const int qi = min(q0 + 16 * f + r, p.Tq - 1);
-      const unsigned long long row = DROP ? p.offset + (unsigned long long)((srow + qi) * p.Tk) : 0ull;
+      for (int f = 0; f < NQ; ++f) {
+        const int qi = min(q0 + 16 * f + r, p.Tq - 1);
+        const unsigned long long row = DROP ? p.offset + (unsigned long long)((srow + qi) * p.Tk) : 0ull;
 #pragma unroll
-      for (int kf = 0; kf < KF; ++kf) {
-        float keep[4];
-        if constexpr (DROP) nsp_keep_scale4(p.seed, row + (unsigned long long)(kt * X::KT + 16 * kf + 4 * g), p.drop, keep);
+        for (int kf = 0; kf < 2; ++kf) {
+          float keep[4];
+          if constexpr (DROP)
+            nsp_keep_scale4(p.seed, row + (unsigned long long)(kt * X::KT + 32 * u + 16 * kf + 4 * g), p.drop, keep);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -m[f]));
-          if constexpr (sizeof(T) == 4) x *= inv[f];
-          s[f][kf][e] = x * (DROP ? fmaf(dp[f][kf][e], keep[e], -ds[f]) : dp[f][kf][e]);
+          for (int e = 0; e < 4; ++e) {
+            float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -m[f]));
+            if constexpr (sizeof(T) == 4) x *= inv[f];
+            s[f][kf][e] = x * (DROP ? fmaf(dp[f][kf][e], keep[e], -ds[f]) : dp[f][kf][e]);
+          }
         }
       }
-    }
-    if ((kt + 1) * X::KT > klen) {
+      if (kt * X::KT + 32 * (u + 1) > klen) {
 #pragma unroll
-      for (int f = 0; f < NQ; ++f)
+        for (int f = 0; f < NQ; ++f)
 #pragma unroll
-        for (int kf = 0; kf < KF; ++kf)
+          for (int kf = 0; kf < 2; ++kf)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (kt * X::KT + 16 * kf + 4 * g + e >= klen) s[f][kf][e] = 0.f;
-    }
-    x_accumulate<AT, false, DP, NQ>(acc, none, lds, ta, s, r, g);
+            for (int e = 0; e < 4; ++e)
+              if (kt * X::KT + 32 * u + 16 * kf + 4 * g + e >= klen) s[f][kf][e] = 0.f;
+      }
+      k.template product<R, false, NQ>(acc, none, s, lds, r, g);
+    };
+    rows32(std::integral_constant<int, 0>());
+    if constexpr (X::U == 2) rows32(std::integral_constant<int, 1>());
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   };
@@ -547,7 +631,6 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
 template <typename T, int DP, int NK, bool DROP>
 __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
-  constexpr int QF = X::KT / 16;
   // tiles, then per buffer KT maxima, KT reciprocal sums, KT values of D
   __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES + 2 * 3 * X::KT * 4];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -567,11 +650,6 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
     for (int i = 0; i < X::NB; ++i) dk[f][i] = dv[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (item * (64 * NK) < klen && p.Tq > 0) {      // (uniform over the workgroup; keys behind klen get zeros)
     const int chunks = p.D / X::E::CE, nqt = (p.Tq + X::KT - 1) / X::KT, n = G * nqt;
-    typename X::E::chunk K[NK][X::NS], V[NK][X::NS];
-    x_load_rows<T, NK>(K, reinterpret_cast<const T*>(p.k) + (long long)b * p.k_sb + (long long)hkv * p.k_sh, p.k_st, k0, klen,
-                          p.D, r, g);
-    x_load_rows<T, NK>(V, reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh, p.v_st, k0, klen,
-                          p.D, r, g);
     const T* qb = reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)hkv * G * p.q_sh;
     const T* gb = reinterpret_cast<const T*>(p.dout) + (long long)b * p.g_sb + (long long)hkv * G * p.g_sh;
     const long long srow = ((long long)b * p.H + (long long)hkv * G) * p.Tq, nst = (long long)p.B * p.H * p.Tq;
@@ -596,56 +674,68 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
       qs.request(to, (long long)hq * p.q_sh * (long long)sizeof(T), row0, p.Tq);
       gs.request(to + X::BYTES, (long long)hq * p.g_sh * (long long)sizeof(T), row0, p.Tq);
     };
+    fetch(lds, 0);
+    typename X::E::chunk K[NK][X::NS], V[NK][X::NS];
+    x_load_rows<T, NK>(K, reinterpret_cast<const T*>(p.k) + (long long)b * p.k_sb + (long long)hkv * p.k_sh, p.k_st, k0, klen,
+                          p.D, r, g);
+    x_load_rows<T, NK>(V, reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh, p.v_st, k0, klen,
+                          p.D, r, g);
     const float first = stat(0);
     if ((int)threadIdx.x < 3 * X::KT) st[threadIdx.x] = first;
-    fetch(lds, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     auto step = [&](int it, auto BUF) {
       constexpr int B01 = decltype(BUF)::value, AT = B01 * 2 * X::BYTES, NEXT = 2 * X::BYTES - AT;
-      const unsigned char* Qc = lds + AT;
       const float* sc = st + B01 * (3 * X::KT);
       float next = 0.f;
       if (it + 1 < n) {
         next = stat(it + 1);
         fetch(lds + NEXT, it + 1);
       }
-      f32x4 s[NK][QF], dp[NK][QF];
-      x_product<T, DP, NK>(s, Qc, K, r, g, XZero());
-      x_product<T, DP, NK>(dp, Qc + X::BYTES, V, r, g, [&](int, int qf) -> f32x4 {
-        return DROP ? f32x4{0.f, 0.f, 0.f, 0.f} : -*reinterpret_cast<const f32x4*>(sc + 2 * X::KT + 16 * qf + 4 * g);
-      });
-      if (uniform) {
+      auto rows32 = [&](auto UC) {
+        constexpr int u = decltype(UC)::value, R = AT + u * X::HALF;
+        f32x4 s[NK][2], dp[NK][2];
+        x_product<T, DP, NK>(s, lds + R, K, r, g, XZero());
+        x_product<T, DP, NK>(dp, lds + R + X::BYTES, V, r, g, [&](int, int qf) -> f32x4 {
+          return DROP ? f32x4{0.f, 0.f, 0.f, 0.f} : -*reinterpret_cast<const f32x4*>(sc + 2 * X::KT + 32 * u + 16 * qf + 4 * g);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        XAcross<T, DP> go, qo;
+        XAcross<T, DP>::template read2<R + X::BYTES, R>(go, qo, lds, ta);
+        __builtin_amdgcn_sched_barrier(0);
+        if (uniform) {
 #pragma unroll
-        for (int f = 0; f < NK; ++f)
+          for (int f = 0; f < NK; ++f) s[f][0] = s[f][1] = f32x4{0.f, 0.f, 0.f, 0.f};      // (exponent 0 - 0, see the forward kernel)
+        }
 #pragma unroll
-          for (int qf = 0; qf < QF; ++qf) s[f][qf] = f32x4{0.f, 0.f, 0.f, 0.f};      // (exponent 0 - 0, see the forward kernel)
-      }
+        for (int qf = 0; qf < 2; ++qf) {
+          const int at = 32 * u + 16 * qf + 4 * g;
+          const f32x4 m4 = *reinterpret_cast<const f32x4*>(sc + at);
+          const f32x4 i4 = *reinterpret_cast<const f32x4*>(sc + X::KT + at);
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(sc + 2 * X::KT + at);
 #pragma unroll
-      for (int qf = 0; qf < QF; ++qf) {
-        const f32x4 m4 = *reinterpret_cast<const f32x4*>(sc + 16 * qf + 4 * g);
-        const f32x4 i4 = *reinterpret_cast<const f32x4*>(sc + X::KT + 16 * qf + 4 * g);
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(sc + 2 * X::KT + 16 * qf + 4 * g);
+          for (int f = 0; f < NK; ++f)
 #pragma unroll
-        for (int f = 0; f < NK; ++f)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = __builtin_amdgcn_exp2f(fmaf(s[f][qf][e], p.sl2, -m4[e]));
-            if constexpr (sizeof(T) == 4) x *= i4[e];
-            if constexpr (DROP) {
-              const int qi = min((it % nqt) * X::KT + 16 * qf + 4 * g + e, p.Tq - 1);
-              const float keep = nsp_keep_scale(
-                  p.seed, p.offset + (unsigned long long)((srow + (long long)(it / nqt) * p.Tq + qi) * p.Tk + k0 + 16 * f + r), p.drop);
-              dp[f][qf][e] = x * fmaf(dp[f][qf][e], keep, -d4[e]);
-              s[f][qf][e] = x * keep;
-            } else {
-              dp[f][qf][e] *= x;
-              s[f][qf][e] = x;
+            for (int e = 0; e < 4; ++e) {
+              float x = __builtin_amdgcn_exp2f(fmaf(s[f][qf][e], p.sl2, -m4[e]));
+              if constexpr (sizeof(T) == 4) x *= i4[e];
+              if constexpr (DROP) {
+                const int qi = min((it % nqt) * X::KT + at + e, p.Tq - 1);
+                const float keep = nsp_keep_scale(
+                    p.seed, p.offset + (unsigned long long)((srow + (long long)(it / nqt) * p.Tq + qi) * p.Tk + k0 + 16 * f + r), p.drop);
+                dp[f][qf][e] = x * fmaf(dp[f][qf][e], keep, -d4[e]);
+                s[f][qf][e] = x * keep;
+              } else {
+                dp[f][qf][e] *= x;
+                s[f][qf][e] = x;
+              }
             }
-          }
-      }
-      x_accumulate<AT + X::BYTES, false, DP, NK>(dv, none, lds, ta, s, r, g);
-      x_accumulate<AT, false, DP, NK>(dk, none, lds, ta, dp, r, g);
+        }
+        go.template product<R + X::BYTES, false, NK>(dv, none, s, lds, r, g);
+        qo.template product<R, false, NK>(dk, none, dp, lds, r, g);
+      };
+      rows32(std::integral_constant<int, 0>());
+      if constexpr (X::U == 2) rows32(std::integral_constant<int, 1>());
       if (it + 1 < n && (int)threadIdx.x < 3 * X::KT) st[(1 - B01) * (3 * X::KT) + threadIdx.x] = next;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
