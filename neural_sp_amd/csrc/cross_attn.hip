@@ -29,7 +29,7 @@ struct XArgs {
   const void *q, *k, *v, *dout;
   void *out, *o_lo, *dq, *dk, *dv;
   float* stats;        // [2][B,H,Tq]: maximum, 1 / sum
-  float* dsum;         // [B,H,Tq]
+  float* rows;         // [3][B,H,Tq rounded up to 64]: what dK / dV need of every query, from the dQ kernel
   const int* klens;
   int B, H, Hkv, D, Tq, Tk;
   long long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
@@ -53,6 +53,9 @@ struct XTile {
   static constexpr int BYTES = KT * RB;
   static constexpr int U = KT / 32;                  // 32-row steps of a tile
   static constexpr int HALF = 32 * RB;
+  // pairs of tiles in LDS: with three, two are on their way while one is worked on (48 KB and three workgroups per compute unit);
+  // the 128-wide pairs are too large for that
+  static constexpr int STAGES = DP <= 64 ? 3 : 2;
   __device__ static __forceinline__ int swz(int row) { return RB >= 128 ? (row & 7) : ((row >> 1) & 3); }
   // operand of a product over the head size: chunk 4 s + g of row rbase + r
   __device__ static __forceinline__ typename E::chunk rows(const unsigned char* tile, int rbase, int s, int r, int g) {
@@ -357,6 +360,17 @@ __device__ __forceinline__ void x_product(f32x4 (&s)[N][2], const unsigned char*
     }
   }
 }
+// Behind the last read of a tile: the next one has landed (all but the newest `NEWER` requests of the wave are done; `last`: all)
+// and every wave has read this one.  A bare barrier: the fence of __syncthreads would wait for the tiles still on their way.
+template <int NEWER>
+__device__ __forceinline__ void x_turn(bool last) {
+  if (NEWER > 0 && !last) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NEWER) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 struct XZero {
   __device__ __forceinline__ f32x4 operator()(int, int) const { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 };
@@ -364,7 +378,7 @@ struct XZero {
 template <typename T, int DP, int NQ, bool DROP>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[X::STAGES * 2 * X::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int G = p.H / p.Hkv, nqt = (p.Tq + 64 * NQ - 1) / (64 * NQ);
@@ -398,17 +412,19 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
   ks.init(kb, p.k_st, chunks, wave, lane);
   vs.init(vb, p.v_st, chunks, wave, lane);
   const int nkt = (klen + X::KT - 1) / X::KT;
-  ks.request(lds, 0, 0, klen);
-  vs.request(lds + X::BYTES, 0, 0, klen);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  constexpr int PAIR = 2 * X::BYTES, AHEAD = X::STAGES - 1, NEWER = (AHEAD - 1) * 2 * XSource<T, DP>::P;
+  auto fetch = [&](int at, int kt) {
+    ks.request(lds + at, 0, kt * X::KT, klen);
+    vs.request(lds + at + X::BYTES, 0, kt * X::KT, klen);
+  };
+  fetch(0, 0);
+  if (AHEAD > 1 && nkt > 1) fetch(PAIR, 1);
+  x_turn<NEWER>(nkt <= AHEAD - 1);
   auto step = [&](int kt, auto BUF) {
-    constexpr int AT = decltype(BUF)::value * 2 * X::BYTES, NEXT = 2 * X::BYTES - AT;
+    constexpr int AT = decltype(BUF)::value * PAIR, NEXT = (decltype(BUF)::value + AHEAD) % X::STAGES * PAIR;
     const unsigned char* Kc = lds + AT;
-    if (kt + 1 < nkt) {     // the other buffers were last read in iteration kt - 1, behind that iteration's barrier
-      ks.request(lds + NEXT, 0, (kt + 1) * X::KT, klen);
-      vs.request(lds + NEXT + X::BYTES, 0, (kt + 1) * X::KT, klen);
-    }
+    // (that buffer was last read in step kt - 1, behind that step's barrier)
+    if (kt + AHEAD < nkt) fetch(NEXT, kt + AHEAD);
     f32x4 s[X::U][NQ][2];
 #pragma unroll
     for (int u = 0; u < X::U; ++u) x_product<T, DP, NQ>(s[u], Kc + u * X::HALF, Q, r, g, XZero());
@@ -478,12 +494,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
     }
     v[0].template product<AT + X::BYTES, SUM, NQ>(o, sum, s[0], lds, r, g);
     if constexpr (X::U == 2) v[1].template product<AT + X::BYTES + X::HALF, SUM, NQ>(o, sum, s[1], lds, r, g);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    x_turn<NEWER>(kt + AHEAD >= nkt);
   };
-  for (int kt = 0; kt < nkt; kt += 2) {
+  for (int kt = 0; kt < nkt; kt += X::STAGES) {
     step(kt, std::integral_constant<int, 0>());
     if (kt + 1 < nkt) step(kt + 1, std::integral_constant<int, 1>());
+    if constexpr (X::STAGES == 3)
+      if (kt + 2 < nkt) step(kt + 2, std::integral_constant<int, 2>());
   }
 #pragma unroll
   for (int f = 0; f < NQ; ++f) {
@@ -504,7 +521,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
 template <typename T, int DP, int NQ, bool DROP>
 __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[X::STAGES * 2 * X::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int G = p.H / p.Hkv, nqt = (p.Tq + 64 * NQ - 1) / (64 * NQ);
@@ -524,10 +541,12 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
   XSource<T, DP> ks, vs;
   ks.init(kb, p.k_st, chunks, wave, lane);
   vs.init(vb, p.v_st, chunks, wave, lane);
-  if (nkt > 0) {
-    ks.request(lds, 0, 0, klen);
-    vs.request(lds + X::BYTES, 0, 0, klen);
-  }
+  constexpr int PAIR = 2 * X::BYTES, AHEAD = X::STAGES - 1, NEWER = (AHEAD - 1) * 2 * XSource<T, DP>::P;
+  auto fetch = [&](int at, int kt) {
+    ks.request(lds + at, 0, kt * X::KT, klen);
+    vs.request(lds + at + X::BYTES, 0, kt * X::KT, klen);
+  };
+  if (nkt > 0) fetch(0, 0);
   typename X::E::chunk Q[NQ][X::NS], dO[NQ][X::NS];
   x_load_rows<T, NQ>(Q, reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)h * p.q_sh, p.q_st, q0, p.Tq,
                          p.D, r, g);
@@ -558,19 +577,23 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
       m[f] = p.stats[srow + qi];
       inv[f] = p.stats[(long long)p.B * p.H * p.Tq + srow + qi];
       if constexpr (sizeof(T) == 2) m[f] -= __log2f(inv[f]);      // (one rounding of the exponent more, far below bf16's)
-      if (g == 0 && q0 + 16 * f + r < p.Tq) p.dsum[srow + qi] = ds[f];
+      // for the dK / dV kernel, which reads 64 at a time: rows behind the last query have probability 0
+      const int pitch = (p.Tq + 63) / 64 * 64, q = q0 + 16 * f + r;
+      if (g == 0 && q < pitch) {
+        const long long at = ((long long)b * p.H + h) * pitch + q, n = (long long)p.B * p.H * pitch;
+        p.rows[at] = q < p.Tq ? m[f] : INFINITY;
+        p.rows[n + at] = q < p.Tq ? inv[f] : 0.f;
+        p.rows[2 * n + at] = q < p.Tq ? ds[f] : 0.f;
+      }
 #pragma unroll
       for (int i = 0; i < X::NB; ++i) acc[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  x_turn<0>(true);
+  if (AHEAD > 1 && nkt > 1) fetch(PAIR, 1);
   auto step = [&](int kt, auto BUF) {
-    constexpr int AT = decltype(BUF)::value * 2 * X::BYTES, NEXT = 2 * X::BYTES - AT;
-    if (kt + 1 < nkt) {
-      ks.request(lds + NEXT, 0, (kt + 1) * X::KT, klen);
-      vs.request(lds + NEXT + X::BYTES, 0, (kt + 1) * X::KT, klen);
-    }
+    constexpr int AT = decltype(BUF)::value * PAIR, NEXT = (decltype(BUF)::value + AHEAD) % X::STAGES * PAIR;
+    if (kt + AHEAD < nkt) fetch(NEXT, kt + AHEAD);
     auto rows32 = [&](auto UC) {
       constexpr int u = decltype(UC)::value, R = AT + u * X::HALF;
       f32x4 s[NQ][2], dp[NQ][2];
@@ -613,12 +636,13 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
     };
     rows32(std::integral_constant<int, 0>());
     if constexpr (X::U == 2) rows32(std::integral_constant<int, 1>());
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    x_turn<NEWER>(kt + AHEAD >= nkt);
   };
-  for (int kt = 0; kt < nkt; kt += 2) {
+  for (int kt = 0; kt < nkt; kt += X::STAGES) {
     step(kt, std::integral_constant<int, 0>());
     if (kt + 1 < nkt) step(kt + 1, std::integral_constant<int, 1>());
+    if constexpr (X::STAGES == 3)
+      if (kt + 2 < nkt) step(kt + 2, std::integral_constant<int, 2>());
   }
 #pragma unroll
   for (int f = 0; f < NQ; ++f) {
@@ -631,8 +655,9 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
 template <typename T, int DP, int NK, bool DROP>
 __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
-  // tiles, then per buffer KT maxima, KT reciprocal sums, KT values of D
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * X::BYTES + 2 * 3 * X::KT * 4];
+  // pairs of tiles, then for each the rows' maxima, reciprocal sums and D (64 each, and 64 that are not used)
+  constexpr int PAIR = 2 * X::BYTES, ROWS = X::STAGES * PAIR;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[ROWS + X::STAGES * 1024];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int G = p.H / p.Hkv, nkt = (p.Tk + 64 * NK - 1) / (64 * NK);
@@ -652,52 +677,43 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
     const int chunks = p.D / X::E::CE, nqt = (p.Tq + X::KT - 1) / X::KT, n = G * nqt;
     const T* qb = reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)hkv * G * p.q_sh;
     const T* gb = reinterpret_cast<const T*>(p.dout) + (long long)b * p.g_sb + (long long)hkv * G * p.g_sh;
-    const long long srow = ((long long)b * p.H + (long long)hkv * G) * p.Tq, nst = (long long)p.B * p.H * p.Tq;
-    float* st = reinterpret_cast<float*>(lds + 4 * X::BYTES);
-    auto stat = [&](int it) -> float {     // this thread's statistic of tile it
-      const int which = (int)threadIdx.x / X::KT, q = (it % nqt) * X::KT + (int)threadIdx.x % X::KT;
-      if (which >= 3) return 0.f;
-      const long long at = srow + (long long)(it / nqt) * p.Tq + min(q, p.Tq - 1);
-      if (which == 2) return p.dsum[at];
-      if (q >= p.Tq) return which == 0 ? INFINITY : 0.f;      // rows behind the last query: probability 0
-      if constexpr (sizeof(T) == 2) return which == 0 ? p.stats[at] - __log2f(p.stats[nst + at]) : 0.f;
-      return p.stats[(which == 0 ? 0 : nst) + at];
-    };
+    const long long srow = ((long long)b * p.H + (long long)hkv * G) * p.Tq;
+    const int pitch = (p.Tq + 63) / 64 * 64;
+    const long long nrow = (long long)p.B * p.H * pitch;
+    const float* rows = p.rows + min(wave, 2) * nrow + ((long long)b * p.H + (long long)hkv * G) * pitch;
     unsigned ta[4];
     f32x4 none[NK];
     if constexpr (sizeof(T) == 2) x_tr_addr<DP>(ta, lds, r, g);
     XSource<T, DP> qs, gs;
     qs.init(qb, p.q_st, chunks, wave, lane);
     gs.init(gb, p.g_st, chunks, wave, lane);
-    auto fetch = [&](unsigned char* to, int it) {
+    constexpr int AHEAD = X::STAGES - 1, NEWER = (AHEAD - 1) * (2 * XSource<T, DP>::P + 1);
+    auto fetch = [&](int buf, int it) {
       const int hq = it / nqt, row0 = (it % nqt) * X::KT;
-      qs.request(to, (long long)hq * p.q_sh * (long long)sizeof(T), row0, p.Tq);
-      gs.request(to + X::BYTES, (long long)hq * p.g_sh * (long long)sizeof(T), row0, p.Tq);
+      qs.request(lds + buf * PAIR, (long long)hq * p.q_sh * (long long)sizeof(T), row0, p.Tq);
+      gs.request(lds + buf * PAIR + X::BYTES, (long long)hq * p.g_sh * (long long)sizeof(T), row0, p.Tq);
+      // one of the three per wave (the fourth wave's copy keeps its count of requests equal)
+      __builtin_amdgcn_global_load_lds((x_glb_void*)(rows + (long long)hq * pitch + min(row0 + lane, pitch - 1)),
+                                       (x_lds_void*)(lds + ROWS + buf * 1024 + wave * 256), 4, 0, 0);
     };
-    fetch(lds, 0);
+    fetch(0, 0);
     typename X::E::chunk K[NK][X::NS], V[NK][X::NS];
     x_load_rows<T, NK>(K, reinterpret_cast<const T*>(p.k) + (long long)b * p.k_sb + (long long)hkv * p.k_sh, p.k_st, k0, klen,
                           p.D, r, g);
     x_load_rows<T, NK>(V, reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh, p.v_st, k0, klen,
                           p.D, r, g);
-    const float first = stat(0);
-    if ((int)threadIdx.x < 3 * X::KT) st[threadIdx.x] = first;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    x_turn<0>(true);
+    if (AHEAD > 1 && n > 1) fetch(1, 1);
     auto step = [&](int it, auto BUF) {
-      constexpr int B01 = decltype(BUF)::value, AT = B01 * 2 * X::BYTES, NEXT = 2 * X::BYTES - AT;
-      const float* sc = st + B01 * (3 * X::KT);
-      float next = 0.f;
-      if (it + 1 < n) {
-        next = stat(it + 1);
-        fetch(lds + NEXT, it + 1);
-      }
+      constexpr int BN = decltype(BUF)::value, AT = BN * PAIR;
+      const float* sc = reinterpret_cast<const float*>(lds + ROWS + BN * 1024);
+      if (it + AHEAD < n) fetch((BN + AHEAD) % X::STAGES, it + AHEAD);
       auto rows32 = [&](auto UC) {
         constexpr int u = decltype(UC)::value, R = AT + u * X::HALF;
         f32x4 s[NK][2], dp[NK][2];
         x_product<T, DP, NK>(s, lds + R, K, r, g, XZero());
         x_product<T, DP, NK>(dp, lds + R + X::BYTES, V, r, g, [&](int, int qf) -> f32x4 {
-          return DROP ? f32x4{0.f, 0.f, 0.f, 0.f} : -*reinterpret_cast<const f32x4*>(sc + 2 * X::KT + 32 * u + 16 * qf + 4 * g);
+          return DROP ? f32x4{0.f, 0.f, 0.f, 0.f} : -*reinterpret_cast<const f32x4*>(sc + 128 + 32 * u + 16 * qf + 4 * g);
         });
         __builtin_amdgcn_sched_barrier(0);
         XAcross<T, DP> go, qo;
@@ -711,8 +727,8 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
         for (int qf = 0; qf < 2; ++qf) {
           const int at = 32 * u + 16 * qf + 4 * g;
           const f32x4 m4 = *reinterpret_cast<const f32x4*>(sc + at);
-          const f32x4 i4 = *reinterpret_cast<const f32x4*>(sc + X::KT + at);
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(sc + 2 * X::KT + at);
+          const f32x4 i4 = *reinterpret_cast<const f32x4*>(sc + 64 + at);
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(sc + 128 + at);
 #pragma unroll
           for (int f = 0; f < NK; ++f)
 #pragma unroll
@@ -736,13 +752,13 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
       };
       rows32(std::integral_constant<int, 0>());
       if constexpr (X::U == 2) rows32(std::integral_constant<int, 1>());
-      if (it + 1 < n && (int)threadIdx.x < 3 * X::KT) st[(1 - B01) * (3 * X::KT) + threadIdx.x] = next;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
+      x_turn<NEWER>(it + AHEAD >= n);
     };
-    for (int it = 0; it < n; it += 2) {
+    for (int it = 0; it < n; it += X::STAGES) {
       step(it, std::integral_constant<int, 0>());
       if (it + 1 < n) step(it + 1, std::integral_constant<int, 1>());
+      if constexpr (X::STAGES == 3)
+        if (it + 2 < n) step(it + 2, std::integral_constant<int, 2>());
     }
   }
 #pragma unroll
@@ -825,12 +841,12 @@ int cross_attn(const nsp_cross_attn_params* a, bool bwd, void* stream) {
   if (!(a->dropout_p >= 0. && a->dropout_p < 1.)) return NSP_EINVAL;
   if (a->B == 0 || a->Tk == 0 || (a->Tq == 0 && !bwd)) return NSP_OK;     // (nothing to read, or nothing to write but empty rows: the caller's)
   if (!a->k || !a->v || (a->Tq > 0 && (!a->q || !a->out))) return NSP_EINVAL;
-  if (bwd && (a->Tq == 0 || !a->dout || !a->dq || !a->dk || !a->dv || !a->stats || !a->dsum)) return NSP_EINVAL;
+  if (bwd && (a->Tq == 0 || !a->dout || !a->dq || !a->dk || !a->dv || !a->stats || !a->rows)) return NSP_EINVAL;
   if (bwd && a->dtype == NSP_DT_BF16 && !a->o_lo) return NSP_EINVAL;
   XArgs p;
   p.q = a->q; p.k = a->k; p.v = a->v; p.dout = a->dout; p.out = a->out;
   p.o_lo = a->dtype == NSP_DT_BF16 ? a->o_lo : nullptr;
-  p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.stats = a->stats; p.dsum = a->dsum; p.klens = a->klens;
+  p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.stats = a->stats; p.rows = a->rows; p.klens = a->klens;
   p.B = (int)a->B; p.H = (int)a->H; p.Hkv = (int)a->Hkv; p.D = (int)a->D; p.Tq = (int)a->Tq; p.Tk = (int)a->Tk;
   p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;

@@ -2374,8 +2374,14 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
 
 class CrossAttnFn(torch.autograd.Function):
     """cross_attention with its backward (csrc/cross_attn.hip); arguments as checked there.  One buffer holds what backward
-    needs beside the inputs and the output: stats [2,B,H,Tq] and backward's scratch [B,H,Tq] (fp32), and for bf16 what the
-    rounding of the output left."""
+    needs beside the inputs and the output: stats [2,B,H,Tq] and backward's scratch [3,B,H,Tq rounded up to 64] (fp32), and for
+    bf16 what the rounding of the output left."""
+
+    @staticmethod
+    def layout(B, Tq, H):
+        """byte offsets of the scratch and of the output's rest"""
+        n = B * H
+        return 8 * n * Tq, (8 * n * Tq + 12 * n * ((Tq + 63) // 64 * 64) + 15) // 16 * 16
 
     @staticmethod
     def forward(ctx, q, k, v, klens, tail, seed, need):
@@ -2388,8 +2394,7 @@ class CrossAttnFn(torch.autograd.Function):
         buf, at, lo = None, 0, 0
         if need:
             half = q.dtype == torch.bfloat16
-            D = q.shape[3]
-            lo = (12 * (rows // D) + 15) // 16 * 16
+            lo = CrossAttnFn.layout(*q.shape[:3])[1]
             buf = q.new_empty(((lo + 2 * rows if half else lo) // 4,), dtype=torch.float32)
             at = buf.data_ptr()
             lo = at + lo if half else 0
@@ -2411,13 +2416,12 @@ class CrossAttnFn(torch.autograd.Function):
             dout = _vec(dout.to(q.dtype))
         g0, g1, g2, _ = dout.stride()
         dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
-        n = q.numel() // q.shape[3]
+        rows, lo = CrossAttnFn.layout(*q.shape[:3])
         at = buf.data_ptr()
         with _on(q.get_device()):
             _check(_lib.lib().nsp_cross_attn_bwd(_CROSS_PTRS(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(),
-                at + (12 * n + 15) // 16 * 16 if q.dtype == torch.bfloat16 else 0, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                at, at + 8 * n, 0 if klens is None else klens.data_ptr(), g0, g1, g2, ctx.seed, 0) + ctx.tail, _stream()),
+                at + lo if q.dtype == torch.bfloat16 else 0, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), at, at + rows, 0 if klens is None else klens.data_ptr(), g0, g1, g2, ctx.seed, 0) + ctx.tail, _stream()),
                 'nsp_cross_attn_bwd')
         return dq, dk, dv, None, None, None, None
 
