@@ -655,9 +655,10 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
 template <typename T, int DP, int NK, bool DROP>
 __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
-  // pairs of tiles, then for each the rows' maxima, reciprocal sums and D (64 each, and 64 that are not used)
-  constexpr int PAIR = 2 * X::BYTES, ROWS = X::STAGES * PAIR;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[ROWS + X::STAGES * 1024];
+  // pairs of tiles, then for each the rows' maxima, reciprocal sums and D (64 each)
+  // (two pairs: a fourth workgroup per compute unit is worth more than a third tile, 199 against 210 us)
+  constexpr int STAGES = 2, PAIR = 2 * X::BYTES, ROWS = STAGES * PAIR;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[ROWS + STAGES * 1024];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int G = p.H / p.Hkv, nkt = (p.Tk + 64 * NK - 1) / (64 * NK);
@@ -687,14 +688,13 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
     XSource<T, DP> qs, gs;
     qs.init(qb, p.q_st, chunks, wave, lane);
     gs.init(gb, p.g_st, chunks, wave, lane);
-    constexpr int AHEAD = X::STAGES - 1, NEWER = (AHEAD - 1) * (2 * XSource<T, DP>::P + 1);
     auto fetch = [&](int buf, int it) {
       const int hq = it / nqt, row0 = (it % nqt) * X::KT;
       qs.request(lds + buf * PAIR, (long long)hq * p.q_sh * (long long)sizeof(T), row0, p.Tq);
       gs.request(lds + buf * PAIR + X::BYTES, (long long)hq * p.g_sh * (long long)sizeof(T), row0, p.Tq);
-      // one of the three per wave (the fourth wave's copy keeps its count of requests equal)
-      __builtin_amdgcn_global_load_lds((x_glb_void*)(rows + (long long)hq * pitch + min(row0 + lane, pitch - 1)),
-                                       (x_lds_void*)(lds + ROWS + buf * 1024 + wave * 256), 4, 0, 0);
+      if (wave < 3)      // one of the three per wave
+        __builtin_amdgcn_global_load_lds((x_glb_void*)(rows + (long long)hq * pitch + min(row0 + lane, pitch - 1)),
+                                         (x_lds_void*)(lds + ROWS + buf * 1024 + wave * 256), 4, 0, 0);
     };
     fetch(0, 0);
     typename X::E::chunk K[NK][X::NS], V[NK][X::NS];
@@ -703,11 +703,10 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
     x_load_rows<T, NK>(V, reinterpret_cast<const T*>(p.v) + (long long)b * p.v_sb + (long long)hkv * p.v_sh, p.v_st, k0, klen,
                           p.D, r, g);
     x_turn<0>(true);
-    if (AHEAD > 1 && n > 1) fetch(1, 1);
     auto step = [&](int it, auto BUF) {
       constexpr int BN = decltype(BUF)::value, AT = BN * PAIR;
       const float* sc = reinterpret_cast<const float*>(lds + ROWS + BN * 1024);
-      if (it + AHEAD < n) fetch((BN + AHEAD) % X::STAGES, it + AHEAD);
+      if (it + 1 < n) fetch(1 - BN, it + 1);      // (that buffer was last read in step it - 1, behind that step's barrier)
       auto rows32 = [&](auto UC) {
         constexpr int u = decltype(UC)::value, R = AT + u * X::HALF;
         f32x4 s[NK][2], dp[NK][2];
@@ -752,13 +751,11 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
       };
       rows32(std::integral_constant<int, 0>());
       if constexpr (X::U == 2) rows32(std::integral_constant<int, 1>());
-      x_turn<NEWER>(it + AHEAD >= n);
+      x_turn<0>(true);
     };
-    for (int it = 0; it < n; it += X::STAGES) {
+    for (int it = 0; it < n; it += 2) {
       step(it, std::integral_constant<int, 0>());
       if (it + 1 < n) step(it + 1, std::integral_constant<int, 1>());
-      if constexpr (X::STAGES == 3)
-        if (it + 2 < n) step(it + 2, std::integral_constant<int, 2>());
     }
   }
 #pragma unroll
@@ -805,25 +802,18 @@ int launch_dkv(const XArgs& p, hipStream_t st) {
   return NSP_OK;
 }
 
-// Two owned 16-row fragments per wave halve the LDS reads per score, which bound the bf16 kernels with one; they pay once the
-// halved number of workgroups still fills the 256 compute units.  fp32 spends eight times as long in the matrix cores and keeps
-// one.
+// Two owned 16-row fragments per wave halve the tile reads per score.  They pay once the halved number of workgroups still fills
+// the 256 compute units twice (bf16, 128 x 8 heads, 256 x 600..800, d 64: forward 124 -> 104 us, dQ 133 -> 117; 4 x 16 heads, 500 x
+// 2048, d 128, 256 workgroups left: forward 52 -> 61, dQ 63 -> 68).  fp32 spends eight times as long in the matrix cores and keeps
+// one; so does dK / dV, whose two accumulators leave too few registers for a third workgroup (205 us either way, and 9.0 against
+// 10.9 us for 32 x 8 heads, 61 x 90..187).
 template <typename T, int DP, bool DROP>
 int launch(const XArgs& p, bool bwd, hipStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    const bool two_q = p.Tq > 64 && (long long)p.B * p.H * ((p.Tq + 127) / 128) >= 512;
-    const bool two_k = DP <= 64 && p.Tk > 64 && (long long)p.B * p.Hkv * ((p.Tk + 127) / 128) >= 512;
-    if (!bwd) return two_q ? launch_fwd<T, DP, 2, DROP>(p, st) : launch_fwd<T, DP, 1, DROP>(p, st);
-    const int rc = two_q ? launch_dq<T, DP, 2, DROP>(p, st) : launch_dq<T, DP, 1, DROP>(p, st);
-    if (rc != NSP_OK) return rc;
-    if constexpr (DP <= 64)
-      if (two_k) return launch_dkv<T, DP, 2, DROP>(p, st);
-    return launch_dkv<T, DP, 1, DROP>(p, st);
-  } else {
-    if (!bwd) return launch_fwd<T, DP, 1, DROP>(p, st);
-    const int rc = launch_dq<T, DP, 1, DROP>(p, st);
-    return rc != NSP_OK ? rc : launch_dkv<T, DP, 1, DROP>(p, st);
-  }
+  constexpr int TWO = sizeof(T) == 2 ? 2 : 1;
+  const bool two = TWO == 2 && p.Tq > 64 && (long long)p.B * p.H * ((p.Tq + 127) / 128) >= 512;
+  if (!bwd) return two ? launch_fwd<T, DP, TWO, DROP>(p, st) : launch_fwd<T, DP, 1, DROP>(p, st);
+  const int rc = two ? launch_dq<T, DP, TWO, DROP>(p, st) : launch_dq<T, DP, 1, DROP>(p, st);
+  return rc != NSP_OK ? rc : launch_dkv<T, DP, 1, DROP>(p, st);
 }
 template <typename T, bool DROP>
 int launch_d(const XArgs& p, bool bwd, hipStream_t st) {

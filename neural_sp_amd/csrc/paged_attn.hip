@@ -260,10 +260,10 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
                           (MODE == CONTIG || ((cur.ok >> (MODE == BLOCK16 ? kf : 4 * kf + e)) & 1u));
         const float x = uniform ? 0.f : s[e] * p.sl2;
         pr[kf][e] = seen ? x : -INFINITY;
-        mx = fmaxf(mx, pr[kf][e]);
+        mx = attn_max(mx, pr[kf][e]);
       }
     }
-    const float mn = fmaxf(m, attn_max4(mx));
+    const float mn = attn_max(m, attn_max4(mx));
     const float base = mn == -INFINITY ? 0.f : mn;     // (nothing seen so far: every exponent below is -inf)
     const float alpha = __builtin_amdgcn_exp2f(m - base);
     m = mn;
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
   if (q >= nrow) return;
   float M = has_new ? new_s[q] : -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, part_m[w][q]);
+  for (int w = 0; w < 4; ++w) M = attn_max(M, part_m[w][q]);
   const float base = M == -INFINITY ? 0.f : M;
   float L = 0.f, acc[VW];
 #pragma unroll
@@ -355,10 +355,15 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
   }
 }
 
-// one workgroup per query row: the parts of its splits (maximum, sum, unnormalised output) into one
+// one wave per query row: the parts of its splits (maximum, sum, unnormalised output) into one.  Lane s holds the weight of split
+// s (64 at a time), so that the parts' loads depend on nothing but their address.
 template <typename T, int DP, bool PAGED>
-__global__ __launch_bounds__(DP) void decode_join_kernel(const DecodeArgs p) {
-  const int rr = blockIdx.x, hkv = blockIdx.y, b = blockIdx.z, G = p.H / p.Hkv, d = threadIdx.x;
+__global__ __launch_bounds__(256) void decode_join_kernel(const DecodeArgs p) {
+  constexpr int VW = DP < 64 ? 1 : DP / 64;
+  const int lane = threadIdx.x & 63, G = p.H / p.Hkv;
+  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (long long)p.B * p.Hkv * p.rows) return;
+  const int rr = (int)(id % p.rows), hkv = (int)(id / p.rows % p.Hkv), b = (int)(id / ((long long)p.rows * p.Hkv));
   int len = p.lens ? p.lens[b] : p.cap;
   len = max(0, min(len, p.cap));
   if (!PAGED && len == 0) len = p.cap;
@@ -366,18 +371,35 @@ __global__ __launch_bounds__(DP) void decode_join_kernel(const DecodeArgs p) {
   const float* w = p.ws + ((((long long)b * p.Hkv + hkv) * p.nsplit) * p.rows + rr) * (DP + 2);
   const long long step = (long long)p.rows * (DP + 2);
   float M = -INFINITY;
-  for (int s = 0; s < ns; ++s) M = fmaxf(M, w[s * step + DP]);
+  for (int s = lane; s < ns; s += 64) M = attn_max(M, w[s * step + DP]);
+  for (int o = 32; o > 0; o >>= 1) M = attn_max(M, __shfl_xor(M, o, 64));
   const float base = M == -INFINITY ? 0.f : M;
-  float L = 0.f, acc = 0.f;
-  for (int s = 0; s < ns; ++s) {
-    const float f = __builtin_amdgcn_exp2f(w[s * step + DP] - base);
-    L = fmaf(f, w[s * step + DP + 1], L);
-    acc = fmaf(f, w[s * step + d], acc);
+  float L = 0.f, acc[VW];
+#pragma unroll
+  for (int j = 0; j < VW; ++j) acc[j] = 0.f;
+  const int d = lane * VW;
+  for (int s0 = 0; s0 < ns; s0 += 64) {
+    float f = 0.f;
+    if (s0 + lane < ns) {
+      f = __builtin_amdgcn_exp2f(w[(s0 + lane) * step + DP] - base);
+      L = fmaf(f, w[(s0 + lane) * step + DP + 1], L);
+    }
+    const int n = min(64, ns - s0);
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float fs = __shfl(f, s, 64);
+      if (d < DP) {
+#pragma unroll
+        for (int j = 0; j < VW; ++j) acc[j] = fmaf(fs, w[(s0 + s) * step + d + j], acc[j]);
+      }
+    }
   }
+  L = wave_reduce_sum(L);
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-  if (d < p.D)
-    reinterpret_cast<T*>(p.out)[(((long long)b * p.Tq + rr / G) * p.H + hkv * G + rr % G) * p.D + d] =
-        AttnElem<T>::from_f32(acc * inv);
+  T* out = reinterpret_cast<T*>(p.out) + (((long long)b * p.Tq + rr / G) * p.H + hkv * G + rr % G) * p.D;
+#pragma unroll
+  for (int j = 0; j < VW; ++j)
+    if (d + j < p.D) out[d + j] = AttnElem<T>::from_f32(acc[j] * inv);
 }
 
 template <typename T, int DP>
@@ -388,9 +410,9 @@ int launch_decode(const DecodeArgs& p, hipStream_t st) {
   else hipLaunchKernelGGL((decode_attn_kernel<T, DP, ROWS>), grid, dim3(256), 0, st, p);
   NSP_LAUNCH_CHECK();
   if (p.nsplit > 1) {
-    const dim3 jg((unsigned)p.rows, (unsigned)p.Hkv, (unsigned)p.B);
-    if (p.table) hipLaunchKernelGGL((decode_join_kernel<T, DP, true>), jg, dim3(DP), 0, st, p);
-    else hipLaunchKernelGGL((decode_join_kernel<T, DP, false>), jg, dim3(DP), 0, st, p);
+    const dim3 jg((unsigned)(((long long)p.B * p.Hkv * p.rows + 3) / 4));
+    if (p.table) hipLaunchKernelGGL((decode_join_kernel<T, DP, true>), jg, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((decode_join_kernel<T, DP, false>), jg, dim3(256), 0, st, p);
     NSP_LAUNCH_CHECK();
   }
   return NSP_OK;
