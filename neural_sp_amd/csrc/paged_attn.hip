@@ -132,9 +132,29 @@ struct Tile {
   unsigned ok;   // BLOCK16: bit kf; ROWS: bit 4 kf + e of the lane's eight keys
 };
 
+// BLOCK16: pages and slots of a tile's two 16-key blocks.  Looked up ahead of the keys, and without regard to the sequence's
+// length, so that the first tile's lookup runs beside the load of that length and the others' behind the tile before.
+struct TilePages {
+  int id[2], slot[2];
+};
+template <int MODE>
+__device__ __forceinline__ TilePages load_pages(const DecodeArgs& p, const int* tab, int j0) {
+  TilePages t;
+  if constexpr (MODE == BLOCK16) {
+#pragma unroll
+    for (int kf = 0; kf < 2; ++kf) {
+      unsigned pg, slot;
+      page_split(p, (unsigned)min(j0 + 16 * kf, p.cap - 16), pg, slot);       // (cap: a multiple of the page)
+      t.id[kf] = tab[pg];
+      t.slot[kf] = (int)slot;
+    }
+  }
+  return t;
+}
+
 template <typename T, int DP, int MODE>
 __device__ __forceinline__ void load_tile(Tile<T, DP>& t, const DecodeArgs& p, const T* kb, const T* vb, const int* tab,
-                                          int j0, int end, int r, int g, bool full_d) {
+                                          const TilePages& pages, int j0, int end, int r, int g, bool full_d) {
   typedef AttnElem<T> E;
   constexpr int NS = Tile<T, DP>::NS, VW = Tile<T, DP>::VW;
   t.ok = 0u;
@@ -150,17 +170,13 @@ __device__ __forceinline__ void load_tile(Tile<T, DP>& t, const DecodeArgs& p, c
 #pragma unroll
       for (int e = 0; e < 4; ++e) vrow[e] = vb + (long long)min(jb + 4 * g + e, end - 1) * p.v_ss;
     } else if constexpr (MODE == BLOCK16) {
-      const bool in = jb < end;
-      unsigned pg, slot;
-      page_split(p, (unsigned)(in ? jb : j0), pg, slot);
-      const int id = tab[pg];
-      kok = in && id >= 0 && id < p.n_pages;
-      const long long at = kok ? id : 0;
-      const int top = kok ? min(15, end - 1 - jb) : 0;
-      krow = kb + at * p.k_sp + (long long)((int)slot + min(r, top)) * p.k_ss;
+      kok = jb < end && pages.id[kf] >= 0 && pages.id[kf] < p.n_pages;
+      const long long at = kok ? pages.id[kf] : 0;
+      const int slot = kok ? pages.slot[kf] : 0, top = kok ? min(15, end - 1 - jb) : 0;
+      krow = kb + at * p.k_sp + (long long)(slot + min(r, top)) * p.k_ss;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        vrow[e] = vb + at * p.v_sp + (long long)((int)slot + min(4 * g + e, top)) * p.v_ss;
+        vrow[e] = vb + at * p.v_sp + (long long)(slot + min(4 * g + e, top)) * p.v_ss;
         vok[e] = kok;
       }
       t.ok |= kok ? (1u << kf) : 0u;
@@ -205,23 +221,24 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
   const int split = blockIdx.x, b = blockIdx.z;
   const int hkv = (int)blockIdx.y / p.ngrp, grp = (int)blockIdx.y % p.ngrp;
   const int G = p.H / p.Hkv, row0 = grp * 16, nrow = min(16, p.rows - row0);
+  const int* tab = MODE == CONTIG ? nullptr : p.table + (long long)b * p.width;
+  const int start = split * p.chunk;
+  int j0 = start + 32 * wave;
+  TilePages pages = load_pages<MODE>(p, tab, j0);
   int len = p.lens ? p.lens[b] : p.cap;
   const bool unused = MODE != CONTIG && len < 0;
   len = max(0, min(len, p.cap));
   // an utterance without a visible key: the finite mask value of the training path makes its softmax uniform over ALL keys
   const bool uniform = MODE == CONTIG && len == 0;
   if (uniform) len = p.cap;
-  const int start = split * p.chunk, end = min(len, start + p.chunk);
+  const int end = min(len, start + p.chunk);
   if (split > 0 && start >= len) return;
   const bool full_d = p.D == DP;
   const T* kb = reinterpret_cast<const T*>(p.k) + (long long)hkv * p.k_sh;
   const T* vb = reinterpret_cast<const T*>(p.v) + (long long)hkv * p.v_sh;
-  const int* tab = nullptr;
   if constexpr (MODE == CONTIG) {
     kb += (long long)b * p.k_sp;
     vb += (long long)b * p.v_sp;
-  } else {
-    tab = p.table + (long long)b * p.width;
   }
   const T* qb = reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb;
 
@@ -242,11 +259,16 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
   float m = -INFINITY, l = 0.f;
 
   Tile<T, DP> cur, nxt;
-  int j0 = start + 32 * wave;
-  if (j0 < end) load_tile<T, DP, MODE>(cur, p, kb, vb, tab, j0, end, r, g, full_d);
+  if (j0 < end) {
+    load_tile<T, DP, MODE>(cur, p, kb, vb, tab, pages, j0, end, r, g, full_d);
+    pages = load_pages<MODE>(p, tab, j0 + 128);
+  }
   while (j0 < end) {
     const int jn = j0 + 128;
-    if (jn < end) load_tile<T, DP, MODE>(nxt, p, kb, vb, tab, jn, end, r, g, full_d);
+    if (jn < end) {
+      load_tile<T, DP, MODE>(nxt, p, kb, vb, tab, pages, jn, end, r, g, full_d);
+      pages = load_pages<MODE>(p, tab, jn + 128);
+    }
     float pr[2][4];
     float mx = -INFINITY;
 #pragma unroll
@@ -355,51 +377,63 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
   }
 }
 
-// one wave per query row: the parts of its splits (maximum, sum, unnormalised output) into one.  Lane s holds the weight of split
-// s (64 at a time), so that the parts' loads depend on nothing but their address.
+// One wave per query row: the parts of its splits (maximum, sum, unnormalised output) into one, eight at a time.  What a part's
+// loads need is its number alone -- neither the sequence's length nor another part's maximum -- so that the launch costs one
+// round trip to memory; parts that no workgroup wrote are dropped after the load.
 template <typename T, int DP, bool PAGED>
 __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeArgs p) {
-  constexpr int VW = DP < 64 ? 1 : DP / 64;
+  constexpr int VW = DP < 64 ? 1 : DP / 64, N = 8;
   const int lane = threadIdx.x & 63, G = p.H / p.Hkv;
-  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long id = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   if (id >= (long long)p.B * p.Hkv * p.rows) return;
   const int rr = (int)(id % p.rows), hkv = (int)(id / p.rows % p.Hkv), b = (int)(id / ((long long)p.rows * p.Hkv));
-  int len = p.lens ? p.lens[b] : p.cap;
-  len = max(0, min(len, p.cap));
-  if (!PAGED && len == 0) len = p.cap;
-  const int ns = max(1, (len + p.chunk - 1) / p.chunk);
   const float* w = p.ws + ((((long long)b * p.Hkv + hkv) * p.nsplit) * p.rows + rr) * (DP + 2);
   const long long step = (long long)p.rows * (DP + 2);
-  float M = -INFINITY;
-  for (int s = lane; s < ns; s += 64) M = attn_max(M, w[s * step + DP]);
-  for (int o = 32; o > 0; o >>= 1) M = attn_max(M, __shfl_xor(M, o, 64));
-  const float base = M == -INFINITY ? 0.f : M;
-  float L = 0.f, acc[VW];
+  const int d = min(lane * VW, DP - VW);
+  int len = p.lens ? p.lens[b] : p.cap;
+  float M = -INFINITY, L = 0.f, acc[VW];
 #pragma unroll
   for (int j = 0; j < VW; ++j) acc[j] = 0.f;
-  const int d = lane * VW;
-  for (int s0 = 0; s0 < ns; s0 += 64) {
-    float f = 0.f;
-    if (s0 + lane < ns) {
-      f = __builtin_amdgcn_exp2f(w[(s0 + lane) * step + DP] - base);
-      L = fmaf(f, w[(s0 + lane) * step + DP + 1], L);
-    }
-    const int n = min(64, ns - s0);
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float fs = __shfl(f, s, 64);
-      if (d < DP) {
+  for (int s0 = 0; s0 < p.nsplit; s0 += N) {
+    float m[N], l[N], o[N][VW];
 #pragma unroll
-        for (int j = 0; j < VW; ++j) acc[j] = fmaf(fs, w[(s0 + s) * step + d + j], acc[j]);
-      }
+    for (int s = 0; s < N; ++s) {
+      const float* part = w + min(s0 + s, p.nsplit - 1) * step;
+      m[s] = part[DP];
+      l[s] = part[DP + 1];
+#pragma unroll
+      for (int j = 0; j < VW; ++j) o[s][j] = part[d + j];
     }
+    if (s0 == 0) {
+      len = max(0, min(len, p.cap));
+      if (!PAGED && len == 0) len = p.cap;
+    }
+    const int ns = max(1, (len + p.chunk - 1) / p.chunk);
+    float mx = M;
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      if (s0 + s >= ns) { m[s] = -INFINITY; l[s] = 0.f; }
+      mx = attn_max(mx, m[s]);
+    }
+    const float base = mx == -INFINITY ? 0.f : mx, old = __builtin_amdgcn_exp2f(M - base);
+    M = mx;
+    L *= old;
+#pragma unroll
+    for (int j = 0; j < VW; ++j) acc[j] *= old;
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      const float f = __builtin_amdgcn_exp2f(m[s] - base);
+      L = fmaf(f, l[s], L);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) acc[j] = s0 + s < ns ? fmaf(f, o[s][j], acc[j]) : acc[j];
+    }
+    if (s0 + N >= ns) break;
   }
-  L = wave_reduce_sum(L);
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
   T* out = reinterpret_cast<T*>(p.out) + (((long long)b * p.Tq + rr / G) * p.H + hkv * G + rr % G) * p.D;
 #pragma unroll
   for (int j = 0; j < VW; ++j)
-    if (d + j < p.D) out[d + j] = AttnElem<T>::from_f32(acc[j] * inv);
+    if (lane * VW + j < p.D) out[lane * VW + j] = AttnElem<T>::from_f32(acc[j] * inv);
 }
 
 template <typename T, int DP>
@@ -459,13 +493,16 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const S* __restrict__
 }
 
 // keys per workgroup and the number of workgroups a row of keys is split over
-void decode_plan(long long groups, long long cap, int* nsplit, int* chunk) {
-  // Enough workgroups to fill 256 CUs four times over, but no stretch below 256 keys: a workgroup's four waves then work
-  // through two tiles each, and below that the join costs more than the parallelism brings.
-  long long want = (1024 + groups - 1) / groups;
+void decode_plan(long long groups, long long cap, int DP, int* nsplit, int* chunk) {
+  // The chip holds 512 workgroups (d > 64) or 1024 at a time; four times as many even out sequences of unequal length, which
+  // reach only part of the capacity that the call knows.  16 x 8 key heads, d 128, 9000..32000 of 32064 keys: 8 / 16 / 32 stretches
+  // 282 / 274 / 294 us; 64 x 8, d 64, 700..1500 of 1500: 2 / 4 / 6 stretches 31.4 / 31.2 / 26.9 us.  No stretch is below 256 keys: a
+  // workgroup's four waves then work through two tiles each; and up to 512 keys stay one: the second launch (3 us, and 4 us of the
+  // host's time) costs more than it brings.
+  long long want = ((DP == 128 ? 2048 : 4096) + groups - 1) / groups;
   const long long most = (cap + 255) / 256;
   if (want > most) want = most;
-  if (want < 1) want = 1;
+  if (want < 1 || cap <= 512) want = 1;
   long long c = (cap + want - 1) / want;
   c = (c + 127) / 128 * 128;
   if (c < 128) c = 128;
@@ -473,6 +510,7 @@ void decode_plan(long long groups, long long cap, int* nsplit, int* chunk) {
   *nsplit = (int)((cap + c - 1) / c);
   if (*nsplit < 1) *nsplit = 1;
 }
+int padded_head(long long D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 }  // namespace
 
@@ -480,8 +518,8 @@ extern "C" long long nsp_decode_attn_workspace_bytes(int B, int H, int Hkv, int 
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || Tq <= 0 || D <= 0 || D > 128 || cap < 0) return 0;
   const long long rows = (long long)(H / Hkv) * Tq;
   int nsplit, chunk;
-  decode_plan((long long)B * Hkv * ((rows + 15) / 16), cap, &nsplit, &chunk);
-  const int DP = D <= 32 ? 32 : D <= 64 ? 64 : 128;
+  const int DP = padded_head(D);
+  decode_plan((long long)B * Hkv * ((rows + 15) / 16), cap, DP, &nsplit, &chunk);
   return nsplit == 1 ? 0 : (long long)B * Hkv * nsplit * rows * (DP + 2) * 4;
 }
 
@@ -509,7 +547,7 @@ extern "C" int nsp_decode_attn(const nsp_decode_attn_params* a, void* stream) {
   p.v_sp = a->v_sp; p.v_ss = a->v_ss; p.v_sh = a->v_sh;
   p.kn_sb = a->kn_sb; p.kn_sh = a->kn_sh; p.vn_sb = a->vn_sb; p.vn_sh = a->vn_sh;
   p.sl2 = (float)(a->scale * 1.4426950408889634);
-  decode_plan(a->B * a->Hkv * ngrp, cap, &p.nsplit, &p.chunk);
+  decode_plan(a->B * a->Hkv * ngrp, cap, padded_head(a->D), &p.nsplit, &p.chunk);
   if (p.nsplit > 1 && !p.ws) return NSP_EINVAL;
   return a->dtype == NSP_DT_BF16 ? launch_decode_d<__bf16>(p, (hipStream_t)stream) : launch_decode_d<float>(p, (hipStream_t)stream);
 }
