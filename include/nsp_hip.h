@@ -824,14 +824,14 @@ int nsp_sample_rows(const nsp_sample_params* p, void* stream);
 
 /* nsp_cross_attn_fwd / _bwd: out[b,i,h,:] = sum_j dropout(p_ij) v_j, p = softmax_j(scale q[b,i,h] . k[b,j,h / (H / Hkv)]) over
  *   j < klens[b] (klens NULL: all Tk; klens[b] <= 0: all Tk keys alike and no gradient through the scores).  q [B,Tq,H,D],
- *   k / v [B,Tk,Hkv,D] and dout (strides g_*) as above; out, o_lo, dq [B,Tq,H,D] and dk, dv [B,Tk,Hkv,D] contiguous, all of type
- *   dtype.  Training: fwd also fills stats [2][B,H,Tq] fp32 and, for bf16, o_lo (what the rounding of out left; both NULL for
- *   inference); bwd reads out, o_lo, stats, uses rows [3][B,H,Tq rounded up to 64] fp32 as scratch and writes dq, dk, dv completely.
+ *   k / v [B,Tk,Hkv,D] and dout (strides g_*) as above; out, dq [B,Tq,H,D] and dk, dv [B,Tk,Hkv,D] contiguous, all of type
+ *   dtype.  Training: fwd also fills stats [2][B,H,Tq] fp32 (NULL for inference); bwd reads out
+ *   and stats, uses rows [3][B,H,Tq rounded up to 64] fp32 as scratch and writes dq, dk, dv completely.
  *   dropout: element (b,h,i,j) is kept as nsp_attn_softmax_fwd keeps it: counter offset + ((b H + h) Tq + i) Tk + j.
  *   scale > 0.  Tq == 0 or Tk == 0: nothing is written. */
 typedef struct {
   const void* q; const void* k; const void* v; const void* dout;
-  void* out; void* o_lo; void* dq; void* dk; void* dv;
+  void* out; void* dq; void* dk; void* dv;
   float* stats; float* rows; const int* klens;
   long long g_sb, g_st, g_sh;
   unsigned long long seed, offset;

@@ -16,8 +16,9 @@
 // it with the transposing LDS read (ds_read_b64_tr_b16), fp32 holds one contraction element per lane and instruction and
 // just picks the row.
 // The softmax is kept as its maximum (log2 domain) and the reciprocal of its sum, both fp32; backward recomputes P from them.
-// bf16 roundings inside: P resp. dS, once each, as operands of the second products (their error, 2^-9 rms 2^-10, is that of the
-// output's own rounding); O is kept for D as two bf16 parts (16 bits) because D is subtracted from dP.
+// bf16 roundings inside: P resp. dS, once each, as operands of the second products; with the outputs' own rounding the results are
+// 1.2 (out) to 1.5 times (dQ) as far from exact as a rounding of the exact result.  (Two bf16 parts for dS bring dQ to 1.2 and cost
+// 36 us of the 417 us of the largest measured call.)  Sums, statistics and D are fp32.
 // A row without a visible key is uniform over all Tk keys, as with the finite mask value of attn_softmax_fwd, and passes no
 // gradient through its scores.  Keys behind klens are never read.
 #include "attn_frag.h"
@@ -27,7 +28,7 @@ namespace {
 
 struct XArgs {
   const void *q, *k, *v, *dout;
-  void *out, *o_lo, *dq, *dk, *dv;
+  void *out, *dq, *dk, *dv;
   float* stats;        // [2][B,H,Tq]: maximum, 1 / sum
   float* rows;         // [3][B,H,Tq rounded up to 64]: what dK / dV need of every query, from the dQ kernel
   const int* klens;
@@ -260,8 +261,8 @@ struct XAcross<__bf16, DP> {
       b.template read<OB>(lds, ta);
     }
   }
-  // SUM: sum[f] (every element) += the column's weights as rounded, by a product with ones -- the matrix cores have room for
-  // it, the vector units, which bound the forward kernel, do not
+  // SUM: sum[f] (every element) += the column's weights as they enter, by a product with ones -- the matrix cores have more room
+  // for it than the vector units
   template <int OFF, bool SUM, int N>
   __device__ __forceinline__ void product(f32x4 (&acc)[N][X::NB], f32x4 (&sum)[N], const f32x4 (&w)[N][2], const unsigned char*, int,
                                           int) const {
@@ -284,8 +285,8 @@ struct XAcross<__bf16, DP> {
   }
 };
 
-// row `dst` (D elements) <- a transposed accumulator's column, times f; LO: what the rounding to T left, as T
-template <int DP, bool LO>
+// row `dst` (D elements) <- a transposed accumulator's column, times f
+template <int DP>
 __device__ __forceinline__ void x_store(float* dst, const f32x4 (&acc)[DP / 16], float f, int D, int g) {
   constexpr int VW = DP / 16;
 #pragma unroll
@@ -301,7 +302,7 @@ __device__ __forceinline__ void x_store(float* dst, const f32x4 (&acc)[DP / 16],
     }
   }
 }
-template <int DP, bool LO>
+template <int DP>
 __device__ __forceinline__ void x_store(__bf16* dst, const f32x4 (&acc)[DP / 16], float f, int D, int g) {
 #pragma unroll
   for (int blk = 0; blk < DP / 16; ++blk) {
@@ -310,9 +311,7 @@ __device__ __forceinline__ void x_store(__bf16* dst, const f32x4 (&acc)[DP / 16]
     bf16x4 x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float v = acc[blk][e] * f;
-      x[e] = (__bf16)v;
-      if (LO) x[e] = (__bf16)(v - (float)x[e]);
+      x[e] = (__bf16)(acc[blk][e] * f);
     }
     *reinterpret_cast<bf16x4*>(dst + d) = x;
   }
@@ -508,8 +507,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
     const int qi = q0 + 16 * f + r;
     if (qi >= p.Tq) continue;
     const long long at = (((long long)b * p.Tq + qi) * p.H + h) * p.D;
-    x_store<DP, false>(reinterpret_cast<T*>(p.out) + at, o[f], inv, p.D, g);
-    if (p.o_lo) x_store<DP, true>(reinterpret_cast<T*>(p.o_lo) + at, o[f], inv, p.D, g);
+    x_store<DP>(reinterpret_cast<T*>(p.out) + at, o[f], inv, p.D, g);
     if (p.stats && g == 0) {
       const long long sr = ((long long)b * p.H + h) * p.Tq + qi;
       p.stats[sr] = m[f];
@@ -536,7 +534,11 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
   const long long srow = ((long long)b * p.H + h) * p.Tq;
   const int nkt = klen <= 0 ? 0 : (klen + X::KT - 1) / X::KT;     // no visible key: no gradient
   unsigned ta[4];
-  f32x4 none[NQ];
+  // bf16: O was rounded, and so were the probabilities in it, so D is a little off.  The probabilities sum to 1, hence D is what is used
+  // for it here plus the sum of dS, and what that changes is that sum times sum_j p_j k_j: both are kept and settled at the end.
+  constexpr bool MEND = sizeof(T) == 2;
+  float off[NQ];
+  f32x4 pk[MEND ? NQ : 1][X::NB], none[NQ];
   if constexpr (sizeof(T) == 2) x_tr_addr<DP>(ta, lds, r, g);
   XSource<T, DP> ks, vs;
   ks.init(kb, p.k_st, chunks, wave, lane);
@@ -565,25 +567,15 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
       for (int s = 0; s < X::NS; ++s)
 #pragma unroll
         for (int e = 0; e < X::E::CE; ++e) d = fmaf((float)dO[f][s][e], (float)O[0][s][e], d);
-      if (p.o_lo) {
-        x_load_rows<T, 1>(O, reinterpret_cast<const T*>(p.o_lo) + orow, (long long)p.H * p.D, q0 + 16 * f, p.Tq, p.D, r, g);
-#pragma unroll
-        for (int s = 0; s < X::NS; ++s)
-#pragma unroll
-          for (int e = 0; e < X::E::CE; ++e) d = fmaf((float)dO[f][s][e], (float)O[0][s][e], d);
-      }
       ds[f] = attn_sum4(d);
       const int qi = min(q0 + 16 * f + r, p.Tq - 1);
       m[f] = p.stats[srow + qi];
       inv[f] = p.stats[(long long)p.B * p.H * p.Tq + srow + qi];
       if constexpr (sizeof(T) == 2) m[f] -= __log2f(inv[f]);      // (one rounding of the exponent more, far below bf16's)
-      // for the dK / dV kernel, which reads 64 at a time: rows behind the last query have probability 0
-      const int pitch = (p.Tq + 63) / 64 * 64, q = q0 + 16 * f + r;
-      if (g == 0 && q < pitch) {
-        const long long at = ((long long)b * p.H + h) * pitch + q, n = (long long)p.B * p.H * pitch;
-        p.rows[at] = q < p.Tq ? m[f] : INFINITY;
-        p.rows[n + at] = q < p.Tq ? inv[f] : 0.f;
-        p.rows[2 * n + at] = q < p.Tq ? ds[f] : 0.f;
+      off[f] = 0.f;
+      if constexpr (MEND) {
+#pragma unroll
+        for (int i = 0; i < X::NB; ++i) pk[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
       for (int i = 0; i < X::NB; ++i) acc[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -618,8 +610,9 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float x = __builtin_amdgcn_exp2f(fmaf(s[f][kf][e], p.sl2, -m[f]));
-            if constexpr (sizeof(T) == 4) x *= inv[f];
-            s[f][kf][e] = x * (DROP ? fmaf(dp[f][kf][e], keep[e], -ds[f]) : dp[f][kf][e]);
+            if constexpr (!MEND) x *= inv[f];
+            s[f][kf][e] = x;
+            if constexpr (DROP) dp[f][kf][e] = fmaf(dp[f][kf][e], keep[e], -ds[f]);
           }
         }
       }
@@ -632,7 +625,15 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
             for (int e = 0; e < 4; ++e)
               if (kt * X::KT + 32 * u + 16 * kf + 4 * g + e >= klen) s[f][kf][e] = 0.f;
       }
-      k.template product<R, false, NQ>(acc, none, s, lds, r, g);
+#pragma unroll
+      for (int f = 0; f < NQ; ++f)
+#pragma unroll
+        for (int kf = 0; kf < 2; ++kf) {
+          dp[f][kf] *= s[f][kf];
+          if constexpr (MEND) off[f] += (dp[f][kf][0] + dp[f][kf][1]) + (dp[f][kf][2] + dp[f][kf][3]);
+        }
+      k.template product<R, false, NQ>(acc, none, dp, lds, r, g);
+      if constexpr (MEND) k.template product<R, false, NQ>(pk, none, s, lds, r, g);
     };
     rows32(std::integral_constant<int, 0>());
     if constexpr (X::U == 2) rows32(std::integral_constant<int, 1>());
@@ -644,11 +645,24 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
     if constexpr (X::STAGES == 3)
       if (kt + 2 < nkt) step(kt + 2, std::integral_constant<int, 2>());
   }
+  // D and the statistics for the dK / dV kernel, which reads 64 at a time: rows behind the last query have probability 0
+  const int pitch = (p.Tq + 63) / 64 * 64;
 #pragma unroll
   for (int f = 0; f < NQ; ++f) {
-    const int qi = q0 + 16 * f + r;
-    if (qi < p.Tq)
-      x_store<DP, false>(reinterpret_cast<T*>(p.dq) + (((long long)b * p.Tq + qi) * p.H + h) * p.D, acc[f], p.scale, p.D, g);
+    if constexpr (MEND) {
+      off[f] = attn_sum4(off[f]);
+#pragma unroll
+      for (int i = 0; i < X::NB; ++i) acc[f][i] -= off[f] * pk[f][i];
+    }
+    const int q = q0 + 16 * f + r;
+    if (g == 0 && q < pitch) {
+      const long long at = ((long long)b * p.H + h) * pitch + q, n = (long long)p.B * p.H * pitch;
+      p.rows[at] = q < p.Tq ? m[f] : INFINITY;
+      p.rows[n + at] = q < p.Tq ? inv[f] : 0.f;
+      p.rows[2 * n + at] = q < p.Tq ? ds[f] + off[f] : 0.f;
+    }
+    if (q < p.Tq)
+      x_store<DP>(reinterpret_cast<T*>(p.dq) + (((long long)b * p.Tq + q) * p.H + h) * p.D, acc[f], p.scale, p.D, g);
   }
 }
 
@@ -771,8 +785,8 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
 #pragma unroll
       for (int i = 0; i < X::NB; ++i) dk[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    x_store<DP, false>(reinterpret_cast<T*>(p.dk) + at, dk[f], p.scale, p.D, g);
-    x_store<DP, false>(reinterpret_cast<T*>(p.dv) + at, dv[f], 1.f, p.D, g);
+    x_store<DP>(reinterpret_cast<T*>(p.dk) + at, dk[f], p.scale, p.D, g);
+    x_store<DP>(reinterpret_cast<T*>(p.dv) + at, dv[f], 1.f, p.D, g);
   }
 }
 
@@ -812,7 +826,8 @@ int launch(const XArgs& p, bool bwd, hipStream_t st) {
   constexpr int TWO = sizeof(T) == 2 ? 2 : 1;
   const bool two = TWO == 2 && p.Tq > 64 && (long long)p.B * p.H * ((p.Tq + 127) / 128) >= 512;
   if (!bwd) return two ? launch_fwd<T, DP, TWO, DROP>(p, st) : launch_fwd<T, DP, 1, DROP>(p, st);
-  const int rc = two ? launch_dq<T, DP, TWO, DROP>(p, st) : launch_dq<T, DP, 1, DROP>(p, st);
+  constexpr int TWO_DQ = DP <= 64 ? TWO : 1;      // (its two accumulators of 128 dimensions do not fit twice)
+  const int rc = two ? launch_dq<T, DP, TWO_DQ, DROP>(p, st) : launch_dq<T, DP, 1, DROP>(p, st);
   return rc != NSP_OK ? rc : launch_dkv<T, DP, 1, DROP>(p, st);
 }
 template <typename T, bool DROP>
@@ -832,10 +847,8 @@ int cross_attn(const nsp_cross_attn_params* a, bool bwd, void* stream) {
   if (a->B == 0 || a->Tk == 0 || (a->Tq == 0 && !bwd)) return NSP_OK;     // (nothing to read, or nothing to write but empty rows: the caller's)
   if (!a->k || !a->v || (a->Tq > 0 && (!a->q || !a->out))) return NSP_EINVAL;
   if (bwd && (a->Tq == 0 || !a->dout || !a->dq || !a->dk || !a->dv || !a->stats || !a->rows)) return NSP_EINVAL;
-  if (bwd && a->dtype == NSP_DT_BF16 && !a->o_lo) return NSP_EINVAL;
   XArgs p;
   p.q = a->q; p.k = a->k; p.v = a->v; p.dout = a->dout; p.out = a->out;
-  p.o_lo = a->dtype == NSP_DT_BF16 ? a->o_lo : nullptr;
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.stats = a->stats; p.rows = a->rows; p.klens = a->klens;
   p.B = (int)a->B; p.H = (int)a->H; p.Hkv = (int)a->Hkv; p.D = (int)a->D; p.Tq = (int)a->Tq; p.Tk = (int)a->Tk;
   p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;

@@ -2157,7 +2157,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _PLANS = {}
 _DECODE_PTRS, _DECODE_TAIL = _struct.Struct('<9q').pack, _struct.Struct('<22qd').pack        # nsp_decode_attn_params
 _APPEND_PTRS, _APPEND_TAIL = _struct.Struct('<7q').pack, _struct.Struct('<21q').pack         # nsp_paged_append_params
-_CROSS_PTRS, _CROSS_TAIL = _struct.Struct('<12q3q2Q').pack, _struct.Struct('<16q2d').pack    # nsp_cross_attn_params
+_CROSS_PTRS, _CROSS_TAIL = _struct.Struct('<11q3q2Q').pack, _struct.Struct('<16q2d').pack    # nsp_cross_attn_params
 _SAMPLE_PACK = _struct.Struct('<12q3d').pack                                                 # nsp_sample_params
 
 
@@ -2374,14 +2374,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
 
 class CrossAttnFn(torch.autograd.Function):
     """cross_attention with its backward (csrc/cross_attn.hip); arguments as checked there.  One buffer holds what backward
-    needs beside the inputs and the output: stats [2,B,H,Tq] and backward's scratch [3,B,H,Tq rounded up to 64] (fp32), and for
-    bf16 what the rounding of the output left."""
-
-    @staticmethod
-    def layout(B, Tq, H):
-        """byte offsets of the scratch and of the output's rest"""
-        n = B * H
-        return 8 * n * Tq, (8 * n * Tq + 12 * n * ((Tq + 63) // 64 * 64) + 15) // 16 * 16
+    needs beside the inputs and the output, stats [2,B,H,Tq], and backward's scratch [3,B,H,Tq rounded up to 64] (fp32)."""
 
     @staticmethod
     def forward(ctx, q, k, v, klens, tail, seed, need):
@@ -2391,16 +2384,14 @@ class CrossAttnFn(torch.autograd.Function):
             ctx.empty = True
             ctx.save_for_backward(q, k, v)
             return out.zero_()
-        buf, at, lo = None, 0, 0
+        buf, at = None, 0
         if need:
-            half = q.dtype == torch.bfloat16
-            lo = CrossAttnFn.layout(*q.shape[:3])[1]
-            buf = q.new_empty(((lo + 2 * rows if half else lo) // 4,), dtype=torch.float32)
+            B, Tq, H, _ = q.shape
+            buf = q.new_empty((B * H * (2 * Tq + 3 * ((Tq + 63) // 64 * 64)),), dtype=torch.float32)
             at = buf.data_ptr()
-            lo = at + lo if half else 0
         with _on(q.get_device()):
             _check(_lib.lib().nsp_cross_attn_fwd(_CROSS_PTRS(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), lo, 0, 0, 0, at, 0,
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, at, 0,
                 0 if klens is None else klens.data_ptr(), 0, 0, 0, seed, 0) + tail, _stream()), 'nsp_cross_attn_fwd')
         if need:
             ctx.empty, ctx.tail, ctx.seed = False, tail, seed
@@ -2416,12 +2407,13 @@ class CrossAttnFn(torch.autograd.Function):
             dout = _vec(dout.to(q.dtype))
         g0, g1, g2, _ = dout.stride()
         dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
-        rows, lo = CrossAttnFn.layout(*q.shape[:3])
+        B, Tq, H, _ = q.shape
         at = buf.data_ptr()
         with _on(q.get_device()):
             _check(_lib.lib().nsp_cross_attn_bwd(_CROSS_PTRS(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(),
-                at + lo if q.dtype == torch.bfloat16 else 0, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), at, at + rows, 0 if klens is None else klens.data_ptr(), g0, g1, g2, ctx.seed, 0) + ctx.tail, _stream()),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), at, at + 8 * B * H * Tq,
+                0 if klens is None else klens.data_ptr(), g0, g1, g2, ctx.seed, 0) + ctx.tail, _stream()),
                 'nsp_cross_attn_bwd')
         return dq, dk, dv, None, None, None, None
 
