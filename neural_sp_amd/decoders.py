@@ -20,6 +20,7 @@ import copy
 from itertools import groupby
 
 from neural_sp_amd import ops
+from neural_sp_amd.kv_cache import PagedKVCache
 
 logger = logging.getLogger(__name__)
 
@@ -557,6 +558,39 @@ class TransformerDecoderBlock(nn.Module):
         return self.feed_forward(on, residual=out, alpha=1.0, out_dropout=p)
 
 
+    # ---- one token at a time, with the keys and values of the tokens before it cached (TransformerDecoder.sample)
+    def source_kv(self, xs, dtype):
+        """keys and values of the encoder's states, computed once per utterance: two `[B,T,H,dk]`"""
+        B, T, _ = xs.shape
+        att = self.src_attn
+        return tuple(_step_linear(xs, w, dtype).view(B, T, att.n_heads, att.d_k) for w in (att.w_key, att.w_value))
+
+    def step(self, x, cache, lth, src, elens, dtype):
+        """x `[B,d_model]` of the newest tokens -> the block's output; their keys and values join layer `lth` of the cache"""
+        B = x.shape[0]
+        att = self.self_attn
+        xn = ops.layer_norm(x, self.norm1.weight, self.norm1.bias, self.norm1.eps)
+        q, k, v = (_step_linear(xn, w, dtype).view(B, att.n_heads, att.d_k) for w in (att.w_query, att.w_key, att.w_value))
+        cv = ops.paged_attention(q, cache.k(lth), cache.v(lth), cache.block_table, cache.lens, k, v)
+        x = ops.linear_fwd(cv.view(B, -1), att.w_out.weight, att.w_out.bias, res=x)
+        if self.src_attn is not None:
+            att = self.src_attn
+            xn = ops.layer_norm(x, self.norm2.weight, self.norm2.bias, self.norm2.eps)
+            q = _step_linear(xn, att.w_query, dtype).view(B, 1, att.n_heads, att.d_k)
+            cv = ops.cross_attention(q, src[0], src[1], elens)
+            x = ops.linear_fwd(cv.view(B, -1), att.w_out.weight, att.w_out.bias, res=x)
+        xn = ops.layer_norm(x, self.norm3.weight, self.norm3.bias, self.norm3.eps)
+        return self.feed_forward(xn, residual=x)
+
+
+def _step_linear(x, lin, dtype):
+    """x `[..,K]` @ weight^T + bias as `[rows,N]` of `dtype` (no autograd)"""
+    sh = getattr(x, '_nsp16', None)
+    x2 = sh if sh is not None else ops._f32c(x)
+    y = ops.linear_fwd(x2.reshape(-1, x2.shape[-1]), lin.weight, lin.bias, out_bf16=dtype == torch.bfloat16)
+    return y if y.dtype == dtype else ops.to_bf16(y)      # (an input width that is no multiple of 8 takes the fp32 GEMM)
+
+
 class TransformerDecoder(DecoderBase):
     """decoders/transformer.py:28-458, training side: hybrid CTC / attention loss of a Transformer
     decoder (BASELINE config 3's loss head family).  forward() = CTC branch
@@ -730,6 +764,64 @@ class TransformerDecoder(DecoderBase):
         hyps = [hb[b, :ylens[b]][::-1] if self.bwd else hb[b, :ylens[b]] for b in range(B)]
         if exclude_eos:
             hyps = [(h[1:] if self.bwd else h[:-1]) if eos_flags[b] else h for b, h in enumerate(hyps)]
+        return hyps, None
+
+    @torch.no_grad()
+    def sample(self, eouts, elens, max_len_ratio=1.0, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed=None,
+               exclude_eos=False, page_size=16, check_every=8):
+        """One hypothesis per utterance drawn token by token from the decoder's distribution (ops.sample_rows: temperature,
+        top_k, top_p, min_p; temperature 0 is the arg-max), at most ceil(T * max_len_ratio) tokens.  Every step works on the
+        newest token alone: self-attention over a paged key / value cache, source attention over keys and values computed once.
+        Source attention sees each utterance's own frames (elens), as in training -- `greedy` attends to the padding as well.
+
+        seed: the random numbers (one per utterance and step, drawn on the host) repeat with it; None takes torch's generator.
+        The device is asked every `check_every` steps whether all utterances have ended.
+        -> (hyps: list of int arrays, None), as `greedy`."""
+        if self.attn_type == 'mocha':
+            raise NotImplementedError('sampling with monotonic multi-head attention is not built')
+        if '1dconv' in self.pe_type:
+            raise NotImplementedError('sampling with 1dconv positions is not built (their state is not cached)')
+        d_k = self.d_model // self.n_heads
+        if d_k % 8 or d_k > 128:
+            raise NotImplementedError('sampling: head size %d (multiples of 8 up to 128)' % d_k)
+        dev = eouts.device
+        B, T = eouts.shape[:2]
+        dtype = torch.bfloat16 if ops.bf16_mode() else torch.float32
+        ymax = max(1, int(math.ceil(T * max_len_ratio)))
+        gen = None if seed is None else torch.Generator().manual_seed(int(seed))
+        u = ops.h2d(torch.rand((ymax, B), generator=gen, dtype=torch.float32), dev)
+        elens_d = ops.h2d(elens, dev, torch.int32)
+        cache = PagedKVCache(self.n_layers, B, ymax, self.n_heads, d_k, dtype, dev, page_size=page_size)
+        cache.lens.zero_()
+        src = [layer.source_kv(eouts, dtype) if layer.src_attn is not None else None for layer in self.layers]
+        y = torch.full((B,), self.eos, dtype=torch.int64, device=dev)
+        labels = torch.empty((ymax, B), device=dev, dtype=torch.int32)
+        done = torch.zeros((B,), device=dev, dtype=torch.bool)
+        n = 0
+        while n < ymax:
+            if n % page_size == 0:
+                cache.reserve(range(B), min(ymax, n + page_size))
+            x = self.pos_enc(self.embed(y).unsqueeze(1), scale=True, offset=n).view(B, -1)
+            for lth, layer in enumerate(self.layers):
+                x = layer.step(x, cache, lth, src[lth], elens_d, dtype)
+            x = ops.layer_norm(x, self.norm_out.weight, self.norm_out.bias, self.norm_out.eps)
+            logits = ops.linear(x, self.output.weight, self.output.bias)
+            y = ops.sample_rows(logits, u[n], temperature, top_k, top_p, min_p)
+            labels[n] = y
+            done |= y == self.eos
+            n += 1
+            if n % check_every == 0 and bool(done.all()):
+                break
+            # an utterance that has ended leaves the cache alone
+            cache.lens = torch.where(done, torch.full_like(cache.lens, -1), cache.lens + 1)
+            y = y.long()
+        lab = labels[:n].cpu().numpy()
+        hyps = []
+        for b in range(B):
+            end = np.flatnonzero(lab[:, b] == self.eos)
+            h = lab[:end[0] + 1, b] if len(end) else lab[:, b]
+            h = h[:-1] if exclude_eos and len(end) else h
+            hyps.append(h[::-1].copy() if self.bwd else h.copy())
         return hyps, None
 
     def beam_search(self, *a, **k):

@@ -13,6 +13,7 @@ Reference files (relative to the reference root):
 import logging
 import copy
 import math
+import os
 import random
 
 import torch
@@ -296,8 +297,18 @@ class MultiheadAttentionMechanism(nn.Module):
         v = ops.linear(value, self.w_value.weight, self.w_value.bias).view(bs, klen, H, dk)
         q = ops.linear(query, self.w_query.weight, self.w_query.bias).view(bs, qlen, H, dk)
         cfg = mask.cfg() if mask is not None else {}
-        cfg.update(clamp=-1, dropout=self.dropout_attn_p, training=self.training)
-        cv, aw = ops.AttentionFn.apply(q, None, k, v, None, mask.klens if mask is not None else None, cfg)
+        if (os.environ.get('NSP_CROSS_ATTN', '0') == '1' and key is not query and dk % 8 == 0 and dk <= 128
+                and not cfg.get('causal', False) and cfg.get('chunk_nc', 0) == 0):
+            # source attention without its [B,H,qlen,klen] scores: same mask, same dropout decisions; in bf16 mode its operands
+            # and its context are bf16.  Not the default: the results differ from AttentionFn's by roundings.
+            if ops.bf16_mode():
+                q, k, v = ops.cast_bf16(q), ops.cast_bf16(k), ops.cast_bf16(v)
+            cv = ops.cross_attention(q, k, v, mask.klens if mask is not None else None,
+                                     dropout_p=self.dropout_attn_p if self.training else 0.0)
+            cv, aw = (ops.cast_f32(cv) if cv.dtype != torch.float32 else cv).view(bs, qlen, d), None
+        else:
+            cfg.update(clamp=-1, dropout=self.dropout_attn_p, training=self.training)
+            cv, aw = ops.AttentionFn.apply(q, None, k, v, None, mask.klens if mask is not None else None, cfg)
         if headdrop:
             # HeadDrop (modules/headdrop.py:10-32, multihead_attention.py:147-148): whole heads are zeroed with
             # probability dropout_head (Python's `random`, one draw per head) and the survivors rescaled; the context

@@ -2477,6 +2477,42 @@ def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
     return CrossAttnFn.apply(q, k, v, klens, tail, next_dropout_seed()[0] if dropout_p > 0 else 0, need)
 
 
+class CastBF16Fn(torch.autograd.Function):
+    """fp32 -> bf16 (nearest even); the gradient comes back as fp32"""
+
+    @staticmethod
+    def forward(ctx, x):
+        n = x.shape[-1]
+        y = to_bf16(_f32c(x).reshape(-1, n))
+        return (y if y.shape[1] == n else y[:, :n].contiguous()).view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return dy.float()
+
+
+def cast_bf16(x):
+    return CastBF16Fn.apply(x)
+
+
+class CastF32Fn(torch.autograd.Function):
+    """bf16 -> fp32; the gradient is rounded to bf16 (nearest even)"""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.float()
+
+    @staticmethod
+    def backward(ctx, dy):
+        n = dy.shape[-1]
+        g = to_bf16(_f32c(dy).reshape(-1, n))
+        return (g if g.shape[1] == n else g[:, :n].contiguous()).view(dy.shape)
+
+
+def cast_f32(x):
+    return CastF32Fn.apply(x)
+
+
 def _sample_setting(x, dtype, rows, dev, what):
     """(device address or 0, value) of a per-row tensor or a number; a tensor has to stay alive over the launch"""
     if not torch.is_tensor(x):

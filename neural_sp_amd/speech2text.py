@@ -340,6 +340,8 @@ class Speech2Text(nn.Module):
         validate() (train.py:341,513-557 -> evaluators/*.py) runs during training with the default
         recog_* arguments: CTC best path (ctc.py:219-243) when the model is CTC-only or
         recog_ctc_weight == 1, else the RNN-T frame-synchronous 1-best (rnn_transducer.py:330-382).
+        `recog_sampling` (not in the reference) draws a hypothesis from the Transformer decoder instead of taking the 1-best:
+        recog_temperature, recog_top_k, recog_top_p, recog_min_p, recog_seed (TransformerDecoder.sample).
         Returns (nbest_hyps_id `[B][1][L]`, aws None).  Beam search / LM fusion / streaming /
         ensembles are inference-side and raise NotImplementedError."""
         self.eval()
@@ -365,6 +367,14 @@ class Speech2Text(nn.Module):
             return dec.ctc.greedy(eouts, elens), None
         if beam != 1 or P(params, 'recog_fwd_bwd_attention', False):
             dec.beam_search()
+        if P(params, 'recog_sampling', False):
+            # not in the reference: one sampled hypothesis per utterance from the attention decoder, with cached states
+            if not hasattr(dec, 'sample'):
+                raise NotImplementedError('recog_sampling: the Transformer decoder only')
+            hyps, aws = dec.sample(eouts, elens, P(params, 'recog_max_len_ratio', 1.0), P(params, 'recog_temperature', 1.0),
+                                   P(params, 'recog_top_k', 0), P(params, 'recog_top_p', 1.0), P(params, 'recog_min_p', 0.0),
+                                   P(params, 'recog_seed', None), exclude_eos)
+            return [[hyp] for hyp in hyps], aws
         kw = {}
         if 'trigger_points' in inspect.signature(dec.greedy).parameters:
             kw['trigger_points'] = trigger_points        # triggered attention decodes from the CTC alignment
