@@ -184,6 +184,28 @@ def sample_case(ops, dev, x, u, t=1.0, k=0, tp=1.0, mp=0.0):
     assert got.cpu().tolist() == want, (got.cpu().tolist(), want)
 
 
+# what can stay, gathered: (V, settings) where equal logits, the list's size (two entries per thread: 512 up to 1024 logits, 1024
+# above) or its bins of several indices are met
+SAMPLE_GATHERED = [
+    (1000, dict(k=511)), (1000, dict(k=512, tp=.9)), (1000, dict(k=513, tp=.9)), (1000, dict(k=999, tp=.99)),
+    (1025, dict(k=1024, tp=.97)), (3000, dict(k=1023, tp=.8)), (3000, dict(k=1024, mp=.02)), (3000, dict(k=1025, tp=.8)),
+    (3000, dict(tp=.5)), (3000, dict(tp=.98, t=1.5)), (12000, dict(k=300, tp=.9)), (12000, dict(tp=.6)),
+    (40000, dict(k=900, tp=.95, t=2.)), (40000, dict(tp=.3)),
+]
+
+
+def gathered_case(ops, dev, V, kw):
+    """normal logits; 400 equal ones within the list before the border's bin (top_p ends among them); one outlier so low
+    that all others share a bin"""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(3, V, generator=g) * 2
+    at = torch.randperm(V, generator=g)[:400]
+    x[1, at] = 7.5
+    x[1, at[:3]] = 12.0
+    x[2, V // 2] = -1e30
+    sample_case(ops, dev, x, [0.03, 0.5, 0.98], **kw)
+
+
 def cross_ref(q, k, v, dout, klens, dtype, scale=None, keep=None):
     """forward and formula gradients in 64 bits, with a bound for every element.  keep [B,H,Tq,Tk]: dropout factors (0 or
     1 / (1 - p)).  -> {'out': (ref, tol), 'dq': ..., 'dk': ..., 'dv': ...}"""

@@ -95,6 +95,11 @@ def test_sample_rows_of_equal_logits(emu, kw):
     C.sample_case(emu, 'cpu', x, u, **kw)
 
 
+@pytest.mark.parametrize('V,kw', C.SAMPLE_GATHERED, ids=str)
+def test_sample_rows_gathered(emu, V, kw):
+    C.gathered_case(emu, 'cpu', V, kw)
+
+
 def test_sample_rows_infinities_and_nan(emu):
     inf, nan = float('inf'), float('nan')
     x = torch.tensor([[nan, 1.0, nan, 2.0], [-inf, -inf, -inf, -inf], [0.0, inf, 1.0, inf], [nan, nan, nan, nan],

@@ -95,6 +95,11 @@ def test_sample_rows_long_rows_and_ties(ops):
         C.sample_case(ops, DEV, x, [0.2, 0.9], **kw)
 
 
+@pytest.mark.parametrize('V,kw', C.SAMPLE_GATHERED, ids=str)
+def test_sample_rows_gathered(ops, V, kw):
+    C.gathered_case(ops, DEV, V, kw)
+
+
 def test_sample_rows_temperature_zero_is_argmax_rows(ops):
     x = torch.randn(33, 777, generator=torch.Generator().manual_seed(4)).to(DEV).round()
     assert torch.equal(ops.sample_rows(x, torch.zeros(33, device=DEV), temperature=0.0), ops.argmax_rows(x))
