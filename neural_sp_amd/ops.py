@@ -2169,23 +2169,17 @@ def _plan(key, make, *args):
     return plan
 
 
-class _NoCtx(object):
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *a):
-        return False
-
-
-_NULL_CTX = _NoCtx()
-
-
-def _on(dev):
-    """context that makes device number `dev` current around a launch when it is not (whose stream is then that device's
-    current one)"""
+def _call(name, dev, params):
+    """one entry point with its packed parameters, on device number `dev`'s current stream (made current around the launch
+    when it is not)"""
+    fn = getattr(_lib.lib(), name)
     if dev < 0 or dev == torch._C._cuda_getDevice():
-        return _NULL_CTX
-    return torch.cuda.device(dev)
+        rc = fn(params, _stream())
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(params, _stream())
+    if rc != 0:
+        _check(rc, name)
 
 
 def _devices_differ(*tensors):
@@ -2311,12 +2305,10 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
         _need_aligned(k_pages, v_pages)
         return paged_attention(_vec(q), k_pages, v_pages, block_table.contiguous(), lens.contiguous(),
                                None if k_new is None else _vec(k_new), None if v_new is None else _vec(v_new), scale)
-    with _on(dev):
-        out = q.new_empty(q.shape)
-        ws = q.new_empty((ws_floats,), dtype=torch.float32) if ws_floats else None
-        _check(_lib.lib().nsp_decode_attn(_DECODE_PTRS(
-            qa, out.data_ptr(), ka, va, block_table.data_ptr(), lens.data_ptr(), kn, vn, ws.data_ptr() if ws_floats else 0) + tail,
-            _stream()), 'nsp_decode_attn')
+    out = q.new_empty(q.shape)
+    ws = q.new_empty((ws_floats,), dtype=torch.float32) if ws_floats else None
+    _call('nsp_decode_attn', dev, _DECODE_PTRS(
+        qa, out.data_ptr(), ka, va, block_table.data_ptr(), lens.data_ptr(), kn, vn, ws.data_ptr() if ws_floats else 0) + tail)
     return out
 
 
@@ -2366,10 +2358,8 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
         _need_aligned(k_pages, v_pages)
         return paged_append(_vec(k), _vec(v), k_pages, v_pages, block_table.contiguous(), starts.contiguous(),
                             None if counts is None else counts.contiguous())
-    with _on(dev):
-        _check(_lib.lib().nsp_paged_append(_APPEND_PTRS(
-            ka, va, kp, vp, block_table.data_ptr(), starts.data_ptr(), 0 if counts is None else counts.data_ptr()) + tail,
-            _stream()), 'nsp_paged_append')
+    _call('nsp_paged_append', dev, _APPEND_PTRS(
+        ka, va, kp, vp, block_table.data_ptr(), starts.data_ptr(), 0 if counts is None else counts.data_ptr()) + tail)
 
 
 class CrossAttnFn(torch.autograd.Function):
@@ -2389,10 +2379,9 @@ class CrossAttnFn(torch.autograd.Function):
             B, Tq, H, _ = q.shape
             buf = q.new_empty((B * H * (2 * Tq + 3 * ((Tq + 63) // 64 * 64)),), dtype=torch.float32)
             at = buf.data_ptr()
-        with _on(q.get_device()):
-            _check(_lib.lib().nsp_cross_attn_fwd(_CROSS_PTRS(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, at, 0,
-                0 if klens is None else klens.data_ptr(), 0, 0, 0, seed, 0) + tail, _stream()), 'nsp_cross_attn_fwd')
+        _call('nsp_cross_attn_fwd', q.get_device(), _CROSS_PTRS(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, at, 0,
+            0 if klens is None else klens.data_ptr(), 0, 0, 0, seed, 0) + tail)
         if need:
             ctx.empty, ctx.tail, ctx.seed = False, tail, seed
             ctx.save_for_backward(q, k, v, klens, out, buf)
@@ -2409,12 +2398,9 @@ class CrossAttnFn(torch.autograd.Function):
         dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
         B, Tq, H, _ = q.shape
         at = buf.data_ptr()
-        with _on(q.get_device()):
-            _check(_lib.lib().nsp_cross_attn_bwd(_CROSS_PTRS(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(),
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), at, at + 8 * B * H * Tq,
-                0 if klens is None else klens.data_ptr(), g0, g1, g2, ctx.seed, 0) + ctx.tail, _stream()),
-                'nsp_cross_attn_bwd')
+        _call('nsp_cross_attn_bwd', q.get_device(), _CROSS_PTRS(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), at, at + 8 * B * H * Tq, 0 if klens is None else klens.data_ptr(), g0, g1, g2, ctx.seed, 0) + ctx.tail)
         return dq, dk, dv, None, None, None, None
 
 
@@ -2467,12 +2453,10 @@ def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
         return cross_attention(_vec(q), _vec(k), _vec(v), klens if klens is None else klens.contiguous(), scale, dropout_p)
     need = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
     if one is not None and not need:
-        with _on(dev):
-            out = q.new_empty(q.shape)
-            ws = q.new_empty((floats,), dtype=torch.float32) if floats else None
-            _check(_lib.lib().nsp_decode_attn(_DECODE_PTRS(
-                qa, out.data_ptr(), ka, va, 0, 0 if klens is None else klens.data_ptr(), 0, 0, ws.data_ptr() if floats else 0)
-                + one, _stream()), 'nsp_decode_attn')
+        out = q.new_empty(q.shape)
+        ws = q.new_empty((floats,), dtype=torch.float32) if floats else None
+        _call('nsp_decode_attn', dev, _DECODE_PTRS(
+            qa, out.data_ptr(), ka, va, 0, 0 if klens is None else klens.data_ptr(), 0, 0, ws.data_ptr() if floats else 0) + one)
         return out
     return CrossAttnFn.apply(q, k, v, klens, tail, next_dropout_seed()[0] if dropout_p > 0 else 0, need)
 
@@ -2546,19 +2530,18 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     k, k_all = _sample_setting(top_k, torch.int32, rows, dev, 'top_k')
     tp, tp_all = _sample_setting(top_p, torch.float32, rows, dev, 'top_p')
     mp, mp_all = _sample_setting(min_p, torch.float32, rows, dev, 'min_p')
-    with _on(dev):
-        out = torch.empty((rows,), device=logits.device, dtype=torch.int32)
-        if rows == 0:
-            return out
-        ld, step = logits.stride()
-        if (step != 1 and V > 1) or (ld < V and rows > 1):
-            logits = logits.contiguous()
-            ld = V
-        if not u.is_contiguous():
-            u = u.contiguous()
-        _check(_lib.lib().nsp_sample_rows(_SAMPLE_PACK(
-            logits.data_ptr(), u.data_ptr(), t, k, tp, mp, out.data_ptr(), rows, V, ld if rows > 1 else V,
-            _DTYPES[logits.dtype], min(max(k_all, 0), V), t_all, tp_all, mp_all), _stream()), 'nsp_sample_rows')
+    out = logits.new_empty((rows,), dtype=torch.int32)
+    if rows == 0:
+        return out
+    ld, step = logits.stride()
+    if (step != 1 and V > 1) or (ld < V and rows > 1):
+        logits = logits.contiguous()
+        ld = V
+    if not u.is_contiguous():
+        u = u.contiguous()
+    _call('nsp_sample_rows', dev, _SAMPLE_PACK(
+        logits.data_ptr(), u.data_ptr(), t, k, tp, mp, out.data_ptr(), rows, V, ld if rows > 1 else V, _DTYPES[logits.dtype],
+        min(max(k_all, 0), V), t_all, tp_all, mp_all))
     return out
 
 
