@@ -768,7 +768,7 @@ int nsp_lstm_cell_bwd(const float* dh, const float* dc_next, const float* gates,
  *   k_j), j < lens[b]; query head h reads key head h / (H / Hkv).              *
  *   table != NULL: keys are slots j % page of page table[b][j / page] of        *
  *     k / v = [n_pages, Hkv, page, D] (strides *_sp, *_sh, *_ss); width =       *
- *     entries of a table row.  k_new / v_new [B,Hkv,D] (or both NULL): stored    *
+ *     entries of a table row (>= 1).  k_new / v_new [B,Hkv,D] or both NULL: stored *
  *     at position lens[b] and attended to as well.  A sequence without a key     *
  *     gets zeros; lens[b] < 0 marks an unused row (zeros, nothing stored);       *
  *     lens[b] > width * page counts as that; keys of a page outside [0, n_pages) *

@@ -402,7 +402,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
 #pragma unroll
     for (int i = 0; i < X::NB; ++i) o[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     sum[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m[f] = -INFINITY;
+    m[f] = -3.4028235e38f;      // (finite: a tile whose scores are all -inf leaves the row as it is)
     l[f] = 0.f;
   }
   unsigned ta[4];
@@ -456,7 +456,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
 #pragma unroll
         for (int kf = 0; kf < 2; ++kf)
           mx[f] = attn_max(attn_max(attn_max(mx[f], s[u][f][kf][0]), attn_max(s[u][f][kf][1], s[u][f][kf][2])), s[u][f][kf][3]);
-      mx[f] = attn_max4(mx[f]) * p.sl2;    // (scale > 0: the maximum commutes with it; a tile has a visible key: finite)
+      mx[f] = attn_max4(mx[f]) * p.sl2;    // (scale > 0: the maximum commutes with it)
       move = move || !(mx[f] <= m[f] + 8.f);
     }
     if (__any(move)) {
@@ -842,7 +842,8 @@ int cross_attn(const nsp_cross_attn_params* a, bool bwd, void* stream) {
   if (a->D % 8 || a->D > 128 || (a->dtype != NSP_DT_F32 && a->dtype != NSP_DT_BF16)) return NSP_EUNSUPPORTED;
   if (a->B * a->H > 0x7ffffff0LL || a->Tq > 0x7fffff00LL || a->Tk > 0x7fffff00LL || !(a->scale > 0.)) return NSP_EUNSUPPORTED;
   const long long far = 1 << 24;      // (32-bit offsets inside a tile)
-  if (a->q_st >= far || a->k_st >= far || a->v_st >= far || a->g_st >= far) return NSP_EUNSUPPORTED;
+  for (const long long ld : {a->q_st, a->k_st, a->v_st, a->g_st})
+    if (ld < 0 || ld >= far) return NSP_EUNSUPPORTED;
   if (!(a->dropout_p >= 0. && a->dropout_p < 1.)) return NSP_EINVAL;
   if (a->B == 0 || a->Tk == 0 || (a->Tq == 0 && !bwd)) return NSP_OK;     // (nothing to read, or nothing to write but empty rows: the caller's)
   if (!a->k || !a->v || (a->Tq > 0 && (!a->q || !a->out))) return NSP_EINVAL;

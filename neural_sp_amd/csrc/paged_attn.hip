@@ -528,13 +528,13 @@ extern "C" int nsp_decode_attn(const nsp_decode_attn_params* a, void* stream) {
   if (a->B < 0 || a->Tq < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->D <= 0) return NSP_EINVAL;
   if (a->D % 8 || a->D > 128 || (a->dtype != NSP_DT_F32 && a->dtype != NSP_DT_BF16)) return NSP_EUNSUPPORTED;
   if (a->B == 0 || a->Tq == 0) return NSP_OK;
-  if (a->width < 0 || (a->table && (a->page <= 0 || a->n_pages < 0 || !a->lens)) || (!a->table && a->k_new)) return NSP_EINVAL;
+  if (a->width < 0 || (a->table && (a->width == 0 || a->page <= 0 || a->n_pages < 0 || !a->lens)) || (!a->table && a->k_new)) return NSP_EINVAL;
   if ((a->k_new != nullptr) != (a->v_new != nullptr)) return NSP_EINVAL;
   const long long cap = a->table ? a->width * a->page : a->width;
   if (cap > 0 && (!a->k || !a->v)) return NSP_EINVAL;
   const long long rows = a->H / a->Hkv * a->Tq, ngrp = (rows + 15) / 16;
   // 32-bit key positions; grid dimensions
-  if (cap > 0x7fff0000LL || a->B > 65535 || a->Hkv * ngrp > 65535 || rows > 0x7fffffffLL) return NSP_EUNSUPPORTED;
+  if (cap > 0x7f000000LL || a->B > 65535 || a->Hkv * ngrp > 65535 || rows > 0x7fffffffLL) return NSP_EUNSUPPORTED;
   DecodeArgs p;
   p.q = a->q; p.out = a->out; p.k = a->k; p.v = a->v; p.table = a->table; p.lens = a->lens;
   p.k_new = a->k_new; p.v_new = a->v_new; p.ws = a->ws;
@@ -555,7 +555,7 @@ extern "C" int nsp_decode_attn(const nsp_decode_attn_params* a, void* stream) {
 extern "C" int nsp_paged_append(const nsp_paged_append_params* a, void* stream) {
   if (!a || !a->k || !a->v || !a->k_pages || !a->v_pages || !a->table || !a->starts) return NSP_EINVAL;
   if (a->B < 0 || a->n < 0 || a->Hkv <= 0 || a->D <= 0 || a->page <= 0 || a->width < 0 || a->n_pages < 0) return NSP_EINVAL;
-  if (a->D % 8 || a->D > 128 || a->B > 65535 || a->n > 0x7fffffffLL || a->width * a->page > 0x7fff0000LL) return NSP_EUNSUPPORTED;
+  if (a->D % 8 || a->D > 128 || a->B > 65535 || a->n > 0x7fffffffLL || a->width * a->page > 0x7f000000LL) return NSP_EUNSUPPORTED;
   if (a->B == 0 || a->n == 0 || a->width == 0) return NSP_OK;
   const long long pieces = a->D / (a->dtype == NSP_DT_BF16 ? 8 : 4);
   long long gx = (a->n * a->Hkv * pieces + 255) / 256;

@@ -11,6 +11,7 @@ import os
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from neural_sp_amd import _lib
 from neural_sp_amd._lib import AttnMaskParams
@@ -2207,6 +2208,12 @@ def _need(t, dtype, shape, what):
         raise ValueError('%s: %s %s expected, got %s %s' % (what, dtype, list(shape), t.dtype, list(t.shape)))
 
 
+def _need_number(x, what):
+    """(a tensor would stand in the table of calls by its identity, and keep the value it had then)"""
+    if torch.is_tensor(x):
+        raise ValueError('%s: a number expected, got a tensor' % what)
+
+
 def _need_head_size(D):
     if D % 8 or not 0 < D <= 128:
         raise ValueError('head size %d: multiples of 8 up to 128 are supported' % D)
@@ -2221,8 +2228,14 @@ def _need_pages(k_pages, v_pages, block_table, B, Hkv, D):
         raise ValueError('pages: contiguous last dimension, other strides multiples of 8 elements expected')
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError('block_table: int32 [%d, pages] expected, got %s %s' % (B, block_table.dtype, tuple(block_table.shape)))
-    if block_table.shape[1] * k_pages.shape[2] > 0x7fff0000:
-        raise ValueError('more than 2^31 positions in a block table row')
+    if block_table.shape[1] * k_pages.shape[2] > 0x7f000000:
+        raise ValueError('a block table row holds up to 2^31 - 2^24 positions')
+
+
+def _need_writable(*pages):
+    for t in pages:
+        if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+            raise ValueError('pages: an expanded tensor cannot be written to')
 
 
 def _need_aligned(*pages):
@@ -2256,8 +2269,10 @@ def _paged_plan(q, k_pages, v_pages, block_table, lens, k_new, v_new, scale):
     if k_new is not None:
         _need(k_new, q.dtype, (B, Hkv, D), 'k_new')
         _need(v_new, q.dtype, (B, Hkv, D), 'v_new')
+        _need_writable(k_pages, v_pages)
         as_is = as_is and _vec_strides(k_new) and _vec_strides(v_new)
         ns = (k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1))
+    _need_number(scale, 'scale')
     scale = D ** -0.5 if scale is None else float(scale)
     if B == 0 or block_table.shape[1] == 0 or k_pages.shape[0] == 0:
         return 'zeros', None, 0               # no sequence, or no key and no room
@@ -2301,6 +2316,8 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
     if how == 'zeros':
         return torch.zeros(q.shape, device=q.device, dtype=q.dtype)
     qa, ka, va = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
+    if kn and ka == va:
+        raise ValueError('k_pages and v_pages are the same memory')
     if how == 'copy' or (qa | ka | va | kn | vn) & 15:
         _need_aligned(k_pages, v_pages)
         return paged_attention(_vec(q), k_pages, v_pages, block_table.contiguous(), lens.contiguous(),
@@ -2318,6 +2335,7 @@ def _append_plan(k, v, k_pages, v_pages, block_table, starts, counts):
     B, n, Hkv, D = k.shape
     _need_head_size(D)
     _need_pages(k_pages, v_pages, block_table, B, Hkv, D)
+    _need_writable(k_pages, v_pages)
     if k.dtype == torch.bfloat16 and k_pages.dtype != torch.bfloat16:
         raise ValueError('%s into a %s cache' % (k.dtype, k_pages.dtype))
     _need(starts, torch.int32, (B,), 'starts')
@@ -2354,6 +2372,8 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
     if how == 'nothing':
         return
     ka, va, kp, vp = k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
+    if kp == vp:
+        raise ValueError('k_pages and v_pages are the same memory')
     if how == 'copy' or (ka | va | kp | vp) & 15:
         _need_aligned(k_pages, v_pages)
         return paged_append(_vec(k), _vec(v), k_pages, v_pages, block_table.contiguous(), starts.contiguous(),
@@ -2363,45 +2383,53 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
 
 
 class CrossAttnFn(torch.autograd.Function):
-    """cross_attention with its backward (csrc/cross_attn.hip); arguments as checked there.  One buffer holds what backward
-    needs beside the inputs and the output, stats [2,B,H,Tq], and backward's scratch [3,B,H,Tq rounded up to 64] (fp32)."""
+    """cross_attention with its backward (csrc/cross_attn.hip); arguments as checked there.  Saved beside the inputs and the
+    output: stats [2,B,H,Tq] (fp32).  Backward's scratch [3,B,H,Tq rounded up to 64] is its own, as two captured backward passes
+    over one forward pass may be replayed side by side."""
 
     @staticmethod
-    def forward(ctx, q, k, v, klens, tail, seed, need):
+    def forward(ctx, q, k, v, klens, tail, seed, need, scale, dropout_p):
         out = q.new_empty(q.shape)
         rows = out.numel()
         if k.numel() == 0 or rows == 0:       # nothing to read: zeros, with zero gradients
             ctx.empty = True
             ctx.save_for_backward(q, k, v)
             return out.zero_()
-        buf, at = None, 0
+        stats, at = None, 0
         if need:
             B, Tq, H, _ = q.shape
-            buf = q.new_empty((B * H * (2 * Tq + 3 * ((Tq + 63) // 64 * 64)),), dtype=torch.float32)
-            at = buf.data_ptr()
+            stats = q.new_empty((2 * B * H * Tq,), dtype=torch.float32)
+            at = stats.data_ptr()
         _call('nsp_cross_attn_fwd', q.get_device(), _CROSS_PTRS(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, at, 0,
             0 if klens is None else klens.data_ptr(), 0, 0, 0, seed, 0) + tail)
         if need:
-            ctx.empty, ctx.tail, ctx.seed = False, tail, seed
-            ctx.save_for_backward(q, k, v, klens, out, buf)
+            ctx.empty, ctx.tail, ctx.seed, ctx.setting = False, tail, seed, (scale, dropout_p)
+            ctx.strides = q.stride(), k.stride(), v.stride()
+            ctx.save_for_backward(q, k, v, klens, out, stats)
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         if ctx.empty:
-            return tuple(torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * 4
-        q, k, v, klens, out, buf = ctx.saved_tensors
+            return tuple(torch.zeros_like(t) for t in ctx.saved_tensors) + (None,) * 6
+        q, k, v, klens, out, stats = ctx.saved_tensors
+        tail = ctx.tail
+        if (q.stride(), k.stride(), v.stride()) != ctx.strides or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 or \
+                not out.is_contiguous() or out.data_ptr() & 15:      # saved-tensor hooks may lay them out anew
+            q, k, v, out = (t.clone(memory_format=torch.contiguous_format) for t in (q, k, v, out))
+            tail = _cross_plan(q, k, v, klens, *ctx.setting)[1]
         if dout.dtype != q.dtype or not dout.is_contiguous() or dout.data_ptr() & 15:
             dout = _vec(dout.to(q.dtype))
         g0, g1, g2, _ = dout.stride()
         dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
         B, Tq, H, _ = q.shape
-        at = buf.data_ptr()
+        rows = q.new_empty((3 * B * H * ((Tq + 63) // 64 * 64),), dtype=torch.float32)
         _call('nsp_cross_attn_bwd', q.get_device(), _CROSS_PTRS(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-            dv.data_ptr(), at, at + 8 * B * H * Tq, 0 if klens is None else klens.data_ptr(), g0, g1, g2, ctx.seed, 0) + ctx.tail)
-        return dq, dk, dv, None, None, None, None
+            dv.data_ptr(), stats.data_ptr(), rows.data_ptr(), 0 if klens is None else klens.data_ptr(), g0, g1, g2, ctx.seed, 0) + tail)
+        return dq, dk, dv, None, None, None, None, None, None
 
 
 def _cross_plan(q, k, v, klens, scale, dropout_p):
@@ -2417,6 +2445,8 @@ def _cross_plan(q, k, v, klens, scale, dropout_p):
     _need_head_size(D)
     if klens is not None:
         _need(klens, torch.int32, (B,), 'klens')
+    _need_number(scale, 'scale')
+    _need_number(dropout_p, 'dropout_p')
     scale = D ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale) and 0.0 <= dropout_p < 1.0):
         raise ValueError('scale %r, dropout_p %r' % (scale, dropout_p))
@@ -2424,7 +2454,7 @@ def _cross_plan(q, k, v, klens, scale, dropout_p):
         return False, None, None, 0
     st = [t.stride()[:3] for t in (q, k, v)]
     tail = _CROSS_TAIL(B, H, Hkv, D, Tq, Tk, _DTYPES[q.dtype], *st[0], *st[1], *st[2], scale, dropout_p)
-    few = dropout_p == 0 and Tq * (H // Hkv) <= 16 and B > 0 and Tq > 0 and Tk > 0
+    few = dropout_p == 0 and 0 < Tq * (H // Hkv) <= 16 and 0 < B <= 65535 and Hkv <= 65535 and 0 < Tk <= 0x7f000000
     one, floats = _decode_tail(B, H, Hkv, D, Tq, 1, 0, Tk, q.dtype, *st, (0, 0, 0, 0), scale) if few else (None, 0)
     return True, tail, one, floats
 
@@ -2458,7 +2488,7 @@ def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
         _call('nsp_decode_attn', dev, _DECODE_PTRS(
             qa, out.data_ptr(), ka, va, 0, 0 if klens is None else klens.data_ptr(), 0, 0, ws.data_ptr() if floats else 0) + one)
         return out
-    return CrossAttnFn.apply(q, k, v, klens, tail, next_dropout_seed()[0] if dropout_p > 0 else 0, need)
+    return CrossAttnFn.apply(q, k, v, klens, tail, next_dropout_seed()[0] if dropout_p > 0 else 0, need, scale, dropout_p)
 
 
 class CastBF16Fn(torch.autograd.Function):

@@ -10,6 +10,7 @@ rounding to t:
 and an error of the terms of sum_j p_j v_j is at most that relative error times sum_j p_j |v_j|."""
 import math
 
+import pytest
 import torch
 
 E32 = torch.finfo(torch.float32).eps / 2
@@ -391,3 +392,46 @@ def difference_case(ops, dev):
         tol = abs(quot64 - slope64) + float(((ref[0][1] + ref[1][1]) * w.abs()).sum()) / (2 * h) + float((t * d[i].abs()).sum())
         assert abs(quot - slope) <= tol, (i, quot, slope, tol)
         assert tol < 0.2 * abs(slope64), (i, tol, slope64)
+
+
+def backward_case(ops, dev):
+    """a second backward pass finds everything as the first one left it, also on saved tensors that hooks laid out anew"""
+    g = torch.Generator().manual_seed(3)
+    def leaf(B, h, t):      # (a view of [B,h,t,d]: strides that a copy does not keep)
+        return torch.randn(B, h, t, 32, generator=g).to(dev).transpose(1, 2).detach().requires_grad_()
+    q, k, v = leaf(2, 4, 5), leaf(2, 2, 70), leaf(2, 2, 70)
+    klens = torch.tensor([70, 33], dtype=torch.int32).to(dev)
+    d1, d2 = (torch.randn(2, 5, 4, 32, generator=g).to(dev) for _ in range(2))
+    kept = []
+
+    def pack(t):
+        kept.append((t, t.detach().clone()))
+        return t
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        out = ops.cross_attention(q, k, v, klens, scale=0.25)
+    first = torch.autograd.grad(out, (q, k, v), d1, retain_graph=True)
+    other = torch.autograd.grad(out, (q, k, v), d2, retain_graph=True)
+    again = torch.autograd.grad(out, (q, k, v), d1, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    assert not any(torch.equal(a, b) for a, b in zip(first, other))
+    assert kept and all(torch.equal(t, was) for t, was in kept)      # nothing saved is written to
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous().clone(), lambda t: t):
+        out = ops.cross_attention(q, k, v, klens, scale=0.25)
+    laid_out = torch.autograd.grad(out, (q, k, v), d1)
+    assert all(torch.equal(a, b) for a, b in zip(first, laid_out))
+    out = ops.cross_attention(q, k, v, klens)
+    with pytest.raises(RuntimeError):
+        gq = torch.autograd.grad(out.square().sum(), q, create_graph=True)[0]
+        torch.autograd.grad(gq.sum(), k)
+
+
+def infinite_scores_case(ops, dev, dtype):
+    """keys with a score of -inf have no probability, also where they fill the first tiles"""
+    g = torch.Generator().manual_seed(8)
+    q, k, v = torch.randn(1, 9, 2, 64, generator=g), torch.randn(1, 150, 2, 64, generator=g), torch.randn(1, 150, 2, 64, generator=g)
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    q[..., 0] = 1.0
+    k[:, :130, :, 0] = float('-inf')
+    want = cross_ref(q[:, :, :, :], k[:, 130:], v[:, 130:], None, None, dtype)['out']
+    for grad in (True, False):
+        check_close(ops.cross_attention(q.to(dev).requires_grad_(grad), k.to(dev), v.to(dev)).detach(), want[0], want[1], 'out')

@@ -195,3 +195,31 @@ def test_cross_attention_dropout_is_the_training_softmax_mask(emu):
 
 def test_cross_attention_against_differences(emu):
     C.difference_case(emu, 'cpu')
+
+
+def test_cross_attention_backward_passes_do_not_meet(emu):
+    C.backward_case(emu, 'cpu')
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+def test_cross_attention_scores_of_minus_infinity(emu, dtype):
+    C.infinite_scores_case(emu, 'cpu', dtype)
+
+
+def test_refusals_of_memory_and_settings(emu):
+    """pages that one write would change in several places, and settings that are tensors"""
+    i32 = torch.int32
+    q, t, lens, n = torch.zeros(2, 4, 16), torch.zeros(2, 2, dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(2, 2, 16)
+    kp, vp = torch.zeros(3, 2, 4, 16), torch.zeros(3, 2, 4, 16)
+    wide = torch.zeros(1, 2, 4, 16).expand(3, 2, 4, 16)
+    x = torch.zeros(2, 1, 2, 16)
+    emu.paged_attention(q, kp, kp, t, lens)             # one tensor for both, and an expanded one, may be read
+    emu.paged_attention(q, wide, wide, t, lens)
+    c = torch.zeros(2, 3, 4, 16)
+    for bad in (lambda: emu.paged_attention(q, kp, kp, t, lens, n, n), lambda: emu.paged_attention(q, wide, vp, t, lens, n, n),
+                lambda: emu.paged_append(x, x, kp, kp, t, lens), lambda: emu.paged_append(x, x, kp, wide, t, lens),
+                lambda: emu.paged_attention(q, kp, vp, t, lens, scale=torch.tensor(0.5)),
+                lambda: emu.cross_attention(c, c, c, scale=torch.tensor(0.5)),
+                lambda: emu.cross_attention(c, c, c, dropout_p=torch.tensor(0.5))):
+        with pytest.raises(ValueError):
+            bad()

@@ -242,3 +242,23 @@ def test_cache_offsets_behind_32_bits(ops):
     for h in range(Hkv):
         ref, dp, av = C.attention_ref(q[0, 2 * h:2 * h + 2], k[0, :, h], v[0, :, h], 150)
         C.check_close(out[0, 2 * h:2 * h + 2], ref, C.half_step(BF) * ref.abs() + (dp + C.E16 ** 2) * av * (1 + C.half_step(BF)), h)
+
+
+def test_cross_attention_backward_passes_do_not_meet(ops):
+    C.backward_case(ops, DEV)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+def test_cross_attention_scores_of_minus_infinity(ops, dtype):
+    C.infinite_scores_case(ops, DEV, dtype)
+
+
+def test_cross_attention_of_more_sequences_than_a_grid_has_rows(ops):
+    """(the single-token kernel has a sequence per grid row, 65535 at most; the other one takes over)"""
+    g = torch.Generator().manual_seed(1)
+    B = 65540
+    q, k, v = (torch.randn(2, t, 1, 8, generator=g).repeat(B // 2, 1, 1, 1) for t in (1, 2, 2))
+    out = ops.cross_attention(q.to(DEV), k.to(DEV), v.to(DEV)).cpu()
+    want = C.cross_ref(q[:2], k[:2], v[:2], None, None, F32)['out']
+    C.check_close(out[:2], want[0], want[1], 'out')
+    assert torch.equal(out, out[:2].repeat(B // 2, 1, 1, 1))
