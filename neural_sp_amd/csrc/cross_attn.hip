@@ -3,8 +3,8 @@
 //   S = scale Q K^T,  P = softmax over the keys j < klens[b],  O = dropout(P) V
 //   dV = dropout(P)^T dO,  dP = dropout'(dO V^T),  D_i = sum_d dO_id O_id,  dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q
 //
-// No score leaves the compute unit.  All three kernels are one loop: a wave owns 16 (NQ x 16) rows whose operands stay in
-// registers, a workgroup of four waves streams tiles of the other side's rows through LDS (LDS-DMA, double buffered, one
+// No score leaves the compute unit.  All three kernels are one loop: a wave owns 16 rows (forward: 16 or 32) whose operands stay in
+// registers, a workgroup of four waves streams tiles of the other side's rows through LDS (LDS-DMA, two or three on their
 // barrier per tile), and the score tile is computed with the OWNED row on the lane's column: row statistics are per lane, and
 // the probabilities already are the operand of the second product -- their contraction runs over the streamed rows, four of
 // which a lane holds per 16.
@@ -18,7 +18,7 @@
 // The softmax is kept as its maximum (log2 domain) and the reciprocal of its sum, both fp32; backward recomputes P from them.
 // bf16 roundings inside: P resp. dS, once each, as operands of the second products; with the outputs' own rounding the results are
 // 1.2 (out) to 1.5 times (dQ) as far from exact as a rounding of the exact result.  (Two bf16 parts for dS bring dQ to 1.2 and cost
-// 36 us of the 417 us of the largest measured call.)  Sums, statistics and D are fp32.
+// 36 us of the 410 us of the largest measured call.)  Sums, statistics and D are fp32.
 // A row without a visible key is uniform over all Tk keys, as with the finite mask value of attn_softmax_fwd, and passes no
 // gradient through its scores.  Keys behind klens are never read.
 #include "attn_frag.h"
@@ -516,9 +516,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
   }
 }
 
-template <typename T, int DP, int NQ, bool DROP>
+template <typename T, int DP, bool DROP>
 __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
+  constexpr int NQ = 1;      // owned 16-query fragments of a wave
   __shared__ __attribute__((aligned(16))) unsigned char lds[X::STAGES * 2 * X::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -666,9 +667,10 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
   }
 }
 
-template <typename T, int DP, int NK, bool DROP>
+template <typename T, int DP, bool DROP>
 __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
   typedef XTile<T, DP> X;
+  constexpr int NK = 1;      // owned 16-key fragments of a wave
   // pairs of tiles, then for each the rows' maxima, reciprocal sums and D (64 each)
   // (two pairs: a fourth workgroup per compute unit is worth more than a third tile, 199 against 210 us)
   constexpr int STAGES = 2, PAIR = 2 * X::BYTES, ROWS = STAGES * PAIR;
@@ -799,36 +801,38 @@ int launch_fwd(const XArgs& p, hipStream_t st) {
   NSP_LAUNCH_CHECK();
   return NSP_OK;
 }
-template <typename T, int DP, int NQ, bool DROP>
+template <typename T, int DP, bool DROP>
 int launch_dq(const XArgs& p, hipStream_t st) {
-  const long long wgs = ((long long)p.B * p.Hkv + 7) / 8 * 8 * (p.H / p.Hkv) * ((p.Tq + 64 * NQ - 1) / (64 * NQ));
+  const long long wgs = ((long long)p.B * p.Hkv + 7) / 8 * 8 * (p.H / p.Hkv) * ((p.Tq + 63) / 64);
   if (wgs > 0x7fffffffLL) return NSP_EUNSUPPORTED;
-  hipLaunchKernelGGL((cross_dq_kernel<T, DP, NQ, DROP>), dim3((unsigned)wgs), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((cross_dq_kernel<T, DP, DROP>), dim3((unsigned)wgs), dim3(256), 0, st, p);
   NSP_LAUNCH_CHECK();
   return NSP_OK;
 }
-template <typename T, int DP, int NK, bool DROP>
+template <typename T, int DP, bool DROP>
 int launch_dkv(const XArgs& p, hipStream_t st) {
-  const long long wgs = ((long long)p.B * p.Hkv + 7) / 8 * 8 * ((p.Tk + 64 * NK - 1) / (64 * NK));
+  const long long wgs = ((long long)p.B * p.Hkv + 7) / 8 * 8 * ((p.Tk + 63) / 64);
   if (wgs > 0x7fffffffLL) return NSP_EUNSUPPORTED;
-  hipLaunchKernelGGL((cross_dkv_kernel<T, DP, NK, DROP>), dim3((unsigned)wgs), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((cross_dkv_kernel<T, DP, DROP>), dim3((unsigned)wgs), dim3(256), 0, st, p);
   NSP_LAUNCH_CHECK();
   return NSP_OK;
 }
 
-// Two owned 16-row fragments per wave halve the tile reads per score.  They pay once the halved number of workgroups still fills
-// the 256 compute units twice (bf16, 128 x 8 heads, 256 x 600..800, d 64: forward 124 -> 104 us, dQ 133 -> 117; 4 x 16 heads, 500 x
-// 2048, d 128, 256 workgroups left: forward 52 -> 61, dQ 63 -> 68).  fp32 spends eight times as long in the matrix cores and keeps
-// one; so does dK / dV, whose two accumulators leave too few registers for a third workgroup (205 us either way, and 9.0 against
-// 10.9 us for 32 x 8 heads, 61 x 90..187).
+// Two owned 16-row fragments per wave halve the tile reads per score.  In the forward kernel they pay once the halved number of
+// workgroups still fills the 256 compute units twice (bf16, 128 x 8 heads, 256 x 800, d 64: 104 -> 85 us; 32 x 16 heads, d 128:
+// 113 -> 87; 4 x 16 heads, 500 x 2048, d 128, 256 workgroups left: 52 -> 61) and while there is no dropout, whose hashes then
+// spill registers (the same calls: 184 -> 236 and 137 -> 187).  fp32 spends eight times as long in the matrix cores and keeps
+// one.  So do dQ and dK / dV, whose accumulators leave too few registers for a third workgroup per compute unit (134 against 132
+// and 205 against 205 us for the first of those calls; dK / dV 9.0 against 10.9 us for 32 x 8 heads, 61 x 90..187).
 template <typename T, int DP, bool DROP>
 int launch(const XArgs& p, bool bwd, hipStream_t st) {
-  constexpr int TWO = sizeof(T) == 2 ? 2 : 1;
-  const bool two = TWO == 2 && p.Tq > 64 && (long long)p.B * p.H * ((p.Tq + 127) / 128) >= 512;
-  if (!bwd) return two ? launch_fwd<T, DP, TWO, DROP>(p, st) : launch_fwd<T, DP, 1, DROP>(p, st);
-  constexpr int TWO_DQ = DP <= 64 ? TWO : 1;      // (its two accumulators of 128 dimensions do not fit twice)
-  const int rc = two ? launch_dq<T, DP, TWO_DQ, DROP>(p, st) : launch_dq<T, DP, 1, DROP>(p, st);
-  return rc != NSP_OK ? rc : launch_dkv<T, DP, 1, DROP>(p, st);
+  if (bwd) {
+    const int rc = launch_dq<T, DP, DROP>(p, st);
+    return rc != NSP_OK ? rc : launch_dkv<T, DP, DROP>(p, st);
+  }
+  if constexpr (sizeof(T) == 2 && !DROP)
+    if (p.Tq > 64 && (long long)p.B * p.H * ((p.Tq + 127) / 128) >= 512) return launch_fwd<T, DP, 2, DROP>(p, st);
+  return launch_fwd<T, DP, 1, DROP>(p, st);
 }
 template <typename T, bool DROP>
 int launch_d(const XArgs& p, bool bwd, hipStream_t st) {
