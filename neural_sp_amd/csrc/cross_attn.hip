@@ -4,7 +4,7 @@
 //   dV = dropout(P)^T dO,  dP = dropout'(dO V^T),  D_i = sum_d dO_id O_id,  dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q
 //
 // No score leaves the compute unit.  All three kernels are one loop: a wave owns 16 rows (forward: 16 or 32) whose operands stay in
-// registers, a workgroup of four waves streams tiles of the other side's rows through LDS (LDS-DMA, two or three on their
+// registers, a workgroup of four waves streams tiles of the other side's rows through LDS (LDS-DMA, two or three pairs, one
 // barrier per tile), and the score tile is computed with the OWNED row on the lane's column: row statistics are per lane, and
 // the probabilities already are the operand of the second product -- their contraction runs over the streamed rows, four of
 // which a lane holds per 16.
