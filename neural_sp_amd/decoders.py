@@ -770,8 +770,9 @@ class TransformerDecoder(DecoderBase):
     def sample(self, eouts, elens, max_len_ratio=1.0, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed=None,
                exclude_eos=False, page_size=16, check_every=8):
         """One hypothesis per utterance drawn token by token from the decoder's distribution (ops.sample_rows: temperature,
-        top_k, top_p, min_p; temperature 0 is the arg-max), at most ceil(T * max_len_ratio) tokens.  Every step works on the
-        newest token alone: self-attention over a paged key / value cache, source attention over keys and values computed once.
+        top_k, top_p, min_p; temperature 0 is the arg-max), at most ceil(T * max_len_ratio) tokens and no more than there are
+        positions in the table of `pe_type` add.  Every step works on the newest token alone: self-attention over a paged key /
+        value cache, source attention over keys and values computed once.
         Source attention sees each utterance's own frames (elens), as in training -- `greedy` attends to the padding as well.
 
         seed: the random numbers (one per utterance and step, drawn on the host) repeat with it; None takes torch's generator.
@@ -788,6 +789,8 @@ class TransformerDecoder(DecoderBase):
         B, T = eouts.shape[:2]
         dtype = torch.bfloat16 if ops.bf16_mode() else torch.float32
         ymax = max(1, int(math.ceil(T * max_len_ratio)))
+        if self.pe_type == 'add':
+            ymax = min(ymax, self.pos_enc.pe.size(1))
         gen = None if seed is None else torch.Generator().manual_seed(int(seed))
         u = ops.h2d(torch.rand((ymax, B), generator=gen, dtype=torch.float32), dev)
         elens_d = ops.h2d(elens, dev, torch.int32)

@@ -76,6 +76,21 @@ def sample_case(dev, settings, seed=5, ratio=1.0, page_size=4, check_every=3):
     return hyps
 
 
+def position_table_case(dev):
+    """no more tokens than there are positions"""
+    model = tiny_model(dev)
+    model.eval()
+    dec = model.dec_fwd
+    assert dec.pe_type == 'add'
+    eouts, elens = states(dev)
+    with torch.no_grad():
+        dec.output.bias[dec.eos] = -1e4           # never ends by itself
+    long, _ = dec.sample(eouts, elens, seed=2)
+    dec.pos_enc.pe = dec.pos_enc.pe[:, :6].contiguous()
+    hyps, _ = dec.sample(eouts, elens, 3.0, seed=2)
+    assert [len(h) for h in long] == [21] * 3 and [h.tolist() for h in hyps] == [h[:6].tolist() for h in long]
+
+
 def decode_case(dev):
     """Speech2Text.decode routes recog_sampling there, and nowhere else without it"""
     from neural_sp_amd.configs import synthetic_batch

@@ -19,6 +19,10 @@ def test_sample_is_what_the_training_path_gives_token_by_token(emu, settings):
     S.sample_case('cpu', settings)
 
 
+def test_sample_ends_with_the_position_table(emu):
+    S.position_table_case('cpu')
+
+
 def test_decode_samples_when_asked(emu):
     S.decode_case('cpu')
 

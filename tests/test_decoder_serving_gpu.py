@@ -28,6 +28,10 @@ def test_sample_in_bf16_mode():
         assert all(0 <= int(t) < 37 for x in a for t in x)
 
 
+def test_sample_ends_with_the_position_table():
+    S.position_table_case('cuda')
+
+
 def test_decode_samples_when_asked():
     S.decode_case('cuda')
 
