@@ -2467,7 +2467,8 @@ def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
     Key j is visible to the queries of row b if j < klens[b] (int32 `[B]`; None: all); a row without a visible key averages
     all Tk values and passes no gradient through its scores, as AttentionFn does with its finite mask.  What lies behind
     klens[b] in k and v is not read.  scale > 0, d^-1/2 by default.  dropout_p: dropout of the probabilities with a mask of its
-    own site (next_dropout_seed), regenerated in backward.
+    own site (next_dropout_seed), regenerated in backward; a captured call repeats its mask with every replay.  A backward pass is
+    captured on leaves of its own (detached ones): an eager graph that is alive ties its leaves to the stream it ran on.
 
     Without gradients and dropout, calls of up to 16 query rows per key head (Tq * H / Hkv) take the kernel that splits the
     keys over workgroups: the single-token form of decoding."""
