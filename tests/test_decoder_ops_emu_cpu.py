@@ -10,6 +10,16 @@ pytestmark = pytest.mark.skipif(not build_emu.available(), reason='no host clang
 BF, F32 = torch.bfloat16, torch.float32
 
 
+@pytest.fixture(autouse=True)
+def random_state_of_the_process():
+    """the tests behind these draw the numbers and the dropout masks that they draw without them"""
+    from neural_sp_amd import ops
+    was = dict(ops._DROPOUT_STATE)
+    with torch.random.fork_rng():
+        yield
+    ops._DROPOUT_STATE.update(was)
+
+
 @pytest.fixture
 def emu():
     from neural_sp_amd import ops

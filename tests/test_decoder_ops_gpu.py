@@ -10,6 +10,16 @@ BF, F32 = torch.bfloat16, torch.float32
 DEV = 'cuda'
 
 
+@pytest.fixture(autouse=True)
+def random_state_of_the_process():
+    """the tests behind these draw the numbers and the dropout masks that they draw without them"""
+    from neural_sp_amd import ops
+    was = dict(ops._DROPOUT_STATE)
+    with torch.random.fork_rng():
+        yield
+    ops._DROPOUT_STATE.update(was)
+
+
 @pytest.fixture
 def ops():
     from neural_sp_amd import ops

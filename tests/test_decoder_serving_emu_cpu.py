@@ -1,10 +1,21 @@
 """Cached decoding and the fused source attention through the model, on the host emulator of the kernels."""
 import pytest
+import torch
 
 from tests import decoder_serving_common as S
 from tests.hipemu import build_emu
 
 pytestmark = pytest.mark.skipif(not build_emu.available(), reason='no host clang++ for the HIP emulator')
+
+
+@pytest.fixture(autouse=True)
+def random_state_of_the_process():
+    """the tests behind these draw the numbers and the dropout masks that they draw without them"""
+    from neural_sp_amd import ops
+    was = dict(ops._DROPOUT_STATE)
+    with torch.random.fork_rng():
+        yield
+    ops._DROPOUT_STATE.update(was)
 
 
 @pytest.fixture

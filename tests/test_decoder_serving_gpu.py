@@ -7,6 +7,16 @@ from tests import decoder_serving_common as S
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def random_state_of_the_process():
+    """the tests behind these draw the numbers and the dropout masks that they draw without them"""
+    from neural_sp_amd import ops
+    was = dict(ops._DROPOUT_STATE)
+    with torch.random.fork_rng():
+        yield
+    ops._DROPOUT_STATE.update(was)
+
+
 @pytest.mark.parametrize('settings', [dict(temperature=0.0), dict(), dict(temperature=0.8, top_k=7, top_p=0.9, min_p=0.01)], ids=str)
 def test_sample_is_what_the_training_path_gives_token_by_token(settings):
     from neural_sp_amd import ops
