@@ -66,40 +66,46 @@ struct XTile {
 };
 
 // where a workgroup's tiles come from: a uniform address per tile and 32-bit offsets per lane that stay (strides below 2^24
-// elements), so that the requests of a tile cost no vector arithmetic
+// elements), so that the requests of a tile cost no vector arithmetic.  What a tile has and the source has not (chunks behind a
+// head size below DP) is read from 16 bytes of zeros: the owned operand is 0 there as well, and 0 times a copy of another
+// element would be NaN where that is infinite.  Every lane takes part in every request, so their number per wave stays the same.
+__device__ const nsp_u32x4 x_zeros = {0u, 0u, 0u, 0u};
 template <typename T, int DP>
 struct XSource {
   typedef XTile<T, DP> X;
   static constexpr int P = X::BYTES / 4096;          // instructions (1 KB each) of a wave
   const unsigned char* base;
   unsigned ldb, off[P];
-  int wave, lane;
-  __device__ __forceinline__ unsigned chunk_byte(int i, int chunks) const {
-    const int row = (wave * P + i) * (64 / X::CPR) + lane / X::CPR;
-    return (unsigned)min(lane % X::CPR ^ X::swz(row), chunks - 1) * 16u;      // (head sizes below DP: the owned operand is 0 there)
-  }
-  __device__ __forceinline__ int row_of(int i) const { return (wave * P + i) * (64 / X::CPR) + lane / X::CPR; }
-  __device__ __forceinline__ void init(const T* src, long long ld, int chunks, int wave_, int lane_) {
+  int wave, lane, chunks;      // (chunks of a source row)
+  __device__ __forceinline__ int row_of(int i, int l) const { return (wave * P + i) * (64 / X::CPR) + l / X::CPR; }
+  __device__ __forceinline__ int chunk_of(int i, int l) const { return l % X::CPR ^ X::swz(row_of(i, l)); }
+  __device__ __forceinline__ void init(const T* src, long long ld, int chunks_, int wave_, int lane_) {
     base = reinterpret_cast<const unsigned char*>(src);
     ldb = (unsigned)ld * (unsigned)sizeof(T);
     wave = wave_;
     lane = lane_;
+    chunks = chunks_;
 #pragma unroll
-    for (int i = 0; i < P; ++i) off[i] = (unsigned)row_of(i) * ldb + chunk_byte(i, chunks);
+    for (int i = 0; i < P; ++i) off[i] = (unsigned)row_of(i, lane) * ldb + (unsigned)chunk_of(i, lane) * 16u;
   }
   // rows row0 .. row0 + KT - 1 into LDS; rows from `limit` (> row0) on re-read the last one
   __device__ __forceinline__ void request(unsigned char* tile, long long skip, int row0, int limit) const {
     const unsigned char* at = base + skip + (long long)row0 * ldb;
-    if (row0 + X::KT <= limit) {
+    if (row0 + X::KT <= limit && chunks == X::CPR) {
 #pragma unroll
       for (int i = 0; i < P; ++i)
         __builtin_amdgcn_global_load_lds((x_glb_void*)(at + off[i]), (x_lds_void*)(tile + (wave * P + i) * 1024), 16, 0, 0);
     } else {
+      int l = lane;
+#ifndef NSP_HOST_EMULATION
+      asm volatile("" : "+v"(l));      // (computed here: held over the loop it would cost a dozen registers)
+#endif
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const int row = row_of(i);
-        const unsigned back = (unsigned)(row - min(row, limit - 1 - row0)) * ldb;
-        __builtin_amdgcn_global_load_lds((x_glb_void*)(at + (off[i] - back)), (x_lds_void*)(tile + (wave * P + i) * 1024), 16, 0, 0);
+        const int row = min(row_of(i, l), limit - 1 - row0), chunk = chunk_of(i, l);
+        const unsigned char* from = at + ((unsigned)row * ldb + (unsigned)chunk * 16u);
+        if (chunk >= chunks) from = reinterpret_cast<const unsigned char*>(&x_zeros);
+        __builtin_amdgcn_global_load_lds((x_glb_void*)from, (x_lds_void*)(tile + (wave * P + i) * 1024), 16, 0, 0);
       }
     }
   }

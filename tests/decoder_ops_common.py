@@ -435,3 +435,17 @@ def infinite_scores_case(ops, dev, dtype):
     want = cross_ref(q[:, :, :, :], k[:, 130:], v[:, 130:], None, None, dtype)['out']
     for grad in (True, False):
         check_close(ops.cross_attention(q.to(dev).requires_grad_(grad), k.to(dev), v.to(dev)).detach(), want[0], want[1], 'out')
+
+
+def infinite_scores_in_the_last_dimension_case(ops, dev, dtype, D):
+    """the same for head sizes between the kernels' widths, where the last dimension's chunk borders on what is not there"""
+    g = torch.Generator().manual_seed(D)
+    q, k, v = torch.randn(1, 70, 2, D, generator=g), torch.randn(1, 150, 1, D, generator=g), torch.randn(1, 150, 1, D, generator=g)
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    q[..., -1] = 1.0
+    k[:, :130, :, -1] = float('-inf')
+    want = cross_ref(q, k[:, 130:], v[:, 130:], None, None, dtype)['out']
+    for rows in (70, 3):
+        for grad in (True, False):
+            out = ops.cross_attention(q[:, :rows].to(dev).requires_grad_(grad), k.to(dev), v.to(dev)).detach()
+            check_close(out, want[0][:, :rows], want[1][:, :rows], 'out')

@@ -233,3 +233,9 @@ def test_refusals_of_memory_and_settings(emu):
                 lambda: emu.cross_attention(c, c, c, dropout_p=torch.tensor(0.5))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize('D', [8, 40, 72, 96])
+@pytest.mark.parametrize('dtype', [BF, F32])
+def test_cross_attention_scores_of_minus_infinity_by_the_last_dimension(emu, dtype, D):
+    C.infinite_scores_in_the_last_dimension_case(emu, 'cpu', dtype, D)

@@ -272,3 +272,9 @@ def test_cross_attention_of_more_sequences_than_a_grid_has_rows(ops):
     want = C.cross_ref(q[:2], k[:2], v[:2], None, None, F32)['out']
     C.check_close(out[:2], want[0], want[1], 'out')
     assert torch.equal(out, out[:2].repeat(B // 2, 1, 1, 1))
+
+
+@pytest.mark.parametrize('D', [8, 40, 72, 96])
+@pytest.mark.parametrize('dtype', [BF, F32])
+def test_cross_attention_scores_of_minus_infinity_by_the_last_dimension(ops, dtype, D):
+    C.infinite_scores_in_the_last_dimension_case(ops, DEV, dtype, D)
