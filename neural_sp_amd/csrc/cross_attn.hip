@@ -67,8 +67,9 @@ struct XTile {
 
 // where a workgroup's tiles come from: a uniform address per tile and 32-bit offsets per lane that stay (strides below 2^24
 // elements), so that the requests of a tile cost no vector arithmetic.  What a tile has and the source has not (chunks behind a
-// head size below DP) is read from 16 bytes of zeros: the owned operand is 0 there as well, and 0 times a copy of another
-// element would be NaN where that is infinite.  Every lane takes part in every request, so their number per wave stays the same.
+// head size below DP, rows behind the last) is read from 16 bytes of zeros: the other operand is 0 there as well, and 0 times a
+// copy of another element would be NaN where that is infinite.  Every lane takes part in every request, so their number per wave
+// stays the same.
 __device__ const nsp_u32x4 x_zeros = {0u, 0u, 0u, 0u};
 template <typename T, int DP>
 struct XSource {
@@ -88,7 +89,8 @@ struct XSource {
 #pragma unroll
     for (int i = 0; i < P; ++i) off[i] = (unsigned)row_of(i, lane) * ldb + (unsigned)chunk_of(i, lane) * 16u;
   }
-  // rows row0 .. row0 + KT - 1 into LDS; rows from `limit` (> row0) on re-read the last one
+  // rows row0 .. row0 + KT - 1 into LDS; rows from `limit` (> row0) on are zeros, or (AGAIN) the last one again
+  template <bool AGAIN>
   __device__ __forceinline__ void request(unsigned char* tile, long long skip, int row0, int limit) const {
     const unsigned char* at = base + skip + (long long)row0 * ldb;
     if (row0 + X::KT <= limit && chunks == X::CPR) {
@@ -102,9 +104,9 @@ struct XSource {
 #endif
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const int row = min(row_of(i, l), limit - 1 - row0), chunk = chunk_of(i, l);
-        const unsigned char* from = at + ((unsigned)row * ldb + (unsigned)chunk * 16u);
-        if (chunk >= chunks) from = reinterpret_cast<const unsigned char*>(&x_zeros);
+        const int last = limit - 1 - row0, row = row_of(i, l), chunk = chunk_of(i, l);
+        const unsigned char* from = at + ((unsigned)min(row, last) * ldb + (unsigned)chunk * 16u);
+        if (chunk >= chunks || (!AGAIN && row > last)) from = reinterpret_cast<const unsigned char*>(&x_zeros);
         __builtin_amdgcn_global_load_lds((x_glb_void*)from, (x_lds_void*)(tile + (wave * P + i) * 1024), 16, 0, 0);
       }
     }
@@ -419,8 +421,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void cross_fwd_kernel(const 
   const int nkt = (klen + X::KT - 1) / X::KT;
   constexpr int PAIR = 2 * X::BYTES, AHEAD = X::STAGES - 1, NEWER = (AHEAD - 1) * 2 * XSource<T, DP>::P;
   auto fetch = [&](int at, int kt) {
-    ks.request(lds + at, 0, kt * X::KT, klen);
-    vs.request(lds + at + X::BYTES, 0, kt * X::KT, klen);
+    ks.template request<false>(lds + at, 0, kt * X::KT, klen);
+    vs.template request<false>(lds + at + X::BYTES, 0, kt * X::KT, klen);
   };
   fetch(0, 0);
   if (AHEAD > 1 && nkt > 1) fetch(PAIR, 1);
@@ -552,8 +554,8 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(const XArgs p) {
   vs.init(vb, p.v_st, chunks, wave, lane);
   constexpr int PAIR = 2 * X::BYTES, AHEAD = X::STAGES - 1, NEWER = (AHEAD - 1) * 2 * XSource<T, DP>::P;
   auto fetch = [&](int at, int kt) {
-    ks.request(lds + at, 0, kt * X::KT, klen);
-    vs.request(lds + at + X::BYTES, 0, kt * X::KT, klen);
+    ks.template request<false>(lds + at, 0, kt * X::KT, klen);
+    vs.template request<false>(lds + at + X::BYTES, 0, kt * X::KT, klen);
   };
   if (nkt > 0) fetch(0, 0);
   typename X::E::chunk Q[NQ][X::NS], dO[NQ][X::NS];
@@ -712,8 +714,9 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
     gs.init(gb, p.g_st, chunks, wave, lane);
     auto fetch = [&](int buf, int it) {
       const int hq = it / nqt, row0 = (it % nqt) * X::KT;
-      qs.request(lds + buf * PAIR, (long long)hq * p.q_sh * (long long)sizeof(T), row0, p.Tq);
-      gs.request(lds + buf * PAIR + X::BYTES, (long long)hq * p.g_sh * (long long)sizeof(T), row0, p.Tq);
+      // (scores of the rows behind the last query are taken from -inf; 0 as their query would be NaN against a key of -inf)
+      qs.template request<true>(lds + buf * PAIR, (long long)hq * p.q_sh * (long long)sizeof(T), row0, p.Tq);
+      gs.template request<false>(lds + buf * PAIR + X::BYTES, (long long)hq * p.g_sh * (long long)sizeof(T), row0, p.Tq);
       if (wave < 3)      // one of the three per wave
         __builtin_amdgcn_global_load_lds((x_glb_void*)(rows + (long long)hq * pitch + min(row0 + lane, pitch - 1)),
                                          (x_lds_void*)(lds + ROWS + buf * 1024 + wave * 256), 4, 0, 0);

@@ -449,3 +449,33 @@ def infinite_scores_in_the_last_dimension_case(ops, dev, dtype, D):
         for grad in (True, False):
             out = ops.cross_attention(q[:, :rows].to(dev).requires_grad_(grad), k.to(dev), v.to(dev)).detach()
             check_close(out, want[0][:, :rows], want[1][:, :rows], 'out')
+
+
+def check_close_but_for_infinities(got, ref, tol, what):
+    """infinities where the reference has them, and only there"""
+    got, far = got.detach().double().cpu(), torch.isinf(ref)
+    assert far.any() and torch.equal(got[far], ref[far]), what
+    check_close(got[~far], ref[~far], tol[~far], what)
+
+
+def infinite_last_row_case(ops, dev, dtype, D, Tq, Tk, klens, train=True):
+    """an infinite value in the last visible row of v, and an infinite gradient of the last query: the sums they enter are
+    infinite, by the definition"""
+    g = torch.Generator().manual_seed(Tk)
+    B = len(klens)
+    q, k, v, dout = (torch.randn(B, t, 2, D, generator=g).to(dtype) for t in (Tq, Tk, Tk, Tq))
+    inf_v, inf_d = v.clone(), dout.clone()
+    for b, n in enumerate(klens):
+        inf_v[b, n - 1, :, 5] = float('inf')
+        inf_d[b, Tq - 1, :, D - 1] = float('-inf')
+    lens = torch.tensor(klens, dtype=torch.int32).to(dev)
+    ref = cross_ref(q, k, inf_v, None, klens, dtype)['out']
+    check_close_but_for_infinities(ops.cross_attention(q.to(dev).requires_grad_(train), k.to(dev), inf_v.to(dev), lens), *ref, 'out')
+    if train:
+        ref, vd = cross_ref(q, k, v, inf_d, klens, dtype)['dv'], v.to(dev).requires_grad_()
+        got = torch.autograd.grad(ops.cross_attention(q.to(dev), k.to(dev), vd, lens), vd, inf_d.to(dev))[0]
+        check_close_but_for_infinities(got, *ref, 'dv')
+
+
+INFINITE_LAST_ROW = [dict(D=64, Tq=70, Tk=150, klens=[150, 33]), dict(D=72, Tq=37, Tk=50, klens=[50]),
+                     dict(D=32, Tq=5, Tk=33, klens=[1, 33, 32])]

@@ -239,3 +239,9 @@ def test_refusals_of_memory_and_settings(emu):
 @pytest.mark.parametrize('dtype', [BF, F32])
 def test_cross_attention_scores_of_minus_infinity_by_the_last_dimension(emu, dtype, D):
     C.infinite_scores_in_the_last_dimension_case(emu, 'cpu', dtype, D)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('a', C.INFINITE_LAST_ROW, ids=str)
+def test_cross_attention_of_an_infinite_last_row(emu, dtype, a):
+    C.infinite_last_row_case(emu, 'cpu', dtype, **a)

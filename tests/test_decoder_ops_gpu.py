@@ -278,3 +278,9 @@ def test_cross_attention_of_more_sequences_than_a_grid_has_rows(ops):
 @pytest.mark.parametrize('dtype', [BF, F32])
 def test_cross_attention_scores_of_minus_infinity_by_the_last_dimension(ops, dtype, D):
     C.infinite_scores_in_the_last_dimension_case(ops, DEV, dtype, D)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('a', C.INFINITE_LAST_ROW, ids=str)
+def test_cross_attention_of_an_infinite_last_row(ops, dtype, a):
+    C.infinite_last_row_case(ops, DEV, dtype, **a)
