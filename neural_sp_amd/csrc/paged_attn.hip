@@ -14,8 +14,9 @@
 // probabilities already are the operand of O^T = V^T P^T.  Keys and values go from memory into the operands' registers, the
 // next tile's while this one is worked on; a value operand wants eight KEYS of one dimension per lane where memory has
 // dimensions side by side, so a lane loads d / 16 dimensions of its eight keys and transposes 8 x d / 16 in registers.
-// Probabilities enter the product as bf16 high + low parts (17 bits): the matrix cores are idle enough that the second
-// product is free, and the result's only rounding to bf16 is the last one.
+// Probabilities enter the product as bf16 high + low parts (16 bits): the matrix cores are idle enough that the second
+// product is free, and the result's only rounding to bf16 is the last one.  Both parts are positive where the probability is, so
+// that an infinite value stays one: the high part is cut off below the probability, and a low part of zero is 2^-24 of it.
 #include "attn_frag.h"
 
 namespace {
@@ -100,9 +101,9 @@ __device__ __forceinline__ void value_product(f32x4 (&o)[VW], const ValueRow<__b
   bf16x8 hi, lo;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float x = pr[i >> 2][i & 3];
-    hi[i] = (__bf16)x;
-    lo[i] = (__bf16)(x - (float)hi[i]);
+    const float x = pr[i >> 2][i & 3], h = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    hi[i] = (__bf16)h;
+    lo[i] = (__bf16)fmaxf(x - h, x * 5.9604644775390625e-8f);
   }
 #pragma unroll
   for (int w = 0; w < VW / 2; ++w) {
@@ -299,6 +300,11 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
       }
 #pragma unroll
     for (int j = 0; j < VW; ++j) o[j] *= alpha;
+    if (j0 + 32 > end) {      // what was loaded for keys behind the end: 0 x an infinite last value would be NaN
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (j0 + 16 * (i >> 2) + 4 * g + (i & 3) >= end) cur.v[i].clear();
+    }
     value_product<VW>(o, cur.v, pr);
     cur = nxt;
     j0 = jn;

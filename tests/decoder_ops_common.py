@@ -479,3 +479,30 @@ def infinite_last_row_case(ops, dev, dtype, D, Tq, Tk, klens, train=True):
 
 INFINITE_LAST_ROW = [dict(D=64, Tq=70, Tk=150, klens=[150, 33]), dict(D=72, Tq=37, Tk=50, klens=[50]),
                      dict(D=32, Tq=5, Tk=33, klens=[1, 33, 32])]
+
+
+def infinite_values_paged_case(ops, dev, dtype, D, page, n):
+    """infinite values of an inner key and of the last one (behind which a tile is partly empty): the sums they enter are
+    infinite, whatever the parts a probability is split into"""
+    g = torch.Generator().manual_seed(n)
+    width = (n + page - 1) // page
+    k, v = (torch.randn(n, 2, D, generator=g).to(dtype) for _ in range(2))
+    v[n // 3, :, 1] = float('inf')
+    v[n - 1, :, D - 2] = float('-inf')
+    kp, vp = (torch.full((width, 2, page, D), float('nan'), dtype=dtype) for _ in range(2))
+    table = torch.randperm(width, generator=g).to(torch.int32).view(1, width)
+    for j in range(n):
+        put(kp, table, 0, j, page, k[j])
+        put(vp, table, 0, j, page, v[j])
+    q = torch.randn(1, 4, D, generator=g).to(dtype)
+    lens = torch.tensor([n], dtype=torch.int32).to(dev)
+    paged = ops.paged_attention(q.to(dev), kp.to(dev), vp.to(dev), table.to(dev), lens)[0]
+    plain = ops.cross_attention(q.to(dev).unsqueeze(1), k.to(dev).unsqueeze(0), v.to(dev).unsqueeze(0))[0, 0]
+    split = E16 * E16 if dtype == torch.bfloat16 else 0.0
+    for out in (paged, plain):
+        for h in range(2):
+            ref, dp, av = attention_ref(q[0, 2 * h:2 * h + 2], k[:, h], v[:, h], n)
+            check_close_but_for_infinities(out[2 * h:2 * h + 2], ref, half_step(dtype) * ref.abs() + (dp + split) * av * (1 + half_step(dtype)), h)
+
+
+INFINITE_VALUES = [dict(D=64, page=16, n=37), dict(D=128, page=64, n=700), dict(D=40, page=7, n=50), dict(D=32, page=16, n=2)]

@@ -284,3 +284,9 @@ def test_cross_attention_scores_of_minus_infinity_by_the_last_dimension(ops, dty
 @pytest.mark.parametrize('a', C.INFINITE_LAST_ROW, ids=str)
 def test_cross_attention_of_an_infinite_last_row(ops, dtype, a):
     C.infinite_last_row_case(ops, DEV, dtype, **a)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('a', C.INFINITE_VALUES, ids=str)
+def test_decoding_with_infinite_values(ops, dtype, a):
+    C.infinite_values_paged_case(ops, DEV, dtype, **a)
