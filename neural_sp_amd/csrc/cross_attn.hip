@@ -102,11 +102,13 @@ struct XSource {
 #ifndef NSP_HOST_EMULATION
       asm volatile("" : "+v"(l));      // (computed here: held over the loop it would cost a dozen registers)
 #endif
+      const int last = limit - 1 - row0;
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const int last = limit - 1 - row0, row = row_of(i, l), chunk = chunk_of(i, l);
-        const unsigned char* from = at + ((unsigned)min(row, last) * ldb + (unsigned)chunk * 16u);
-        if (chunk >= chunks || (!AGAIN && row > last)) from = reinterpret_cast<const unsigned char*>(&x_zeros);
+        const int chunk = chunk_of(i, l);
+        const bool behind = row_of(i, l) > last;
+        const unsigned char* from = at + (AGAIN && behind ? (unsigned)last * ldb + (unsigned)chunk * 16u : off[i]);
+        if (chunk >= chunks || (!AGAIN && behind)) from = reinterpret_cast<const unsigned char*>(&x_zeros);
         __builtin_amdgcn_global_load_lds((x_glb_void*)from, (x_lds_void*)(tile + (wave * P + i) * 1024), 16, 0, 0);
       }
     }
