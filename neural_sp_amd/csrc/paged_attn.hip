@@ -17,6 +17,9 @@
 // Probabilities enter the product as bf16 high + low parts (16 bits): the matrix cores are idle enough that the second
 // product is free, and the result's only rounding to bf16 is the last one.  Both parts are positive where the probability is, so
 // that an infinite value stays one: the high part is cut off below the probability, and a low part of zero is 2^-24 of it.
+//
+// Scores of -inf alone have no softmax.  Over states the result is NaN, as the training kernel and the definition have it; over
+// a cache such a row is one whose keys are all absent: zeros.
 #include "attn_frag.h"
 
 namespace {
@@ -370,7 +373,7 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
   const int rr = row0 + q;
   if (p.nsplit == 1) {
     T* dst = reinterpret_cast<T*>(p.out) + (((long long)b * p.Tq + rr / G) * p.H + hkv * G + rr % G) * p.D;
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);     // no key at all: zeros; a NaN stays one
+    const float inv = MODE != CONTIG && L == 0.f ? 0.f : 1.f / L;     // no key at all: zeros (over states L = 0 is not that)
 #pragma unroll
     for (int j = 0; j < VW; ++j)
       if (d0 + j < p.D) dst[d0 + j] = E::from_f32(acc[j] * inv);
@@ -435,7 +438,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeArgs p) {
     }
     if (s0 + N >= ns) break;
   }
-  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  const float inv = PAGED && L == 0.f ? 0.f : 1.f / L;
   T* out = reinterpret_cast<T*>(p.out) + (((long long)b * p.Tq + rr / G) * p.H + hkv * G + rr % G) * p.D;
 #pragma unroll
   for (int j = 0; j < VW; ++j)

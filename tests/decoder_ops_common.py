@@ -506,3 +506,15 @@ def infinite_values_paged_case(ops, dev, dtype, D, page, n):
 
 
 INFINITE_VALUES = [dict(D=64, page=16, n=37), dict(D=128, page=64, n=700), dict(D=40, page=7, n=50), dict(D=32, page=16, n=2)]
+
+
+def no_softmax_case(ops, dev, dtype, Tk):
+    """every score of a row -inf: NaN in both forms, and only there"""
+    g = torch.Generator().manual_seed(Tk)
+    q, k, v = (torch.randn(2, t, 2, 32, generator=g).to(dtype) for t in (3, Tk, Tk))
+    q[:, :, :, 0] = 1.0
+    k[1, :, 1, 0] = float('-inf')
+    for grad in (True, False):
+        out = ops.cross_attention(q.to(dev).requires_grad_(grad), k.to(dev), v.to(dev)).detach().cpu()
+        assert out[1, :, 1].isnan().all()
+        assert torch.isfinite(out[0]).all() and torch.isfinite(out[1, :, 0]).all()

@@ -251,3 +251,9 @@ def test_cross_attention_of_an_infinite_last_row(emu, dtype, a):
 @pytest.mark.parametrize('a', C.INFINITE_VALUES, ids=str)
 def test_decoding_with_infinite_values(emu, dtype, a):
     C.infinite_values_paged_case(emu, 'cpu', dtype, **a)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('Tk', [40, 1300])
+def test_cross_attention_of_a_row_without_a_softmax(emu, dtype, Tk):
+    C.no_softmax_case(emu, 'cpu', dtype, Tk)
