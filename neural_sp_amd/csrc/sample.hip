@@ -56,9 +56,9 @@ __device__ __forceinline__ void sample_load4(const __bf16* p, float (&y)[4]) {
   for (int j = 0; j < 4; ++j) y[j] = __uint_as_float((unsigned)v[j] << 16);
 }
 
-// order-preserving image of a logit (-0 counts as 0; a NaN is below everything), and of an entry: larger = earlier
+// order-preserving image of a logit (-0 counts as 0, a NaN as -inf), and of an entry: larger = earlier
 __device__ __forceinline__ unsigned sample_key(float x) {
-  if (x != x) return 0u;
+  if (x != x) return 0x007FFFFFu;
   const unsigned b = __float_as_uint(x + 0.f);
   return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }

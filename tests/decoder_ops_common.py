@@ -518,3 +518,17 @@ def no_softmax_case(ops, dev, dtype, Tk):
         out = ops.cross_attention(q.to(dev).requires_grad_(grad), k.to(dev), v.to(dev)).detach().cpu()
         assert out[1, :, 1].isnan().all()
         assert torch.isfinite(out[0]).all() and torch.isfinite(out[1, :, 0]).all()
+
+
+def nan_among_minus_infinities_case(ops, dev, V):
+    """a NaN counts as -inf, also against -inf: rows without a larger logit give their first entry, others are not disturbed"""
+    inf, nan = float('inf'), float('nan')
+    x = torch.full((5, V), -inf)
+    x[0, 0] = nan
+    x[1, 1:] = nan
+    x[2, ::2] = nan
+    x[3, V - 1] = nan
+    x[4, ::2] = nan
+    x[4, V - 2:] = 1.0
+    for kw in (dict(), dict(t=0.0), dict(k=2), dict(tp=0.9), dict(k=V - 1, tp=0.5)):
+        sample_case(ops, dev, x, [0.0, 0.3, 0.5, 0.7, 0.9], **kw)

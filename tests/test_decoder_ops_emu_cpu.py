@@ -257,3 +257,8 @@ def test_decoding_with_infinite_values(emu, dtype, a):
 @pytest.mark.parametrize('Tk', [40, 1300])
 def test_cross_attention_of_a_row_without_a_softmax(emu, dtype, Tk):
     C.no_softmax_case(emu, 'cpu', dtype, Tk)
+
+
+@pytest.mark.parametrize('V', [3, 700, 12000, 33000])
+def test_sample_rows_of_nan_among_minus_infinities(emu, V):
+    C.nan_among_minus_infinities_case(emu, 'cpu', V)

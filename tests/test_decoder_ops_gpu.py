@@ -296,3 +296,8 @@ def test_decoding_with_infinite_values(ops, dtype, a):
 @pytest.mark.parametrize('Tk', [40, 1300])
 def test_cross_attention_of_a_row_without_a_softmax(ops, dtype, Tk):
     C.no_softmax_case(ops, DEV, dtype, Tk)
+
+
+@pytest.mark.parametrize('V', [3, 700, 12000, 33000])
+def test_sample_rows_of_nan_among_minus_infinities(ops, V):
+    C.nan_among_minus_infinities_case(ops, DEV, V)
