@@ -11,6 +11,7 @@ import os
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from neural_sp_amd import _lib
@@ -2244,6 +2245,12 @@ def _need_aligned(*pages):
             raise ValueError('pages: 16-byte aligned memory expected')
 
 
+def _have_tangents(*tensors):
+    """is one of them a dual tensor of forward-mode differentiation (nodes refuse these; a kernel would drop the tangent)"""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _decode_tail(B, H, Hkv, D, Tq, page, n_pages, width, dtype, qs, ks, vs, ns, scale):
     """-> (constant part of nsp_decode_attn_params, workspace floats)"""
     nb = _lib.lib().nsp_decode_attn_workspace_bytes(B, H, Hkv, Tq, D, width * page)
@@ -2482,7 +2489,7 @@ def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
     qa, ka, va = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if not as_is or (qa | ka | va) & 15:
         return cross_attention(_vec(q), _vec(k), _vec(v), klens if klens is None else klens.contiguous(), scale, dropout_p)
-    need = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
+    need = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled() or _have_tangents(q, k, v)
     if one is not None and not need:
         out = q.new_empty(q.shape)
         ws = q.new_empty((floats,), dtype=torch.float32) if floats else None

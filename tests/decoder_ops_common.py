@@ -532,3 +532,17 @@ def nan_among_minus_infinities_case(ops, dev, V):
     x[4, V - 2:] = 1.0
     for kw in (dict(), dict(t=0.0), dict(k=2), dict(tp=0.9), dict(k=V - 1, tp=0.5)):
         sample_case(ops, dev, x, [0.0, 0.3, 0.5, 0.7, 0.9], **kw)
+
+
+def forward_mode_case(ops, dev, tokens, dropout_p=0.0):
+    """dual tensors are refused, whichever kernel would take the call; duals of another level's end and plain tensors are not"""
+    import torch.autograd.forward_ad as fw
+    x = [torch.ones(1, t, 2, 16).to(dev) for t in (tokens, 9, 9)]
+    with fw.dual_level():
+        for i in range(3):
+            y = list(x)
+            y[i] = fw.make_dual(y[i], torch.ones_like(y[i]))
+            with pytest.raises(NotImplementedError):
+                ops.cross_attention(*y, dropout_p=dropout_p)
+        assert ops.cross_attention(*x, dropout_p=dropout_p).shape == x[0].shape
+    assert ops.cross_attention(*y, dropout_p=dropout_p).shape == x[0].shape

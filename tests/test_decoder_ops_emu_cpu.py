@@ -262,3 +262,9 @@ def test_cross_attention_of_a_row_without_a_softmax(emu, dtype, Tk):
 @pytest.mark.parametrize('V', [3, 700, 12000, 33000])
 def test_sample_rows_of_nan_among_minus_infinities(emu, V):
     C.nan_among_minus_infinities_case(emu, 'cpu', V)
+
+
+@pytest.mark.parametrize('tokens', [1, 40])
+def test_cross_attention_of_dual_tensors(emu, tokens):
+    C.forward_mode_case(emu, 'cpu', tokens)
+    C.forward_mode_case(emu, 'cpu', tokens, 0.1)

@@ -301,3 +301,9 @@ def test_cross_attention_of_a_row_without_a_softmax(ops, dtype, Tk):
 @pytest.mark.parametrize('V', [3, 700, 12000, 33000])
 def test_sample_rows_of_nan_among_minus_infinities(ops, V):
     C.nan_among_minus_infinities_case(ops, DEV, V)
+
+
+@pytest.mark.parametrize('tokens', [1, 40])
+def test_cross_attention_of_dual_tensors(ops, tokens):
+    C.forward_mode_case(ops, DEV, tokens)
+    C.forward_mode_case(ops, DEV, tokens, 0.1)
