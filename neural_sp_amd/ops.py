@@ -2251,6 +2251,20 @@ def _have_tangents(*tensors):
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+class _InferenceOnlyFn(torch.autograd.Function):
+    """out as what the operator `name` made of the tensors behind it, with no way back to them: a gradient that arrives here is an
+    error, not silence"""
+
+    @staticmethod
+    def forward(ctx, name, out, *tensors):
+        ctx.name = name
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise NotImplementedError('%s has no backward pass' % ctx.name)
+
+
 def _decode_tail(B, H, Hkv, D, Tq, page, n_pages, width, dtype, qs, ks, vs, ns, scale):
     """-> (constant part of nsp_decode_attn_params, workspace floats)"""
     nb = _lib.lib().nsp_decode_attn_workspace_bytes(B, H, Hkv, Tq, D, width * page)
@@ -2291,7 +2305,8 @@ def _paged_plan(q, k_pages, v_pages, block_table, lens, k_new, v_new, scale):
 
 
 def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=None, scale=None):
-    """Attention of one new token per sequence over a paged key / value cache (inference, no autograd).
+    """Attention of one new token per sequence over a paged key / value cache (inference: a gradient that reaches the result is an
+    error, and so are dual tensors).
 
     q `[B,H,d]`; k_pages / v_pages `[n_pages,Hkv,page,d]` (any strides with a contiguous last dimension; H a multiple of
     Hkv: query head h reads key head h // (H / Hkv)); block_table int32 `[B,pages]`: page of positions page*i ..; lens int32
@@ -2320,8 +2335,13 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
                lens.stride(), lens.dtype, scale, k_new.shape, k_new.stride(), k_new.dtype, v_new.shape, v_new.stride(), v_new.dtype)
         kn, vn = k_new.data_ptr(), v_new.data_ptr()
     how, tail, ws_floats = _PLANS.get(key) or _plan(key, _paged_plan, q, k_pages, v_pages, block_table, lens, k_new, v_new, scale)
+    if _have_tangents(q, k_pages, v_pages, k_new, v_new):
+        raise NotImplementedError('paged_attention of dual tensors')
+    grad = torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (
+        k_new is not None and (k_new.requires_grad or v_new.requires_grad)))
     if how == 'zeros':
-        return torch.zeros(q.shape, device=q.device, dtype=q.dtype)
+        out = torch.zeros(q.shape, device=q.device, dtype=q.dtype)
+        return _InferenceOnlyFn.apply('paged_attention', out, q, k_pages, v_pages, k_new, v_new) if grad else out
     qa, ka, va = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
     if kn and ka == va:
         raise ValueError('k_pages and v_pages are the same memory')
@@ -2333,7 +2353,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
     ws = q.new_empty((ws_floats,), dtype=torch.float32) if ws_floats else None
     _call('nsp_decode_attn', dev, _DECODE_PTRS(
         qa, out.data_ptr(), ka, va, block_table.data_ptr(), lens.data_ptr(), kn, vn, ws.data_ptr() if ws_floats else 0) + tail)
-    return out
+    return _InferenceOnlyFn.apply('paged_attention', out, q, k_pages, v_pages, k_new, v_new) if grad else out
 
 
 def _append_plan(k, v, k_pages, v_pages, block_table, starts, counts):

@@ -546,3 +546,30 @@ def forward_mode_case(ops, dev, tokens, dropout_p=0.0):
                 ops.cross_attention(*y, dropout_p=dropout_p)
         assert ops.cross_attention(*x, dropout_p=dropout_p).shape == x[0].shape
     assert ops.cross_attention(*y, dropout_p=dropout_p).shape == x[0].shape
+
+
+def no_backward_case(ops, dev):
+    """paged_attention under autograd: the same values, and an error where a gradient would get lost"""
+    import torch.autograd.forward_ad as fw
+    g = torch.Generator().manual_seed(2)
+    q, kn, vn = (torch.randn(2, 2, 16, generator=g).to(dev) for _ in range(3))
+    kp, vp = (torch.randn(3, 2, 4, 16, generator=g).to(dev) for _ in range(2))
+    table, lens = torch.tensor([[0], [2]], dtype=torch.int32).to(dev), torch.tensor([3, 0], dtype=torch.int32).to(dev)
+    want = ops.paged_attention(q, kp, vp, table, lens, kn, vn)
+    assert not want.requires_grad
+    w = torch.ones(16, 16, device=dev, requires_grad=True)
+    for i in range(3):
+        y = [q, kn, vn]
+        y[i] = y[i].clone().requires_grad_()
+        out = ops.paged_attention(y[0], kp, vp, table, lens, y[1], y[2])
+        assert torch.equal(out, want)
+        assert torch.autograd.grad((out.detach() @ w).sum(), w)[0].shape == w.shape
+        with pytest.raises(NotImplementedError, match='paged_attention'):
+            out.sum().backward()
+        with torch.no_grad():
+            assert not ops.paged_attention(y[0], kp, vp, table, lens, y[1], y[2]).requires_grad
+    out = ops.paged_attention(q.clone().requires_grad_(), kp, vp, table[:, :0], lens)      # no key: zeros
+    with pytest.raises(NotImplementedError, match='paged_attention'):
+        out.sum().backward()
+    with fw.dual_level(), pytest.raises(NotImplementedError):
+        ops.paged_attention(fw.make_dual(q, q), kp, vp, table, lens)

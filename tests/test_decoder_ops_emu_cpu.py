@@ -268,3 +268,7 @@ def test_sample_rows_of_nan_among_minus_infinities(emu, V):
 def test_cross_attention_of_dual_tensors(emu, tokens):
     C.forward_mode_case(emu, 'cpu', tokens)
     C.forward_mode_case(emu, 'cpu', tokens, 0.1)
+
+
+def test_paged_attention_has_no_backward_pass(emu):
+    C.no_backward_case(emu, 'cpu')

@@ -307,3 +307,7 @@ def test_sample_rows_of_nan_among_minus_infinities(ops, V):
 def test_cross_attention_of_dual_tensors(ops, tokens):
     C.forward_mode_case(ops, DEV, tokens)
     C.forward_mode_case(ops, DEV, tokens, 0.1)
+
+
+def test_paged_attention_has_no_backward_pass(ops):
+    C.no_backward_case(ops, DEV)
