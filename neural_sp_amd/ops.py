@@ -12,6 +12,7 @@ import os
 import numpy as np
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version as _increment_version
 from torch.autograd.function import once_differentiable
 
 from neural_sp_amd import _lib
@@ -2345,6 +2346,8 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
     qa, ka, va = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
     if kn and ka == va:
         raise ValueError('k_pages and v_pages are the same memory')
+    if kn and (k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
+        raise ValueError('pages that require a gradient can be written to under torch.no_grad() only')
     if how == 'copy' or (qa | ka | va | kn | vn) & 15:
         _need_aligned(k_pages, v_pages)
         return paged_attention(_vec(q), k_pages, v_pages, block_table.contiguous(), lens.contiguous(),
@@ -2353,6 +2356,8 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
     ws = q.new_empty((ws_floats,), dtype=torch.float32) if ws_floats else None
     _call('nsp_decode_attn', dev, _DECODE_PTRS(
         qa, out.data_ptr(), ka, va, block_table.data_ptr(), lens.data_ptr(), kn, vn, ws.data_ptr() if ws_floats else 0) + tail)
+    if kn:
+        _increment_version((k_pages, v_pages))      # (a backward pass that saved them notices)
     return _InferenceOnlyFn.apply('paged_attention', out, q, k_pages, v_pages, k_new, v_new) if grad else out
 
 
@@ -2385,7 +2390,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
     k / v `[B,n,Hkv,d]` fp32 or bf16, the cache fp32 or bf16 (fp32 into bf16 rounds to nearest even; bf16 into fp32 is not
     offered); token t of row b goes to position starts[b] + t of its block_table row for t < counts[b] (all n without
     counts).  starts[b] < 0, absent pages (entries outside [0, n_pages)) and positions behind the table: nothing is written.
-    No position may be written twice by one call."""
+    No position may be written twice by one call.  No gradient passes through the cache."""
     _require_device(k)
     dev = k.get_device()
     if v.get_device() != dev or k_pages.get_device() != dev or v_pages.get_device() != dev or \
@@ -2401,12 +2406,15 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
     ka, va, kp, vp = k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
     if kp == vp:
         raise ValueError('k_pages and v_pages are the same memory')
+    if (k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
+        raise ValueError('pages that require a gradient can be written to under torch.no_grad() only')
     if how == 'copy' or (ka | va | kp | vp) & 15:
         _need_aligned(k_pages, v_pages)
         return paged_append(_vec(k), _vec(v), k_pages, v_pages, block_table.contiguous(), starts.contiguous(),
                             None if counts is None else counts.contiguous())
     _call('nsp_paged_append', dev, _APPEND_PTRS(
         ka, va, kp, vp, block_table.data_ptr(), starts.data_ptr(), 0 if counts is None else counts.data_ptr()) + tail)
+    _increment_version((k_pages, v_pages))
 
 
 class CrossAttnFn(torch.autograd.Function):

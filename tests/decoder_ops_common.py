@@ -573,3 +573,33 @@ def no_backward_case(ops, dev):
         out.sum().backward()
     with fw.dual_level(), pytest.raises(NotImplementedError):
         ops.paged_attention(fw.make_dual(q, q), kp, vp, table, lens)
+
+
+def overwritten_pages_case(ops, dev):
+    """autograd notices that pages changed behind its back; pages of its own are not written to"""
+    q = torch.ones(1, 1, 8).to(dev)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32).to(dev), torch.zeros(1, dtype=torch.int32).to(dev)
+
+    def attend(kp, vp):
+        ops.paged_attention(q, kp, vp, table, lens, q, q)
+
+    def append(kp, vp):
+        ops.paged_append(q.unsqueeze(1), q.unsqueeze(1), kp, vp, table, lens)
+    for write in (attend, append):
+        both = torch.zeros(2, 1, 1, 4, 8).to(dev)
+        for i in range(2):
+            w = torch.ones(8, device=dev, requires_grad=True)
+            loss = (both[i] * w).sum()                    # saves the pages
+            write(both[0], both[1])
+            with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+                loss.backward()
+        own = both[0].clone().requires_grad_()
+        with pytest.raises(ValueError):
+            write(own, both[1])
+        with torch.no_grad():
+            write(own, both[1])
+        with torch.inference_mode():                      # (tensors without a version)
+            write(torch.zeros(1, 1, 4, 8).to(dev), torch.zeros(1, 1, 4, 8).to(dev))
+    kp = torch.zeros(1, 1, 4, 8).to(dev)
+    ops.paged_attention(q, kp, kp, table, lens)
+    assert kp._version == 0                               # reading is no change

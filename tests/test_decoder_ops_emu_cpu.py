@@ -272,3 +272,7 @@ def test_cross_attention_of_dual_tensors(emu, tokens):
 
 def test_paged_attention_has_no_backward_pass(emu):
     C.no_backward_case(emu, 'cpu')
+
+
+def test_pages_that_autograd_has_saved(emu):
+    C.overwritten_pages_case(emu, 'cpu')

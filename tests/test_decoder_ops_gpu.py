@@ -311,3 +311,7 @@ def test_cross_attention_of_dual_tensors(ops, tokens):
 
 def test_paged_attention_has_no_backward_pass(ops):
     C.no_backward_case(ops, DEV)
+
+
+def test_pages_that_autograd_has_saved(ops):
+    C.overwritten_pages_case(ops, DEV)
