@@ -700,7 +700,7 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(const XArgs p) {
   for (int f = 0; f < NK; ++f)
 #pragma unroll
     for (int i = 0; i < X::NB; ++i) dk[f][i] = dv[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (item * (64 * NK) < klen && p.Tq > 0) {      // (uniform over the workgroup; keys behind klen get zeros)
+  if (item * (64 * NK) < klen) {      // (uniform over the workgroup; keys behind klen get zeros)
     const int chunks = p.D / X::E::CE, nqt = (p.Tq + X::KT - 1) / X::KT, n = G * nqt;
     const T* qb = reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)hkv * G * p.q_sh;
     const T* gb = reinterpret_cast<const T*>(p.dout) + (long long)b * p.g_sb + (long long)hkv * G * p.g_sh;
@@ -860,9 +860,9 @@ int cross_attn(const nsp_cross_attn_params* a, bool bwd, void* stream) {
   for (const long long ld : {a->q_st, a->k_st, a->v_st, a->g_st})
     if (ld < 0 || ld >= far) return NSP_EUNSUPPORTED;
   if (!(a->dropout_p >= 0. && a->dropout_p < 1.)) return NSP_EINVAL;
-  if (a->B == 0 || a->Tk == 0 || (a->Tq == 0 && !bwd)) return NSP_OK;     // (nothing to read, or nothing to write but empty rows: the caller's)
-  if (!a->k || !a->v || (a->Tq > 0 && (!a->q || !a->out))) return NSP_EINVAL;
-  if (bwd && (a->Tq == 0 || !a->dout || !a->dq || !a->dk || !a->dv || !a->stats || !a->rows)) return NSP_EINVAL;
+  if (a->B == 0 || a->Tk == 0 || a->Tq == 0) return NSP_OK;     // (no query or no key: zeros, which are the caller's)
+  if (!a->q || !a->k || !a->v || !a->out) return NSP_EINVAL;
+  if (bwd && (!a->dout || !a->dq || !a->dk || !a->dv || !a->stats || !a->rows)) return NSP_EINVAL;
   XArgs p;
   p.q = a->q; p.k = a->k; p.v = a->v; p.dout = a->dout; p.out = a->out;
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.stats = a->stats; p.rows = a->rows; p.klens = a->klens;

@@ -276,3 +276,12 @@ def test_paged_attention_has_no_backward_pass(emu):
 
 def test_pages_that_autograd_has_saved(emu):
     C.overwritten_pages_case(emu, 'cpu')
+
+
+def test_c_entries_of_cross_attention_without_queries_or_keys(emu):
+    """nothing is read or written, in both directions"""
+    from neural_sp_amd import _lib
+    for B, Tq, Tk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+        sizes = emu._CROSS_TAIL(B, 2, 2, 16, Tq, Tk, 0, *(512, 32, 16) * 3, 0.25, 0.0)
+        for name in ('nsp_cross_attn_fwd', 'nsp_cross_attn_bwd'):
+            assert getattr(_lib.lib(), name)(emu._CROSS_PTRS(*[0] * 11, 512, 32, 16, 0, 0) + sizes, 0) == 0
