@@ -828,7 +828,7 @@ int nsp_sample_rows(const nsp_sample_params* p, void* stream);
  *   dtype.  Training: fwd also fills stats [2][B,H,Tq] fp32 (NULL for inference); bwd reads out
  *   and stats, uses rows [3][B,H,Tq rounded up to 64] fp32 as scratch and writes dq, dk, dv completely.
  *   dropout: element (b,h,i,j) is kept as nsp_attn_softmax_fwd keeps it: counter offset + ((b H + h) Tq + i) Tk + j.
- *   scale > 0.  B, Tq or Tk == 0: NSP_OK, nothing is written (outputs and gradients that are not empty are zeros: the caller's). */
+ *   scale > 0; token strides (*_st) of more than one row below 2^24.  B, Tq or Tk == 0: NSP_OK, nothing is written (outputs and gradients that are not empty are zeros: the caller's). */
 typedef struct {
   const void* q; const void* k; const void* v; const void* dout;
   void* out; void* dq; void* dk; void* dv;

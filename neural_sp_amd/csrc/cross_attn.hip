@@ -856,8 +856,10 @@ int cross_attn(const nsp_cross_attn_params* a, bool bwd, void* stream) {
   if (!a || a->B < 0 || a->Tq < 0 || a->Tk < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv || a->D <= 0) return NSP_EINVAL;
   if (a->D % 8 || a->D > 128 || (a->dtype != NSP_DT_F32 && a->dtype != NSP_DT_BF16)) return NSP_EUNSUPPORTED;
   if (a->B * a->H > 0x7ffffff0LL || a->Tq > 0x7fffff00LL || a->Tk > 0x7fffff00LL || !(a->scale > 0.)) return NSP_EUNSUPPORTED;
-  const long long far = 1 << 24;      // (32-bit offsets inside a tile)
-  for (const long long ld : {a->q_st, a->k_st, a->v_st, a->g_st})
+  // (32-bit offsets inside a tile; the stride of one row is never used and may be anything)
+  const long long far = 1 << 24, q_st = a->Tq > 1 ? a->q_st : 0, k_st = a->Tk > 1 ? a->k_st : 0, v_st = a->Tk > 1 ? a->v_st : 0,
+                  g_st = a->Tq > 1 ? a->g_st : 0;
+  for (const long long ld : {q_st, k_st, v_st, g_st})
     if (ld < 0 || ld >= far) return NSP_EUNSUPPORTED;
   if (!(a->dropout_p >= 0. && a->dropout_p < 1.)) return NSP_EINVAL;
   if (a->B == 0 || a->Tk == 0 || a->Tq == 0) return NSP_OK;     // (no query or no key: zeros, which are the caller's)
@@ -867,10 +869,10 @@ int cross_attn(const nsp_cross_attn_params* a, bool bwd, void* stream) {
   p.q = a->q; p.k = a->k; p.v = a->v; p.dout = a->dout; p.out = a->out;
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.stats = a->stats; p.rows = a->rows; p.klens = a->klens;
   p.B = (int)a->B; p.H = (int)a->H; p.Hkv = (int)a->Hkv; p.D = (int)a->D; p.Tq = (int)a->Tq; p.Tk = (int)a->Tk;
-  p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
-  p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;
-  p.v_sb = a->v_sb; p.v_st = a->v_st; p.v_sh = a->v_sh;
-  p.g_sb = a->g_sb; p.g_st = a->g_st; p.g_sh = a->g_sh;
+  p.q_sb = a->q_sb; p.q_st = q_st; p.q_sh = a->q_sh;
+  p.k_sb = a->k_sb; p.k_st = k_st; p.k_sh = a->k_sh;
+  p.v_sb = a->v_sb; p.v_st = v_st; p.v_sh = a->v_sh;
+  p.g_sb = a->g_sb; p.g_st = g_st; p.g_sh = a->g_sh;
   p.seed = a->seed; p.offset = a->offset;
   p.scale = (float)a->scale;
   p.sl2 = (float)(a->scale * 1.4426950408889634);

@@ -2417,6 +2417,16 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
     _increment_version((k_pages, v_pages))
 
 
+def _far(t):
+    """a stride between tokens that the training kernels' 32-bit offsets do not reach"""
+    return t.stride(1) >= 1 << 24 and t.shape[1] > 1
+
+
+def _near(t):
+    """t, or a copy whose tokens lie next to each other"""
+    return t.transpose(1, 2).contiguous().transpose(1, 2) if _far(t) else t
+
+
 class CrossAttnFn(torch.autograd.Function):
     """cross_attention with its backward (csrc/cross_attn.hip); arguments as checked there.  Saved beside the inputs and the
     output: stats [2,B,H,Tq] (fp32).  Backward's scratch [3,B,H,Tq rounded up to 64] is its own, as two captured backward passes
@@ -2454,9 +2464,11 @@ class CrossAttnFn(torch.autograd.Function):
         if (q.stride(), k.stride(), v.stride()) != ctx.strides or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 or \
                 not out.is_contiguous() or out.data_ptr() & 15:      # saved-tensor hooks may lay them out anew
             q, k, v, out = (t.clone(memory_format=torch.contiguous_format) for t in (q, k, v, out))
+            q, k, v = _near(q), _near(k), _near(v)
             tail = _cross_plan(q, k, v, klens, *ctx.setting)[1]
         if dout.dtype != q.dtype or not dout.is_contiguous() or dout.data_ptr() & 15:
             dout = _vec(dout.to(q.dtype))
+        dout = _near(dout)
         g0, g1, g2, _ = dout.stride()
         dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
         B, Tq, H, _ = q.shape
@@ -2468,8 +2480,8 @@ class CrossAttnFn(torch.autograd.Function):
 
 
 def _cross_plan(q, k, v, klens, scale, dropout_p):
-    """-> (can the strides be read, constant part for the training kernels, the same for the single-token kernel if it may take
-    the call, its workspace floats)"""
+    """-> (can the strides be read, constant part for the training kernels if they reach all tokens, the same for the single-token
+    kernel if it may take the call, its workspace floats)"""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError('q [B,Tq,H,d] and k / v [B,Tk,Hkv,d], all fp32 or all bf16, expected: got %s %s, %s %s, %s %s' % (
             q.dtype, tuple(q.shape), k.dtype, tuple(k.shape), v.dtype, tuple(v.shape)))
@@ -2488,7 +2500,9 @@ def _cross_plan(q, k, v, klens, scale, dropout_p):
     if not (_vec_strides(q) and _vec_strides(k) and _vec_strides(v) and (klens is None or klens.is_contiguous())):
         return False, None, None, 0
     st = [t.stride()[:3] for t in (q, k, v)]
-    tail = _CROSS_TAIL(B, H, Hkv, D, Tq, Tk, _DTYPES[q.dtype], *st[0], *st[1], *st[2], scale, dropout_p)
+    tail = None
+    if not (_far(q) or _far(k) or _far(v)):
+        tail = _CROSS_TAIL(B, H, Hkv, D, Tq, Tk, _DTYPES[q.dtype], *st[0], *st[1], *st[2], scale, dropout_p)
     few = dropout_p == 0 and 0 < Tq * (H // Hkv) <= 16 and 0 < B <= 65535 and Hkv <= 65535 and 0 < Tk <= 0x7f000000
     one, floats = _decode_tail(B, H, Hkv, D, Tq, 1, 0, Tk, q.dtype, *st, (0, 0, 0, 0), scale) if few else (None, 0)
     return True, tail, one, floats
@@ -2524,6 +2538,8 @@ def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
         _call('nsp_decode_attn', dev, _DECODE_PTRS(
             qa, out.data_ptr(), ka, va, 0, 0 if klens is None else klens.data_ptr(), 0, 0, ws.data_ptr() if floats else 0) + one)
         return out
+    if tail is None:
+        return cross_attention(_near(q), _near(k), _near(v), klens, scale, dropout_p)
     return CrossAttnFn.apply(q, k, v, klens, tail, next_dropout_seed()[0] if dropout_p > 0 else 0, need, scale, dropout_p)
 
 

@@ -603,3 +603,25 @@ def overwritten_pages_case(ops, dev):
     kp = torch.zeros(1, 1, 4, 8).to(dev)
     ops.paged_attention(q, kp, kp, table, lens)
     assert kp._version == 0                               # reading is no change
+
+
+def far_tokens_case(ops, dev):
+    """tokens 2^24 elements and more apart, and a single token whose stride means nothing: the results of dense tensors"""
+    g = torch.Generator().manual_seed(4)
+    far = 1 << 24
+
+    def apart(x, step):
+        n = (x.shape[1] - 1) * step + x.shape[2] * x.shape[3]
+        return torch.zeros(n, dtype=x.dtype, device=dev).as_strided(x.shape, (8, step, x.shape[3], 1)).copy_(x)
+
+    def run(q, k, v, dout):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        out = ops.cross_attention(q, k, v)
+        return [out.detach()] + list(torch.autograd.grad(out, (q, k, v), dout))
+    for Tq, steps in ((2, (far, 64, 64, 64)), (2, (64, far + 8, far, 64)), (2, (64, 64, 64, far)), (1, (3 * far, 64, 64, 3 * far))):
+        x = [torch.randn(1, t, 4, 16, generator=g).to(torch.bfloat16) for t in (Tq, 2, 2, Tq)]
+        want = run(*(t.to(dev) for t in x))
+        assert all(torch.equal(a, b) for a, b in zip(run(*(apart(t, s) for t, s in zip(x, steps))), want))
+        # (the single-token form reads them as they are)
+        assert torch.equal(ops.cross_attention(x[0].to(dev), apart(x[1], far), apart(x[2], far)),
+                           ops.cross_attention(*(t.to(dev) for t in x[:3])))

@@ -285,3 +285,7 @@ def test_c_entries_of_cross_attention_without_queries_or_keys(emu):
         sizes = emu._CROSS_TAIL(B, 2, 2, 16, Tq, Tk, 0, *(512, 32, 16) * 3, 0.25, 0.0)
         for name in ('nsp_cross_attn_fwd', 'nsp_cross_attn_bwd'):
             assert getattr(_lib.lib(), name)(emu._CROSS_PTRS(*[0] * 11, 512, 32, 16, 0, 0) + sizes, 0) == 0
+
+
+def test_cross_attention_of_tokens_far_apart(emu):
+    C.far_tokens_case(emu, 'cpu')

@@ -315,3 +315,7 @@ def test_paged_attention_has_no_backward_pass(ops):
 
 def test_pages_that_autograd_has_saved(ops):
     C.overwritten_pages_case(ops, DEV)
+
+
+def test_cross_attention_of_tokens_far_apart(ops):
+    C.far_tokens_case(ops, DEV)
