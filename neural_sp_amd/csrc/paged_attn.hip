@@ -21,6 +21,7 @@
 // Scores of -inf alone have no softmax.  Over states the result is NaN, as the training kernel and the definition have it; over
 // a cache such a row is one whose keys are all absent: zeros.
 #include "attn_frag.h"
+#include <algorithm>
 
 namespace {
 
@@ -34,8 +35,8 @@ struct DecodeArgs {
   const void* k_new;
   const void* v_new;
   float* ws;
-  int B, H, Hkv, D, Tq, page, n_pages, width, nsplit, chunk, cap, rows, ngrp;
-  unsigned page_magic;
+  int B, H, Hkv, D, Tq, page, width, nsplit, chunk, cap, rows, ngrp;
+  unsigned page_magic, n_pages;
   long long q_sb, q_st, q_sh, k_sp, k_ss, k_sh, v_sp, v_ss, v_sh, kn_sb, kn_sh, vn_sb, vn_sh;
   float sl2;
 };
@@ -46,6 +47,9 @@ __device__ __forceinline__ void page_split(const DecodeArgs& p, unsigned j, unsi
   slot = j - pg * (unsigned)p.page;
   if (slot >= (unsigned)p.page) { ++pg; slot -= (unsigned)p.page; }
 }
+
+// is there such a page (a negative number is behind every page)
+__device__ __forceinline__ bool page_there(const DecodeArgs& p, int id) { return (unsigned)id < p.n_pages; }
 
 // VW consecutive elements of a value row
 template <typename T, int VW>
@@ -174,7 +178,7 @@ __device__ __forceinline__ void load_tile(Tile<T, DP>& t, const DecodeArgs& p, c
 #pragma unroll
       for (int e = 0; e < 4; ++e) vrow[e] = vb + (long long)min(jb + 4 * g + e, end - 1) * p.v_ss;
     } else if constexpr (MODE == BLOCK16) {
-      kok = jb < end && pages.id[kf] >= 0 && pages.id[kf] < p.n_pages;
+      kok = jb < end && page_there(p, pages.id[kf]);
       const long long at = kok ? pages.id[kf] : 0;
       const int slot = kok ? pages.slot[kf] : 0, top = kok ? min(15, end - 1 - jb) : 0;
       krow = kb + at * p.k_sp + (long long)(slot + min(r, top)) * p.k_ss;
@@ -188,13 +192,13 @@ __device__ __forceinline__ void load_tile(Tile<T, DP>& t, const DecodeArgs& p, c
       unsigned pg, slot;
       page_split(p, (unsigned)min(jb + r, end - 1), pg, slot);
       int id = tab[pg];
-      kok = id >= 0 && id < p.n_pages;
+      kok = page_there(p, id);
       krow = kb + (long long)(kok ? id : 0) * p.k_sp + (long long)slot * p.k_ss;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         page_split(p, (unsigned)min(jb + 4 * g + e, end - 1), pg, slot);
         id = tab[pg];
-        vok[e] = id >= 0 && id < p.n_pages;
+        vok[e] = page_there(p, id);
         vrow[e] = vb + (long long)(vok[e] ? id : 0) * p.v_sp + (long long)slot * p.v_ss;
         t.ok |= vok[e] ? (1u << (4 * kf + e)) : 0u;
       }
@@ -320,7 +324,7 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
     unsigned pg, slot;
     page_split(p, (unsigned)len, pg, slot);
     const int id = tab[pg];
-    if (id >= 0 && id < p.n_pages) {
+    if (page_there(p, id)) {
       has_new = true;
       const T* kn = reinterpret_cast<const T*>(p.k_new) + (long long)b * p.kn_sb + (long long)hkv * p.kn_sh;
       const T* vn = reinterpret_cast<const T*>(p.v_new) + (long long)b * p.vn_sb + (long long)hkv * p.vn_sh;
@@ -548,7 +552,7 @@ extern "C" int nsp_decode_attn(const nsp_decode_attn_params* a, void* stream) {
   p.q = a->q; p.out = a->out; p.k = a->k; p.v = a->v; p.table = a->table; p.lens = a->lens;
   p.k_new = a->k_new; p.v_new = a->v_new; p.ws = a->ws;
   p.B = (int)a->B; p.H = (int)a->H; p.Hkv = (int)a->Hkv; p.D = (int)a->D; p.Tq = (int)a->Tq;
-  p.page = (int)a->page; p.n_pages = (int)a->n_pages; p.width = (int)a->width;
+  p.page = (int)a->page; p.n_pages = (unsigned)std::min(a->n_pages, 1LL << 31); p.width = (int)a->width;
   p.cap = (int)cap; p.rows = (int)rows; p.ngrp = (int)ngrp;
   p.page_magic = a->table ? (a->page == 1 ? 0xFFFFFFFFu : (unsigned)(0x100000000ULL / (unsigned long long)a->page)) : 0u;
   p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;

@@ -625,3 +625,19 @@ def far_tokens_case(ops, dev):
         # (the single-token form reads them as they are)
         assert torch.equal(ops.cross_attention(x[0].to(dev), apart(x[1], far), apart(x[2], far)),
                            ops.cross_attention(*(t.to(dev) for t in x[:3])))
+
+
+def many_pages_case(ops, dev, page):
+    """a cache of more pages than 31 or 32 bits count (one page, expanded): its pages are there, negative entries are not"""
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(1, 1, page, 32, generator=g).to(dev) for _ in range(2))
+    q = torch.randn(3, 1, 32, generator=g)
+    table = torch.tensor([[7, 2 ** 31 - 1], [-1, -2 ** 31], [0, -5]], dtype=torch.int32)
+    lens = [2 * page, 2 * page, 2 * page - 1]
+    for n_pages in (2 ** 31, 2 ** 31 + 5, 2 ** 32 + 1):
+        out = ops.paged_attention(q.to(dev), k.expand(n_pages, 1, page, 32), v.expand(n_pages, 1, page, 32), table.to(dev),
+                                  torch.tensor(lens, dtype=torch.int32).to(dev))
+        ref, dp, av = attention_ref(torch.cat([q[0], q[2]]), k[0, 0].cpu(), v[0, 0].cpu(), page)      # (a key twice: the same softmax)
+        dp = dp + page * E32
+        check_close(torch.stack([out[0, 0], out[2, 0]]), ref, E32 * ref.abs() + dp * av * (1 + E32), n_pages)
+        assert not out[1].any()

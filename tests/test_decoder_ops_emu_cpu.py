@@ -289,3 +289,8 @@ def test_c_entries_of_cross_attention_without_queries_or_keys(emu):
 
 def test_cross_attention_of_tokens_far_apart(emu):
     C.far_tokens_case(emu, 'cpu')
+
+
+@pytest.mark.parametrize('page', [16, 5])
+def test_paged_attention_of_more_pages_than_an_int_counts(emu, page):
+    C.many_pages_case(emu, 'cpu', page)

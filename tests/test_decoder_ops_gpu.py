@@ -319,3 +319,8 @@ def test_pages_that_autograd_has_saved(ops):
 
 def test_cross_attention_of_tokens_far_apart(ops):
     C.far_tokens_case(ops, DEV)
+
+
+@pytest.mark.parametrize('page', [16, 5])
+def test_paged_attention_of_more_pages_than_an_int_counts(ops, page):
+    C.many_pages_case(ops, DEV, page)
