@@ -39,13 +39,22 @@ class PagedKVCache(object):
     def free_pages(self):
         return len(self._free)
 
+    def _numbers(self, rows):
+        """each row once, as a number of 0 .. n_rows - 1 (negative ones count from the end); nothing is changed for a wrong one"""
+        n = len(self._rows)
+        rows = [int(r) for r in rows]
+        for r in rows:
+            if not -n <= r < n:
+                raise IndexError('row %d of a cache of %d rows' % (r, n))
+        return list(dict.fromkeys(r % n for r in rows))
+
     def reserve(self, rows, n_tokens):
         """pages for n_tokens tokens (in all, not in addition) of each of `rows`; all or none.  The caller's `lens` says how many
         of them are stored."""
         want = (int(n_tokens) + self.page_size - 1) // self.page_size
         if want > self.max_pages:
             raise ValueError('%d tokens: a row holds %d' % (n_tokens, self.max_pages * self.page_size))
-        rows = list(dict.fromkeys(int(r) for r in rows))
+        rows = self._numbers(rows)
         need = sum(max(0, want - len(self._rows[r])) for r in rows)
         if need > len(self._free):
             raise RuntimeError('PagedKVCache: %d pages wanted, %d free' % (need, len(self._free)))
@@ -60,7 +69,7 @@ class PagedKVCache(object):
     def release(self, rows):
         """give the pages of `rows` back (the caller sets their `lens` to -1); launches in the stream so far still read them
         undisturbed, later ones of the same stream may write them for other rows"""
-        for r in dict.fromkeys(int(r) for r in rows):
+        for r in self._numbers(rows):
             self._free.extend(reversed(self._rows[r]))
             self._rows[r] = []
             self._table[r] = -1

@@ -198,3 +198,28 @@ def cache_case(dev):
     assert c.free_pages == 0 and len(set(t[t >= 0].tolist())) == 5
     with pytest.raises(ValueError):
         PagedKVCache(1, 1, 0, 1, 8, torch.float32, dev)
+
+
+def cache_rows_case(dev):
+    """a row named twice, once from the end, is one row; a wrong row changes nothing"""
+    import pytest
+    from neural_sp_amd.kv_cache import PagedKVCache
+    c = PagedKVCache(1, 3, 16, 1, 8, torch.float32, dev, page_size=8, n_pages=3)
+    c.reserve([2, -1], 16)
+    c.reserve([0], 8)
+    t = c.block_table.cpu()
+    assert (t >= 0).sum(1).tolist() == [1, 0, 2] and c.free_pages == 0
+    for wrong in (3, -4):
+        with pytest.raises(IndexError):
+            c.reserve([0, wrong], 16)
+        with pytest.raises(IndexError):
+            c.release([0, wrong])
+        assert torch.equal(c.block_table.cpu(), t) and c.free_pages == 0
+        c.reserve([0], 8)                               # still its own page
+        assert torch.equal(c.block_table.cpu(), t)
+    c.release([-1, 2])
+    assert c.free_pages == 2 and c.block_table.cpu()[2].tolist() == [-1, -1]
+    c.reserve([1], 16)
+    t = c.block_table.cpu()
+    used = t[t >= 0].tolist()
+    assert len(used) == len(set(used)) == 3

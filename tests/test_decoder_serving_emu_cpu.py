@@ -44,3 +44,7 @@ def test_fused_source_attention_in_a_training_step(emu, monkeypatch):
 
 def test_paged_cache_hands_out_pages():
     S.cache_case('cpu')
+
+
+def test_paged_cache_rows_from_the_end_and_wrong_ones():
+    S.cache_rows_case('cpu')

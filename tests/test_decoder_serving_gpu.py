@@ -57,3 +57,7 @@ def test_fused_source_attention_in_a_bf16_training_step(monkeypatch):
 def test_paged_cache_hands_out_pages():
     S.cache_case('cuda')
     torch.cuda.synchronize()
+
+
+def test_paged_cache_rows_from_the_end_and_wrong_ones():
+    S.cache_rows_case('cuda')
