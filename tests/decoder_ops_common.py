@@ -641,3 +641,39 @@ def many_pages_case(ops, dev, page):
         dp = dp + page * E32
         check_close(torch.stack([out[0, 0], out[2, 0]]), ref, E32 * ref.abs() + dp * av * (1 + E32), n_pages)
         assert not out[1].any()
+
+
+def dropout_widths_case(ops, dev, dtype, B, H, Hkv, Tq, Tk, D, klens, p=0.25, seed=6):
+    """dropout at every width of the kernels, odd lengths over several tiles of either side, shared heads: the factors are those
+    that the training softmax draws from the same site (q = 0: every visible probability is 1 / klen), read off with values that
+    are rows of the identity"""
+    gen = torch.Generator().manual_seed(D)
+    lens = torch.tensor(klens, dtype=torch.int32).to(dev)
+    mode, W = ops.get_compute_mode(), 64
+    ops.set_compute_mode('f32')
+    keep = torch.zeros(B, H, Tq, Tk)
+    for j0 in range(0, Tk, W):
+        n = min(W, Tk - j0)
+        eye = torch.zeros(B, Tk, H, W)
+        eye[:, range(j0, j0 + n), :, range(n)] = 1.0
+        ops.manual_dropout_seed(seed)
+        cv, _ = ops.AttentionFn.apply(torch.zeros(B, Tq, H, W).to(dev), None, torch.zeros(B, Tk, H, W).to(dev), eye.to(dev), None, lens,
+                                      {'dropout': p, 'training': True})
+        cv = cv.detach().cpu().view(B, Tq, H, W)
+        for b in range(B):
+            keep[b, :, :, j0:j0 + n] = (cv[b] * klens[b]).permute(1, 0, 2)[:, :, :n]
+    ops.set_compute_mode(mode)
+    keep = (keep > 0.5).double() / (1 - p)
+    q, k, v, dout = (torch.randn(B, t, h, D, generator=gen).to(dtype) for t, h in ((Tq, H), (Tk, Hkv), (Tk, Hkv), (Tq, H)))
+    ref = cross_ref(q, k, v, dout, klens, dtype, keep=keep)
+    qd, kd, vd = (x.to(dev).requires_grad_(True) for x in (q, k, v))
+    ops.manual_dropout_seed(seed)
+    out = ops.cross_attention(qd, kd, vd, lens, dropout_p=p)
+    check_close(out, *ref['out'], 'out')
+    for name, x in zip(('dq', 'dk', 'dv'), torch.autograd.grad(out, (qd, kd, vd), dout.to(dev))):
+        check_close(x, *ref[name], name)
+
+
+DROPOUT_WIDTHS = [dict(B=2, H=2, Hkv=2, Tq=67, Tk=201, D=64, klens=[201, 139]), dict(B=1, H=4, Hkv=2, Tq=131, Tk=67, D=32, klens=[66]),
+                  dict(B=1, H=2, Hkv=1, Tq=67, Tk=203, D=128, klens=[203]), dict(B=1, H=2, Hkv=2, Tq=5, Tk=71, D=72, klens=[70]),
+                  dict(B=2, H=3, Hkv=1, Tq=70, Tk=69, D=64, klens=[1, 69])]

@@ -294,3 +294,9 @@ def test_cross_attention_of_tokens_far_apart(emu):
 @pytest.mark.parametrize('page', [16, 5])
 def test_paged_attention_of_more_pages_than_an_int_counts(emu, page):
     C.many_pages_case(emu, 'cpu', page)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('a', C.DROPOUT_WIDTHS, ids=str)
+def test_cross_attention_dropout_widths(emu, dtype, a):
+    C.dropout_widths_case(emu, 'cpu', dtype, **a)

@@ -324,3 +324,9 @@ def test_cross_attention_of_tokens_far_apart(ops):
 @pytest.mark.parametrize('page', [16, 5])
 def test_paged_attention_of_more_pages_than_an_int_counts(ops, page):
     C.many_pages_case(ops, DEV, page)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('a', C.DROPOUT_WIDTHS, ids=str)
+def test_cross_attention_dropout_widths(ops, dtype, a):
+    C.dropout_widths_case(ops, DEV, dtype, **a)
