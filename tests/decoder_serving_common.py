@@ -223,3 +223,33 @@ def cache_rows_case(dev):
     t = c.block_table.cpu()
     used = t[t >= 0].tolist()
     assert len(used) == len(set(used)) == 3
+
+
+def bf16_logits_case(dev, monkeypatch, steps=12):
+    """bf16 mode: the logits that the cached steps hand to the sampler, against the training path's on the same prefixes.  Both
+    round, in different places, so each step's logits as a whole: as near to the fp32 mode's as the training path's are -- twice
+    that distance, and one bf16 rounding (of the norm)."""
+    from neural_sp_amd import ops
+    model = tiny_model(dev)
+    model.eval()
+    dec = model.dec_fwd
+    eouts, elens = states(dev)
+    with torch.no_grad():
+        dec.output.bias[dec.eos] = -1e4               # all utterances take every step
+    got, real = [], ops.sample_rows
+    monkeypatch.setattr(ops, 'sample_rows', lambda x, *a: (got.append(x.detach().float().cpu()), real(x, *a))[1])
+    with ops.compute_mode('bf16'):
+        hyps, _ = dec.sample(eouts, elens, steps / eouts.shape[1], seed=3, page_size=4)
+    monkeypatch.setattr(ops, 'sample_rows', real)
+    assert len(got) == steps and [len(h) for h in hyps] == [steps] * 3
+    ys = torch.full((3, steps), dec.eos, dtype=torch.int64)
+    for b, h in enumerate(hyps):
+        ys[b, 1:] = torch.from_numpy(np.ascontiguousarray(h[:-1]).astype(np.int64))
+    with ops.compute_mode('f32'):
+        want = uncached_logits(dec, eouts, elens, ys).double()
+    with ops.compute_mode('bf16'):
+        other = uncached_logits(dec, eouts, elens, ys).double()
+    seen = [i for i in range(want.shape[2]) if i != dec.eos]
+    for n in range(steps):
+        w, o, x = want[:, n, seen], other[:, n, seen], got[n].double()[:, seen]
+        assert float((x - w).norm()) <= 2 * float((o - w).norm()) + 2.0 ** -8 * float(w.norm()), n

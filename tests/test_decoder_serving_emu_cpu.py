@@ -48,3 +48,7 @@ def test_paged_cache_hands_out_pages():
 
 def test_paged_cache_rows_from_the_end_and_wrong_ones():
     S.cache_rows_case('cpu')
+
+
+def test_logits_of_cached_steps_in_bf16_mode(emu, monkeypatch):
+    S.bf16_logits_case('cpu', monkeypatch)

@@ -61,3 +61,7 @@ def test_paged_cache_hands_out_pages():
 
 def test_paged_cache_rows_from_the_end_and_wrong_ones():
     S.cache_rows_case('cuda')
+
+
+def test_logits_of_cached_steps_in_bf16_mode(monkeypatch):
+    S.bf16_logits_case('cuda', monkeypatch)
