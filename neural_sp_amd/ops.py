@@ -12,7 +12,6 @@ import os
 import numpy as np
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.graph import increment_version as _increment_version
 from torch.autograd.function import once_differentiable
 
 from neural_sp_amd import _lib
@@ -2248,8 +2247,7 @@ def _need_aligned(*pages):
 
 def _have_tangents(*tensors):
     """is one of them a dual tensor of forward-mode differentiation (nodes refuse these; a kernel would drop the tangent)"""
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _InferenceOnlyFn(torch.autograd.Function):
@@ -2336,17 +2334,17 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
                lens.stride(), lens.dtype, scale, k_new.shape, k_new.stride(), k_new.dtype, v_new.shape, v_new.stride(), v_new.dtype)
         kn, vn = k_new.data_ptr(), v_new.data_ptr()
     how, tail, ws_floats = _PLANS.get(key) or _plan(key, _paged_plan, q, k_pages, v_pages, block_table, lens, k_new, v_new, scale)
-    if _have_tangents(q, k_pages, v_pages, k_new, v_new):
+    if forward_ad._current_level >= 0 and _have_tangents(q, k_pages, v_pages, k_new, v_new):
         raise NotImplementedError('paged_attention of dual tensors')
-    grad = torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (
-        k_new is not None and (k_new.requires_grad or v_new.requires_grad)))
+    own = k_pages.requires_grad or v_pages.requires_grad
+    grad = (own or q.requires_grad or (kn and (k_new.requires_grad or v_new.requires_grad))) and torch.is_grad_enabled()
     if how == 'zeros':
         out = torch.zeros(q.shape, device=q.device, dtype=q.dtype)
         return _InferenceOnlyFn.apply('paged_attention', out, q, k_pages, v_pages, k_new, v_new) if grad else out
     qa, ka, va = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
     if kn and ka == va:
         raise ValueError('k_pages and v_pages are the same memory')
-    if kn and (k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
+    if kn and own and torch.is_grad_enabled():
         raise ValueError('pages that require a gradient can be written to under torch.no_grad() only')
     if how == 'copy' or (qa | ka | va | kn | vn) & 15:
         _need_aligned(k_pages, v_pages)
@@ -2357,7 +2355,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
     _call('nsp_decode_attn', dev, _DECODE_PTRS(
         qa, out.data_ptr(), ka, va, block_table.data_ptr(), lens.data_ptr(), kn, vn, ws.data_ptr() if ws_floats else 0) + tail)
     if kn:
-        _increment_version((k_pages, v_pages))      # (a backward pass that saved them notices)
+        torch._C._increment_version((k_pages, v_pages))      # (a backward pass that saved them notices)
     return _InferenceOnlyFn.apply('paged_attention', out, q, k_pages, v_pages, k_new, v_new) if grad else out
 
 
@@ -2414,7 +2412,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, starts, counts=None):
                             None if counts is None else counts.contiguous())
     _call('nsp_paged_append', dev, _APPEND_PTRS(
         ka, va, kp, vp, block_table.data_ptr(), starts.data_ptr(), 0 if counts is None else counts.data_ptr()) + tail)
-    _increment_version((k_pages, v_pages))
+    torch._C._increment_version((k_pages, v_pages))
 
 
 def _far(t):
@@ -2531,7 +2529,9 @@ def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
     qa, ka, va = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if not as_is or (qa | ka | va) & 15:
         return cross_attention(_vec(q), _vec(k), _vec(v), klens if klens is None else klens.contiguous(), scale, dropout_p)
-    need = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled() or _have_tangents(q, k, v)
+    need = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
+    if forward_ad._current_level >= 0:
+        need = need or _have_tangents(q, k, v)
     if one is not None and not need:
         out = q.new_empty(q.shape)
         ws = q.new_empty((floats,), dtype=torch.float32) if floats else None
