@@ -770,7 +770,7 @@ int nsp_lstm_cell_bwd(const float* dh, const float* dc_next, const float* gates,
  *     k / v = [n_pages, Hkv, page, D] (strides *_sp, *_sh, *_ss); width =       *
  *     entries of a table row (>= 1).  k_new / v_new [B,Hkv,D] or both NULL: stored *
  *     at position lens[b] and attended to as well.  A sequence without a key     *
- *     gets zeros; lens[b] < 0 marks an unused row (zeros, nothing stored);       *
+ *     (or with scores of -inf alone) gets zeros; lens[b] < 0 marks an unused row (zeros, nothing stored);       *
  *     lens[b] > width * page counts as that; keys of a page outside [0, n_pages) *
  *     count as absent, and a new token whose page is outside, or whose position  *
  *     is behind the table, is neither stored nor attended to.                    *
@@ -828,7 +828,8 @@ int nsp_sample_rows(const nsp_sample_params* p, void* stream);
  *   dtype.  Training: fwd also fills stats [2][B,H,Tq] fp32 (NULL for inference); bwd reads out
  *   and stats, uses rows [3][B,H,Tq rounded up to 64] fp32 as scratch and writes dq, dk, dv completely.
  *   dropout: element (b,h,i,j) is kept as nsp_attn_softmax_fwd keeps it: counter offset + ((b H + h) Tq + i) Tk + j.
- *   scale > 0; token strides (*_st) of more than one row below 2^24.  B, Tq or Tk == 0: NSP_OK, nothing is written (outputs and gradients that are not empty are zeros: the caller's). */
+ *   scale > 0; token strides (*_st) below 2^24 where there is more than one token.  B, Tq or Tk == 0: NSP_OK, nothing is written
+ *   (outputs and gradients that are not empty are zeros: the caller's). */
 typedef struct {
   const void* q; const void* k; const void* v; const void* dout;
   void* out; void* dq; void* dk; void* dv;

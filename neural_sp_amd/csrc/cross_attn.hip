@@ -15,12 +15,15 @@
 // The second operand of those products has the STREAMED row as contraction, i.e. wants a tile read across its rows: bf16 takes
 // it with the transposing LDS read (ds_read_b64_tr_b16), fp32 holds one contraction element per lane and instruction and
 // just picks the row.
-// The softmax is kept as its maximum (log2 domain) and the reciprocal of its sum, both fp32; backward recomputes P from them.
+// The softmax is kept as the forward pass's reference (log2 domain; the row's maximum or up to 8 below it, see there) and the
+// reciprocal of the sum that goes with it, both fp32; backward recomputes P from them.
 // bf16 roundings inside: P resp. dS, once each, as operands of the second products; with the outputs' own rounding the results are
 // 1.2 (out) to 1.5 times (dQ) as far from exact as a rounding of the exact result.  (Two bf16 parts for dS bring dQ to 1.2 and cost
 // 36 us of the 410 us of the largest measured call.)  Sums, statistics and D are fp32.
 // A row without a visible key is uniform over all Tk keys, as with the finite mask value of attn_softmax_fwd, and passes no
-// gradient through its scores.  Keys behind klens are never read.
+// gradient through its scores.  Keys behind klens are never read.  What is not there (dimensions between the head size and the
+// kernel's width, rows behind the last of a tile) enters as zeros on both sides, so infinities stay what the formulas make of them:
+// a key with a score of -inf has no probability, an infinite value makes infinite sums.
 #include "attn_frag.h"
 #include <type_traits>
 
@@ -29,7 +32,7 @@ namespace {
 struct XArgs {
   const void *q, *k, *v, *dout;
   void *out, *dq, *dk, *dv;
-  float* stats;        // [2][B,H,Tq]: maximum, 1 / sum
+  float* stats;        // [2][B,H,Tq]: the exponents' reference, 1 / sum
   float* rows;         // [3][B,H,Tq rounded up to 64]: what dK / dV need of every query, from the dQ kernel
   const int* klens;
   int B, H, Hkv, D, Tq, Tk;

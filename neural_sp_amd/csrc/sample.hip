@@ -82,7 +82,8 @@ struct RowScale {
   }
 };
 // The mass of a logit: exp(d) x 2^44 rounded to a whole number, d = (x - xmax) / T <= 0; relative error of the exponential below
-// 2^-47.  exp(d) = 2^n exp(f), |f| <= ln 2 / 2, Taylor to the 11th power; n and the final rounding come from additions of
+// 2^-47.  exp(d) = 2^n exp(f), |f| <= ln 2 / 2 (f = d - n ln 2 with ln 2 in two parts: Cody and Waite's reduction), the Taylor
+// polynomial of the 11th degree; n and the final rounding come from additions of
 // 1.5 x 2^52 and 2^52, whose low bits then are the whole number (gfx950 has no conversion from 64-bit floats to 64-bit integers).
 __device__ __forceinline__ u64 sample_mass(float x, const RowScale& r) {
   const double d = x == r.xmax ? 0. : ((double)x - (double)r.xmax) * r.inv_t;

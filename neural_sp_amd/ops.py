@@ -2307,16 +2307,16 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, k_new=None, v_new=No
     """Attention of one new token per sequence over a paged key / value cache (inference: a gradient that reaches the result is an
     error, and so are dual tensors).
 
-    q `[B,H,d]`; k_pages / v_pages `[n_pages,Hkv,page,d]` (any strides with a contiguous last dimension; H a multiple of
-    Hkv: query head h reads key head h // (H / Hkv)); block_table int32 `[B,pages]`: page of positions page*i ..; lens int32
+    q `[B,H,d]`; k_pages / v_pages `[n_pages,Hkv,page,d]` (contiguous last dimension, other strides multiples of 8
+    elements, 16-byte aligned; H a multiple of Hkv: query head h reads key head h // (H / Hkv)); block_table int32 `[B,pages]`: page of positions page*i ..; lens int32
     `[B]`: keys in the cache.  All fp32 or all bf16 -> `[B,H,d]` of that type, softmax(scale q k^T) v with scale = d^-1/2
     by default.  k_new / v_new `[B,Hkv,d]`: the new tokens' own keys and values, stored at position lens[b] in the same
     launch and attended to as well (`lens` itself is left to the caller).
 
-    A sequence without any key gets zeros.  lens[b] < 0 marks an unused row of a padded batch (zeros, nothing stored).
-    Table entries behind a sequence's last page are not read; an entry outside [0, n_pages) is an absent page: its keys do
-    not count and a new token that would lie there, or behind the table, is neither stored nor attended to.  No two rows may
-    share the page that a new token is stored to."""
+    A sequence without any key gets zeros, and so does one whose scores are all -inf.  lens[b] < 0 marks an unused row of a padded
+    batch (zeros, nothing stored).  What table entries behind a sequence's last page hold does not matter; an entry outside
+    [0, n_pages) is an absent page: its keys do not count and a new token that would lie there, or behind the table, is neither
+    stored nor attended to.  No two rows may share the page that a new token is stored to."""
     _require_device(q)
     dev = q.get_device()
     if k_pages.get_device() != dev or v_pages.get_device() != dev or block_table.get_device() != dev or lens.get_device() != dev:
@@ -2508,12 +2508,13 @@ def _cross_plan(q, k, v, klens, scale, dropout_p):
 
 def cross_attention(q, k, v, klens=None, scale=None, dropout_p=0.0):
     """Attention of target tokens over encoder states of another length: q `[B,Tq,H,d]`, k / v `[B,Tk,Hkv,d]` (query head h reads
-    key head h // (H / Hkv)), all fp32 or all bf16, any strides -> `[B,Tq,H,d]` of that type.  Differentiable in q, k and v
-    (once); gradients of shared heads are summed in fp32 and rounded once.
+    key head h // (H / Hkv)), all fp32 or all bf16, any strides (what the kernels do not read as it lies is copied) -> `[B,Tq,H,d]`
+    of that type.  Differentiable in q, k and v (once, not in forward mode); gradients of shared heads are summed in fp32 and
+    rounded once.
 
     Key j is visible to the queries of row b if j < klens[b] (int32 `[B]`; None: all); a row without a visible key averages
     all Tk values and passes no gradient through its scores, as AttentionFn does with its finite mask.  What lies behind
-    klens[b] in k and v is not read.  scale > 0, d^-1/2 by default.  dropout_p: dropout of the probabilities with a mask of its
+    klens[b] in k and v is not read.  A key with a score of -inf has no probability; a row of such scores alone is NaN.  scale > 0, d^-1/2 by default.  dropout_p: dropout of the probabilities with a mask of its
     own site (next_dropout_seed), regenerated in backward; a captured call repeats its mask with every replay.  A backward pass is
     captured on leaves of its own (detached ones): an eager graph that is alive ties its leaves to the stream it ran on.
 
