@@ -677,3 +677,12 @@ def dropout_widths_case(ops, dev, dtype, B, H, Hkv, Tq, Tk, D, klens, p=0.25, se
 DROPOUT_WIDTHS = [dict(B=2, H=2, Hkv=2, Tq=67, Tk=201, D=64, klens=[201, 139]), dict(B=1, H=4, Hkv=2, Tq=131, Tk=67, D=32, klens=[66]),
                   dict(B=1, H=2, Hkv=1, Tq=67, Tk=203, D=128, klens=[203]), dict(B=1, H=2, Hkv=2, Tq=5, Tk=71, D=72, klens=[70]),
                   dict(B=2, H=3, Hkv=1, Tq=70, Tk=69, D=64, klens=[1, 69])]
+
+
+# the kernels for rows that LDS holds with their masses, without them, and not at all, with and without settings
+SAMPLE_WIDE = [(V, kw) for V in (9000, 12000, 31000) for kw in (dict(), dict(tp=.9), dict(k=40, t=.7), dict(mp=.05))]
+
+
+def wide_case(ops, dev, dtype, V, kw):
+    x = torch.randn(2, V + 1, generator=torch.Generator().manual_seed(V)).mul_(3).to(dtype)[:, 1:]
+    sample_case(ops, dev, x, [0.25, 0.75], **kw)

@@ -300,3 +300,9 @@ def test_paged_attention_of_more_pages_than_an_int_counts(emu, page):
 @pytest.mark.parametrize('a', C.DROPOUT_WIDTHS, ids=str)
 def test_cross_attention_dropout_widths(emu, dtype, a):
     C.dropout_widths_case(emu, 'cpu', dtype, **a)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('V,kw', C.SAMPLE_WIDE, ids=str)
+def test_sample_rows_wide(emu, dtype, V, kw):
+    C.wide_case(emu, 'cpu', dtype, V, kw)

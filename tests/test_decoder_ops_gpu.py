@@ -330,3 +330,35 @@ def test_paged_attention_of_more_pages_than_an_int_counts(ops, page):
 @pytest.mark.parametrize('a', C.DROPOUT_WIDTHS, ids=str)
 def test_cross_attention_dropout_widths(ops, dtype, a):
     C.dropout_widths_case(ops, DEV, dtype, **a)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('V,kw', C.SAMPLE_WIDE, ids=str)
+def test_sample_rows_wide(ops, dtype, V, kw):
+    C.wide_case(ops, DEV, dtype, V, kw)
+
+
+def test_captured_calls_of_large_shared_memory_and_split_keys(ops):
+    """sampling from long rows (more LDS than a launch has without asking), decoding over split keys: captured before their first
+    eager call of these sizes, replayed with new inputs"""
+    g = torch.Generator().manual_seed(11)
+    x = [torch.randn(5, V, generator=g).to(DEV) for V in (10007, 29000, 33001)]
+    u = torch.rand(5, generator=g).to(DEV)
+    q, k, v = (torch.randn(2, t, 4, 72, generator=g).to(BF).to(DEV) for t in (1, 1777, 1777))
+    lens = torch.tensor([1777, 901], dtype=torch.int32, device=DEV)
+
+    def run():
+        return [ops.sample_rows(y, u, 0.8, 300, 0.9) for y in x] + [ops.sample_rows(x[0], u), ops.cross_attention(q, k, v, lens)]
+    ops.sample_rows(x[0][:, :10], u)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for i in range(4):
+        for t in x + [u, q]:
+            t.copy_(torch.rand(t.shape, generator=g))
+        lens.copy_(torch.tensor([1777 - 400 * i, 5 * i], dtype=torch.int32))
+        graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
