@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256) void decode_attn_kernel(const DecodeArgs p) {
   const int rr = row0 + q;
   if (p.nsplit == 1) {
     T* dst = reinterpret_cast<T*>(p.out) + (((long long)b * p.Tq + rr / G) * p.H + hkv * G + rr % G) * p.D;
-    const float inv = MODE != CONTIG && L == 0.f ? 0.f : 1.f / L;     // no key at all: zeros (over states L = 0 is not that)
+    const float inv = (MODE != CONTIG || p.cap == 0) && L == 0.f ? 0.f : 1.f / L;     // no key at all: zeros
 #pragma unroll
     for (int j = 0; j < VW; ++j)
       if (d0 + j < p.D) dst[d0 + j] = E::from_f32(acc[j] * inv);

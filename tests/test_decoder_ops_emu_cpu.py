@@ -306,3 +306,13 @@ def test_cross_attention_dropout_widths(emu, dtype, a):
 @pytest.mark.parametrize('V,kw', C.SAMPLE_WIDE, ids=str)
 def test_sample_rows_wide(emu, dtype, V, kw):
     C.wide_case(emu, 'cpu', dtype, V, kw)
+
+
+def test_c_entry_of_decode_attention_over_no_state(emu):
+    """table == NULL, width 0: there is no key, so zeros"""
+    from neural_sp_amd import _lib
+    q, out = torch.ones(2, 1, 2, 16), torch.full((2, 1, 2, 16), 7.0)
+    tail, floats = emu._decode_tail(2, 2, 2, 16, 1, 1, 0, 0, F32, (32, 32, 16), (0, 32, 16), (0, 32, 16), (0, 0, 0, 0), 0.25)
+    assert floats == 0
+    assert _lib.lib().nsp_decode_attn(emu._DECODE_PTRS(q.data_ptr(), out.data_ptr(), 0, 0, 0, 0, 0, 0, 0) + tail, 0) == 0
+    assert not out.any()
